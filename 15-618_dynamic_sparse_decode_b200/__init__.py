@@ -2,7 +2,9 @@
 
 The product is the C ABI in ``include/dsd_b200.h`` (``libdsd_b200.so``, built
 from ``csrc/``) and the C++ drop-in host API over it.  This module is the
-ctypes binding the tests and ``bench.py`` use.  It loads the in-tree library
+ctypes binding the tests and ``bench.py`` use; ``ScaledKVCache`` and
+``RotaryTable`` (the scaled 8-bit paged cache, over torch tensors) come from
+``scaled_cache``.  It loads the in-tree library
 and fails loudly when it is missing: there is no CPU fallback.
 
 The directory name is not a Python identifier, so import it with
@@ -22,6 +24,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libdsd_b200.so")
 DSD_OK, DSD_EINVAL, DSD_ERANGE, DSD_ENOMEM, DSD_ECUDA, DSD_ETIMEOUT, DSD_EUNAVAILABLE = range(7)
 OUTPUT_NONE, OUTPUT_OUTPUTS, OUTPUT_DEBUG = 0, 1, 2
 KV_F32, KV_BF16, KV_FP8 = 0, 1, 2
+KV_FP8_SCALED, KV_I8_SCALED = 3, 4   # ScaledKVCache
 
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _F32P = ctypes.POINTER(ctypes.c_float)
@@ -49,6 +52,38 @@ class TransferStats(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in
                 ("h2d_bytes", "d2h_bytes", "h2d_calls", "d2h_calls", "h2d_large_calls",
                  "d2h_large_calls")]
+
+
+class ScaledCacheDesc(ctypes.Structure):
+    """dsd_scaled_cache."""
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("kv_format", "num_pages", "page_size", "num_kv_heads", "head_dim", "block_tokens")] + [
+        (n, _VP) for n in ("k_codes", "v_codes", "k_scales", "v_scales")] + [
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3)]
+
+
+class ScaledAppendArgs(ctypes.Structure):
+    """dsd_scaled_append_args."""
+    _fields_ = [("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("total_tokens", ctypes.c_int32),
+                ("max_pages_per_request", ctypes.c_int32), ("k", _VP), ("v", _VP),
+                ("k_stride", ctypes.c_int64 * 2), ("v_stride", ctypes.c_int64 * 2),
+                ("token_offsets", _VP), ("seq_lens", _VP), ("page_table", _VP),
+                ("page_table_stride", ctypes.c_int64), ("cos", _VP), ("sin", _VP), ("positions", _VP),
+                ("rotary_positions", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("q", _VP), ("q_out", _VP),
+                ("q_stride", ctypes.c_int64 * 2), ("q_out_stride", ctypes.c_int64 * 2),
+                ("token_counts", _VP), ("status", _VP)]
+
+
+class ScaledAttentionArgs(ctypes.Structure):
+    """dsd_scaled_attention_args."""
+    _fields_ = [("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("total_queries", ctypes.c_int32),
+                ("num_q_heads", ctypes.c_int32), ("q", _VP), ("out", _VP), ("lse", _VP),
+                ("q_stride", ctypes.c_int64 * 2), ("out_stride", ctypes.c_int64 * 2),
+                ("q_offsets", _VP), ("lens", _VP), ("page_table", _VP), ("page_table_stride", ctypes.c_int64),
+                ("page_counts", _VP), ("max_pages_per_request", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("workspace", _VP),
+                ("workspace_bytes", ctypes.c_int64), ("status", _VP)]
 
 
 # (name, restype, argtypes) of every exported entry point, in header order.
@@ -108,6 +143,13 @@ SIGNATURES = [
     ("dsd_decode_batch_noalloc", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ModelConfig),
                                                 ctypes.c_int, ctypes.c_int, _I32P, _VP, _VP,
                                                 _VP, _VP, _VP, _VP, _VP, _VP]),
+    ("dsd_scaled_append", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ScaledCacheDesc),
+                                         ctypes.POINTER(ScaledAppendArgs), _VP]),
+    ("dsd_scaled_attention_workspace", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ScaledCacheDesc),
+                                                      ctypes.POINTER(ScaledAttentionArgs),
+                                                      ctypes.POINTER(ctypes.c_int64)]),
+    ("dsd_scaled_attention", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ScaledCacheDesc),
+                                            ctypes.POINTER(ScaledAttentionArgs), _VP]),
 ]
 
 _lib = None
@@ -195,6 +237,14 @@ def generate_normal_host(seed: int, kind: int, first_index: int, count: int) -> 
 
 def normal_index(request: int, token: int, ept: int, element: int = 0) -> int:
     return (request << 40) + token * ept + element
+
+
+def __getattr__(name):
+    # the torch binding of the scaled cache, imported on first use: the rest needs numpy alone
+    if name in ("ScaledKVCache", "RotaryTable"):
+        from . import scaled_cache
+        return getattr(scaled_cache, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class SparseDecodeContext:

@@ -21,8 +21,12 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB = os.path.join(PKG, "libdsd_b200.so")
 
-SOURCES = ["dsd_capi.cu"]
-HEADERS = ["dsd_kernels.cuh"]
+SOURCES = ["dsd_capi.cu", "dsd_scaled_capi.cu"]
+HEADERS = ["dsd_internal.h", "dsd_kernels.cuh", "dsd_scaled_common.cuh", "dsd_scaled_append.cuh",
+           "dsd_scaled_attn.cuh"]
+# headers of one source only: the other need not be compiled again for them
+ONLY = {"dsd_kernels.cuh": "dsd_capi.cu", "dsd_scaled_common.cuh": "dsd_scaled_capi.cu",
+        "dsd_scaled_append.cuh": "dsd_scaled_capi.cu", "dsd_scaled_attn.cuh": "dsd_scaled_capi.cu"}
 
 
 def _newer(target: str, deps: list[str]) -> bool:
@@ -35,16 +39,27 @@ def _newer(target: str, deps: list[str]) -> bool:
 def build_library(force: bool = False, verbose: bool = False, out: str = LIB,
                   defines: tuple = ()) -> str:
     """nvcc the C ABI + kernels into `out` (extra -D `defines` for experiments)."""
-    deps = [os.path.join(CSRC, s) for s in SOURCES + HEADERS] + [os.path.join(INCLUDE, "dsd_b200.h")]
-    if not force and _newer(out, deps):
-        return out
-    cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
-           *[f"-D{d}" for d in defines],
-           f"-I{INCLUDE}", f"-I{CSRC}", "-o", out, *[os.path.join(CSRC, s) for s in SOURCES]]
+    flags = [*ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+             *[f"-D{d}" for d in defines], f"-I{INCLUDE}", f"-I{CSRC}"]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+        flags.insert(0, "-Xptxas=-v")
+    objects, jobs = [], []
+    os.makedirs(os.path.join(PKG, "build"), exist_ok=True)
+    for src in SOURCES:
+        deps = [os.path.join(CSRC, src), os.path.join(INCLUDE, "dsd_b200.h")]
+        deps += [os.path.join(CSRC, h) for h in HEADERS if ONLY.get(h, src) == src]
+        obj = os.path.join(PKG, "build", os.path.basename(out) + "." + src + ".o")
+        objects.append(obj)
+        if force or defines or not _newer(obj, deps):
+            cmd = [NVCC, *flags, "-c", "-o", obj, os.path.join(CSRC, src)]
+            if verbose:
+                print(" ".join(cmd))
+            jobs.append((cmd, subprocess.Popen(cmd)))
+    for cmd, job in jobs:
+        if job.wait():
+            raise subprocess.CalledProcessError(job.returncode, cmd)
+    if jobs or not _newer(out, objects):
+        subprocess.run([NVCC, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", out, *objects], check=True)
     return out
 
 

@@ -1,0 +1,366 @@
+// dsd_scaled_capi.cu -- C ABI of the scaled 8-bit paged cache (include/dsd_b200.h):
+// argument checks, the choice of kernel and the launches.  Stateless apart from
+// per-device attributes that are looked up once.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+#include <string>
+
+#include "dsd_b200.h"
+#include "dsd_internal.h"
+#include "dsd_scaled_append.cuh"
+#include "dsd_scaled_attn.cuh"
+
+namespace {
+
+using namespace dsd_internal;
+using dsds::AppendParams;
+using dsds::AttnParams;
+
+constexpr int kMaxDevices = 64;
+
+// What a launch needs to know of a device, looked up on its first call.
+struct Device {
+  bool ready = false;
+  int sms = 0;
+};
+std::mutex g_mutex;
+Device g_devices[kMaxDevices];
+
+void SetSimpleAttributes();
+
+const Device& DeviceOf(int device) {
+  if (device < 0 || device >= kMaxDevices) Fail(DSD_EINVAL, "device index out of range");
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Device& d = g_devices[device];
+  if (!d.ready) {
+    int major = 0;
+    Check(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device), "device");
+    if (major != 10) Fail(DSD_EUNAVAILABLE, "no sm_100 GPU at this device index");
+    Check(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device), "SM count");
+    SetSimpleAttributes();
+    d.ready = true;
+  }
+  return d;
+}
+
+bool Aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+int ElemBytes(int dtype) { return dtype == DSD_TYPE_F32 ? 4 : 2; }
+
+void CheckCache(const dsd_scaled_cache* c) {
+  if (!c) Fail(DSD_EINVAL, "null cache");
+  if (c->kv_format != DSD_KV_FP8_SCALED && c->kv_format != DSD_KV_I8_SCALED)
+    Fail(DSD_EINVAL, "kv_format must be DSD_KV_FP8_SCALED or DSD_KV_I8_SCALED");
+  if (c->num_pages <= 0) Fail(DSD_EINVAL, "num_pages must be positive");
+  if (c->page_size < 1 || c->page_size > 4096) Fail(DSD_EINVAL, "page_size must be in [1, 4096]");
+  if (c->num_kv_heads < 1 || c->num_kv_heads > 1024) Fail(DSD_EINVAL, "num_kv_heads must be in [1, 1024]");
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8)
+    Fail(DSD_EINVAL, "head_dim must be a multiple of 8 in [8, 256]");
+  if (c->block_tokens < 1 || c->block_tokens > 256 || c->page_size % c->block_tokens)
+    Fail(DSD_EINVAL, "block_tokens must divide page_size and be at most 256");
+  for (int i = 0; i < 3; ++i)
+    if (c->k_stride[i] <= 0 || c->v_stride[i] <= 0) Fail(DSD_EINVAL, "cache strides must be positive");
+}
+
+void CheckCachePointers(const dsd_scaled_cache* c) {
+  if (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) Fail(DSD_EINVAL, "null cache array");
+  if (!Aligned(c->k_scales, 4) || !Aligned(c->v_scales, 4)) Fail(DSD_EINVAL, "scales must be 4-byte aligned");
+}
+
+void CheckType(int dtype) {
+  if (dtype != DSD_TYPE_F32 && dtype != DSD_TYPE_BF16 && dtype != DSD_TYPE_F16)
+    Fail(DSD_EINVAL, "dtype must be DSD_TYPE_F32, DSD_TYPE_BF16 or DSD_TYPE_F16");
+}
+
+// ------------------------------------------------------------------ append
+
+template <typename T, bool I8>
+void LaunchAppendAs(const AppendParams& p, int ve, dim3 grid, cudaStream_t s) {
+  if (ve == 8) dsds::append_kernel<T, I8, 8><<<grid, dsds::kAppendThreads, 0, s>>>(p);
+  else dsds::append_kernel<T, I8, 1><<<grid, dsds::kAppendThreads, 0, s>>>(p);
+}
+
+template <typename T>
+void LaunchAppend(const AppendParams& p, bool i8, int ve, dim3 grid, cudaStream_t s) {
+  if (i8) LaunchAppendAs<T, true>(p, ve, grid, s);
+  else LaunchAppendAs<T, false>(p, ve, grid, s);
+}
+
+void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args* a, cudaStream_t s) {
+  NvtxRange nvtx("dsd_scaled_append");
+  CheckCache(c);
+  if (!a) Fail(DSD_EINVAL, "null arguments");
+  CheckType(a->dtype);
+  if (a->batch < 0 || a->total_tokens < 0) Fail(DSD_EINVAL, "batch and total_tokens must not be negative");
+  if (!a->token_offsets && a->total_tokens != a->batch)
+    Fail(DSD_EINVAL, "without token_offsets every request has one token: total_tokens must equal batch");
+  if (a->num_q_heads < 0 || a->num_q_heads > 4096) Fail(DSD_EINVAL, "num_q_heads must be in [0, 4096]");
+  if (a->max_pages_per_request < 0 || a->page_table_stride < 0)
+    Fail(DSD_EINVAL, "page-table sizes must not be negative");
+  if ((a->cos == nullptr) != (a->sin == nullptr)) Fail(DSD_EINVAL, "cos and sin come together");
+  if (a->cos) {
+    if (a->rotary_dim < 2 || a->rotary_dim % 2 || a->rotary_dim > c->head_dim)
+      Fail(DSD_EINVAL, "rotary_dim must be even, in [2, head_dim]");
+    if (a->rotary_positions <= 0) Fail(DSD_EINVAL, "rotary_positions must be positive");
+    if (!Aligned(a->cos, 4) || !Aligned(a->sin, 4)) Fail(DSD_EINVAL, "cos and sin must be 4-byte aligned");
+  }
+  if (a->batch == 0 || a->total_tokens == 0) return;
+  CheckCachePointers(c);
+  if (!a->k || !a->v || !a->seq_lens || !a->page_table) Fail(DSD_EINVAL, "null device array");
+  if (a->num_q_heads && (!a->q || !a->q_out)) Fail(DSD_EINVAL, "num_q_heads > 0 needs q and q_out");
+  const int eb = ElemBytes(a->dtype);
+  const void* rows[] = {a->k, a->v, a->num_q_heads ? a->q : a->k, a->num_q_heads ? a->q_out : a->k};
+  const int64_t* strides[] = {a->k_stride, a->v_stride, a->num_q_heads ? a->q_stride : a->k_stride,
+                              a->num_q_heads ? a->q_out_stride : a->k_stride};
+  for (int i = 0; i < 4; ++i) {
+    if (!Aligned(rows[i], eb)) Fail(DSD_EINVAL, "k, v, q and q_out must be aligned to their type");
+    if (strides[i][0] < 0 || strides[i][1] < 0) Fail(DSD_EINVAL, "row strides must not be negative");
+  }
+
+  // 8-element accesses where every row starts on their boundary, else single
+  // elements (measured on unaligned rows only: no other path takes those)
+  const int rd = a->cos ? a->rotary_dim : 0;
+  bool wide = rd % 16 == 0;
+  for (int i = 0; i < 4; ++i)
+    wide = wide && Aligned(rows[i], 16) && strides[i][0] % 8 == 0 && strides[i][1] % 8 == 0;
+  if (a->cos) wide = wide && Aligned(a->cos, 16) && Aligned(a->sin, 16);
+  wide = wide && Aligned(c->k_codes, 8) && Aligned(c->v_codes, 8);
+  for (int i = 0; i < 3; ++i) wide = wide && c->k_stride[i] % 8 == 0 && c->v_stride[i] % 8 == 0;
+  const int ve = wide ? 8 : 1;
+
+  DeviceGuard guard(device);
+  const Device& dev = DeviceOf(device);
+  AppendParams p{};
+  p.k = static_cast<uint8_t*>(c->k_codes);
+  p.v = static_cast<uint8_t*>(c->v_codes);
+  p.ks = c->k_scales;
+  p.vs = c->v_scales;
+  for (int i = 0; i < 3; ++i) {
+    p.kst[i] = c->k_stride[i];
+    p.vst[i] = c->v_stride[i];
+  }
+  p.num_pages = c->num_pages;
+  p.P = c->page_size;
+  p.Hk = c->num_kv_heads;
+  p.D = c->head_dim;
+  p.bt = c->block_tokens;
+  p.nblk = c->page_size / c->block_tokens;
+  p.kin = a->k;
+  p.vin = a->v;
+  p.qin = a->q;
+  p.qout = a->q_out;
+  for (int i = 0; i < 2; ++i) {
+    p.kin_st[i] = a->k_stride[i];
+    p.vin_st[i] = a->v_stride[i];
+    p.qin_st[i] = a->q_stride[i];
+    p.qout_st[i] = a->q_out_stride[i];
+  }
+  p.batch = a->batch;
+  p.total = a->total_tokens;
+  p.max_pages = a->max_pages_per_request;
+  p.Hq = a->num_q_heads;
+  p.off = a->token_offsets;
+  p.lens = a->seq_lens;
+  p.table = a->page_table;
+  p.table_stride = a->page_table_stride;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.positions = a->positions;
+  p.rot_positions = a->rotary_positions;
+  p.rd = rd;
+  p.interleaved = a->interleaved != 0;
+  p.counts = a->token_counts;
+  p.status = a->status;
+  p.slots = (p.D + 2 * ve - 1) / (2 * ve);
+  const int64_t units = p.off ? int64_t(p.total) / p.bt + 2 * int64_t(p.batch) : p.batch;
+  if (units > INT32_MAX) Fail(DSD_EINVAL, "too many tokens for one call");
+  // a team's lanes keep the whole block in registers where 8 warps can
+  const int block_slots = (p.off ? std::min(p.bt, p.total) : 1) * p.slots;
+  p.team = 1;
+  while (p.team < 8 && p.team * 32 * dsds::kAppendKeep < block_slots) p.team *= 2;
+  const int teams = dsds::kAppendThreads / 32 / p.team;
+  const int items = 2 * p.Hk + p.Hq, rounds = (items + teams - 1) / teams;
+  const int64_t want = 8ll * dev.sms;
+  const int y = int(std::min<int64_t>(std::min(rounds, 65535), std::max<int64_t>(1, (want + units - 1) / units)));
+  const dim3 grid{static_cast<unsigned>(units), static_cast<unsigned>(y), 1};
+  const bool i8 = c->kv_format == DSD_KV_I8_SCALED;
+  if (a->dtype == DSD_TYPE_F32) LaunchAppend<float>(p, i8, ve, grid, s);
+  else if (a->dtype == DSD_TYPE_BF16) LaunchAppend<__nv_bfloat16>(p, i8, ve, grid, s);
+  else LaunchAppend<__half>(p, i8, ve, grid, s);
+  Check(cudaGetLastError(), "append launch");
+}
+
+// --------------------------------------------------------------- attention
+
+constexpr int kSimpleMaxSmem = 4 * (8 * 256 + 8 * dsds::kTile + 4 * dsds::kTile + 24 + dsds::kMaxBatch) + 64;
+
+template <bool I8, int R>
+void SetSimple() {
+  Check(cudaFuncSetAttribute(dsds::attn_simple_kernel<I8, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kSimpleMaxSmem), "shared memory attribute");
+}
+void SetSimpleAttributes() {
+  SetSimple<false, 1>(); SetSimple<false, 2>(); SetSimple<false, 4>(); SetSimple<false, 8>();
+  SetSimple<true, 1>(); SetSimple<true, 2>(); SetSimple<true, 4>(); SetSimple<true, 8>();
+}
+
+template <bool I8>
+void LaunchSimple(const AttnParams& p, cudaStream_t s) {
+  const size_t smem = dsds::simple_smem(p.R, p.D, p.batch);
+  switch (p.R) {
+    case 1: dsds::attn_simple_kernel<I8, 1><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
+    case 2: dsds::attn_simple_kernel<I8, 2><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
+    case 4: dsds::attn_simple_kernel<I8, 4><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
+    default: dsds::attn_simple_kernel<I8, 8><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
+  }
+}
+
+struct AttnPlan {
+  int R = 1, ncta = 0;
+  int64_t ml_at = 0, o_at = 0, bytes = 0;   // workspace: meta, then ml, then O
+};
+
+AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_scaled_attention_args* a) {
+  AttnPlan pl;
+  const int group = a->num_q_heads / c->num_kv_heads;
+  // query rows of a request: exact for one query each, the average otherwise
+  const int64_t queries = a->q_offsets ? (int64_t(a->total_queries) + a->batch - 1) / a->batch : 1;
+  const int64_t rows = queries * group;
+  while (pl.R < 8 && pl.R < rows) pl.R *= 2;
+  pl.ncta = 8 * dev.sms;
+  pl.ml_at = (int64_t(pl.ncta) * 16 + 255) / 256 * 256;
+  pl.o_at = pl.ml_at + (int64_t(pl.ncta) * 2 * pl.R * 8 + 255) / 256 * 256;
+  pl.bytes = pl.o_at + int64_t(pl.ncta) * 2 * pl.R * c->head_dim * 4;
+  return pl;
+}
+
+void CheckAttention(const dsd_scaled_cache* c, const dsd_scaled_attention_args* a) {
+  CheckCache(c);
+  if (!a) Fail(DSD_EINVAL, "null arguments");
+  CheckType(a->dtype);
+  if (a->batch < 0 || a->batch > dsds::kMaxBatch) Fail(DSD_EINVAL, "batch must be in [0, 4096]");
+  if (a->total_queries < 0) Fail(DSD_EINVAL, "total_queries must not be negative");
+  if (!a->q_offsets && a->total_queries != a->batch)
+    Fail(DSD_EINVAL, "without q_offsets every request has one query: total_queries must equal batch");
+  if (a->num_q_heads < 1 || a->num_q_heads > 4096 || a->num_q_heads % c->num_kv_heads)
+    Fail(DSD_EINVAL, "num_q_heads must be a multiple of num_kv_heads, at most 4096");
+  if (int64_t(a->total_queries) * a->num_q_heads > INT32_MAX) Fail(DSD_EINVAL, "too many query rows for one call");
+  if (a->max_pages_per_request < 0 || a->page_table_stride < 0)
+    Fail(DSD_EINVAL, "page-table sizes must not be negative");
+  if (a->window < 0) Fail(DSD_EINVAL, "window must not be negative");
+  if (a->page_counts && (a->causal || a->window))
+    Fail(DSD_EINVAL, "a page list has no order: causal and window must be 0 with page_counts");
+  if (!std::isfinite(a->scale)) Fail(DSD_EINVAL, "scale must be finite");
+}
+
+void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention_args* a, cudaStream_t s) {
+  NvtxRange nvtx("dsd_scaled_attention");
+  CheckAttention(c, a);
+  if (a->batch == 0 || a->total_queries == 0) return;
+  CheckCachePointers(c);
+  if (!a->q || !a->out || !a->lens || !a->page_table) Fail(DSD_EINVAL, "null device array");
+  const int eb = ElemBytes(a->dtype);
+  if (!Aligned(a->q, eb) || !Aligned(a->out, eb) || !Aligned(a->lse, 4))
+    Fail(DSD_EINVAL, "q, out and lse must be aligned to their type");
+  for (int i = 0; i < 2; ++i)
+    if (a->q_stride[i] < 0 || a->out_stride[i] < 0) Fail(DSD_EINVAL, "row strides must not be negative");
+  DeviceGuard guard(device);
+  const Device& dev = DeviceOf(device);
+  const AttnPlan pl = PlanAttention(dev, c, a);
+  if (!a->workspace || !Aligned(a->workspace, 16) || a->workspace_bytes < pl.bytes)
+    Fail(DSD_EINVAL, "workspace must be 16-byte aligned with at least " + std::to_string(pl.bytes) + " bytes");
+
+  AttnParams p{};
+  p.k = static_cast<const uint8_t*>(c->k_codes);
+  p.v = static_cast<const uint8_t*>(c->v_codes);
+  p.ks = c->k_scales;
+  p.vs = c->v_scales;
+  for (int i = 0; i < 3; ++i) {
+    p.kst[i] = c->k_stride[i];
+    p.vst[i] = c->v_stride[i];
+  }
+  p.num_pages = c->num_pages;
+  p.P = c->page_size;
+  p.Hk = c->num_kv_heads;
+  p.D = c->head_dim;
+  p.bt = c->block_tokens;
+  p.nblk = c->page_size / c->block_tokens;
+  p.q = a->q;
+  p.out = a->out;
+  p.lse = a->lse;
+  for (int i = 0; i < 2; ++i) {
+    p.qst[i] = a->q_stride[i];
+    p.ost[i] = a->out_stride[i];
+  }
+  p.dtype = a->dtype;
+  p.batch = a->batch;
+  p.total_q = a->total_queries;
+  p.H = a->num_q_heads;
+  p.G = a->num_q_heads / c->num_kv_heads;
+  p.q_off = a->q_offsets;
+  p.lens = a->lens;
+  p.table = a->page_table;
+  p.table_stride = a->page_table_stride;
+  p.max_pages = a->max_pages_per_request;
+  p.counts = a->page_counts;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.causal = a->causal != 0;
+  p.window = a->window;
+  p.status = a->status;
+  p.ppt = p.P <= dsds::kTile ? dsds::kTile / p.P : 0;
+  p.tpp = p.P <= dsds::kTile ? 0 : (p.P + dsds::kTile - 1) / dsds::kTile;
+  p.R = pl.R;
+  p.ncta = pl.ncta;
+  char* ws = static_cast<char*>(a->workspace);
+  p.meta = reinterpret_cast<int4*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + pl.ml_at);
+  p.part_o = reinterpret_cast<float*>(ws + pl.o_at);
+
+  if (c->kv_format == DSD_KV_I8_SCALED) LaunchSimple<true>(p, s);
+  else LaunchSimple<false>(p, s);
+  Check(cudaGetLastError(), "attention launch");
+
+  // the join may be scheduled while the last CTAs of the attention run; it waits
+  // for them before it reads
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(p.ncta), unsigned(std::min(p.R, 4)));
+  cfg.blockDim = dim3(unsigned(p.D <= 128 ? 128 : 256));
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  Check(cudaLaunchKernelEx(&cfg, dsds::combine_kernel, p), "combine launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsd_scaled_append(int device, const dsd_scaled_cache* cache, const dsd_scaled_append_args* args,
+                      void* stream) {
+  return Guard([&]() { Append(device, cache, args, static_cast<cudaStream_t>(stream)); });
+}
+
+int dsd_scaled_attention_workspace(int device, const dsd_scaled_cache* cache,
+                                   const dsd_scaled_attention_args* args, int64_t* bytes) {
+  return Guard([&]() {
+    CheckAttention(cache, args);
+    if (!bytes) Fail(DSD_EINVAL, "null result");
+    *bytes = 0;
+    if (args->batch == 0 || args->total_queries == 0) return;
+    DeviceGuard guard(device);
+    *bytes = PlanAttention(DeviceOf(device), cache, args).bytes;
+  });
+}
+
+int dsd_scaled_attention(int device, const dsd_scaled_cache* cache, const dsd_scaled_attention_args* args,
+                         void* stream) {
+  return Guard([&]() { Attention(device, cache, args, static_cast<cudaStream_t>(stream)); });
+}
+
+}  // extern "C"

@@ -1,0 +1,361 @@
+// dsd_scaled_common.cuh -- what the kernels of the scaled 8-bit paged cache share:
+// element conversions, the work split of the attention, its partial results and
+// their join.
+//
+// Attention splits the KEY axis: a unit is one request, one key head and R
+// consecutive query rows (row = query * group + head of the group); it walks the
+// tiles of up to 128 tokens that its rows see.  All units' tiles in a row form
+// one axis, which is cut into equal contiguous ranges, one per CTA, so that one
+// long request fills the machine and a ragged batch leaves no CTA idle.  A CTA
+// derives its range from the lengths on the device (no host knowledge of them,
+// so a captured graph follows them); a unit that spans CTAs leaves partial
+// results, at most two per CTA, which combine_kernel joins in tile order.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dsd_b200.h"
+
+namespace dsds {
+
+constexpr int kTile = 128;          // tokens of a tile at most
+constexpr int kMaxBatch = 4096;     // plan: one int per request in shared memory
+constexpr float kTinyScale = 5.421010862427522e-20f;  // 2^-64, see token_scale()
+
+struct AttnParams {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  long long kst[3], vst[3];
+  int num_pages, P, Hk, D, bt, nblk;
+  const void* q;
+  void* out;
+  float* lse;
+  long long qst[2], ost[2];
+  int dtype, batch, total_q, H, G;
+  const int* q_off;
+  const int* lens;
+  const int* table;
+  long long table_stride;
+  int max_pages;
+  const int* counts;
+  float scale_log2;   // scale * log2(e): logits are kept in powers of two
+  int causal, window;
+  int* status;
+  int ppt;            // pages per tile (page_size <= 128), else 0
+  int tpp;            // tiles per page (page_size > 128), else 0
+  int R;              // query rows of a unit
+  int ncta;
+  float* part_ml;     // [ncta][2][R][2]  running maximum (log2) and sum
+  float* part_o;      // [ncta][2][R][D]
+  int4* meta;         // [ncta]  unit a CTA leaves open: request, head, row tile, last CTA (-1: none)
+};
+
+__device__ __forceinline__ float load_elem(const void* p, long long i, int dtype) {
+  if (dtype == DSD_TYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == DSD_TYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_elem(void* p, long long i, int dtype, float x) {
+  if (dtype == DSD_TYPE_F32) static_cast<float*>(p)[i] = x;
+  else if (dtype == DSD_TYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+template <bool I8>
+__device__ __forceinline__ float code_value(uint8_t c) {
+  if constexpr (I8) return static_cast<float>(static_cast<int8_t>(c));
+  __nv_fp8_e4m3 f;
+  f.__x = c;
+  return static_cast<float>(f);
+}
+
+// One request as the kernel sees it, every number clamped to the arrays.
+struct Request {
+  int q0, nq, rows;   // first query row, queries, query rows (nq * group)
+  int len;            // tokens, or listed pages when page_counts is given
+};
+
+__device__ __forceinline__ Request request_of(const AttnParams& p, int b) {
+  Request r;
+  r.q0 = b;
+  r.nq = 1;
+  if (p.q_off) {
+    const int a = p.q_off[b], e = p.q_off[b + 1];
+    r.q0 = min(max(a, 0), p.total_q);
+    r.nq = min(max(e, r.q0), p.total_q) - r.q0;
+  }
+  r.rows = r.nq * p.G;
+  const long long most = p.counts ? p.max_pages : 1ll * p.max_pages * p.P;
+  r.len = static_cast<int>(min(max(static_cast<long long>(p.lens[b]), 0ll), most));
+  return r;
+}
+
+// Tiles that hold `tokens` tokens of a request, and the tile of token t.
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int tokens) {
+  if (p.tpp) return tokens / p.P * p.tpp + (tokens % p.P + kTile - 1) / kTile;
+  const int tt = p.ppt * p.P;
+  return (tokens + tt - 1) / tt;
+}
+__device__ __forceinline__ int tile_at(const AttnParams& p, int t) {
+  if (p.tpp) return t / p.P * p.tpp + t % p.P / kTile;
+  return t / (p.ppt * p.P);
+}
+
+// The tiles that row tile qt (R rows) sees: the first one and how many.
+struct Span { int first, n; };
+
+__device__ __forceinline__ Span span_of(const AttnParams& p, const Request& r, int qt) {
+  if (p.counts) return {0, p.tpp ? r.len * p.tpp : (r.len + p.ppt - 1) / p.ppt};
+  const long long base = static_cast<long long>(r.len) - r.nq;
+  const long long row0 = 1ll * qt * p.R, row1 = min(static_cast<long long>(r.rows), row0 + p.R) - 1;
+  long long hi = r.len, lo = 0;
+  if (p.causal) hi = min(hi, max(0ll, base + row1 / p.G + 1));
+  if (p.window) lo = max(0ll, base + row0 / p.G - p.window + 1);
+  if (lo >= hi) return {0, 0};
+  const int t0 = tile_at(p, static_cast<int>(lo));
+  return {t0, tiles_of(p, static_cast<int>(hi)) - t0};
+}
+
+// A unit without a tile still takes a slot of the axis: its rows get zeros.
+__device__ __forceinline__ int slots_of(const Span& s) { return max(1, s.n); }
+
+// Where a CTA stands: unit (b, h, qt), slot within the unit, slots left in its range.
+struct Walk {
+  int b, h, qt, slot;
+  long long at, left;   // global slot, slots left
+  long long total;
+};
+
+// Every thread of the CTA calls it; wb has room for p.batch ints, w is shared.
+template <int THREADS>
+__device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned bad = 0;
+  for (int b = p.q_off ? warp : tid; b < p.batch; b += p.q_off ? THREADS / 32 : THREADS) {
+    const Request r = request_of(p, b);
+    if (cta == 0 && p.status && (p.q_off == nullptr || lane == 0)) {
+      const long long most = p.counts ? p.max_pages : 1ll * p.max_pages * p.P;
+      if (p.lens[b] < 0) bad |= DSD_SCALED_BAD_LENGTH;
+      if (p.lens[b] > most) bad |= DSD_SCALED_BAD_PAGE;
+      if (p.q_off && (p.q_off[b] != r.q0 || p.q_off[b + 1] != r.q0 + r.nq)) bad |= DSD_SCALED_BAD_LENGTH;
+    }
+    const int qts = (r.rows + p.R - 1) / p.R;
+    if (!p.q_off) {
+      // one query: every row tile sees the same tokens
+      wb[b] = qts * slots_of(span_of(p, r, 0));
+    } else {
+      int sum = 0;
+      for (int qt = lane; qt < qts; qt += 32) sum += slots_of(span_of(p, r, qt));
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      if (lane == 0) wb[b] = sum;
+    }
+  }
+  if (bad) atomicOr(p.status, static_cast<int>(bad));
+  __syncthreads();
+  if (warp == 0) {
+    long long total = 0;
+    for (int b = lane; b < p.batch; b += 32) total += wb[b];
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+    total *= p.Hk;
+    // no CTA between the first and the last that works is without a slot
+    const long long parts = min(total, static_cast<long long>(p.ncta));
+    const long long lo = cta < parts ? total * cta / parts : 0, hi = cta < parts ? total * (cta + 1) / parts : 0;
+    Walk x{};
+    x.at = lo;
+    x.left = hi - lo;
+    x.total = total;
+    if (x.left > 0) {
+      long long before = 0;
+      for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const long long mine = b0 + lane < p.batch ? 1ll * wb[b0 + lane] * p.Hk : 0;
+        long long upto = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(~0u, upto, o);
+          if (lane >= o) upto += y;
+        }
+        const unsigned past = __ballot_sync(~0u, before + upto > lo);
+        if (past) {
+          const int l = __ffs(past) - 1;
+          x.b = b0 + l;
+          before += __shfl_sync(~0u, upto - mine, l);
+          break;
+        }
+        before += __shfl_sync(~0u, upto, 31);
+      }
+      const int w1 = wb[x.b];
+      const int rest = static_cast<int>((lo - before) % w1);
+      x.h = static_cast<int>((lo - before) / w1);
+      const Request r = request_of(p, x.b);
+      const int qts = (r.rows + p.R - 1) / p.R;
+      if (!p.q_off) {
+        const int per = w1 / qts;
+        x.qt = rest / per;
+        x.slot = rest % per;
+      } else {
+        int sum = 0;
+        for (int q0 = 0; q0 < qts; q0 += 32) {
+          const int mine = q0 + lane < qts ? slots_of(span_of(p, r, q0 + lane)) : 0;
+          int upto = mine;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(~0u, upto, o);
+            if (lane >= o) upto += y;
+          }
+          const unsigned past = __ballot_sync(~0u, sum + upto > rest);
+          if (past) {
+            const int l = __ffs(past) - 1;
+            x.qt = q0 + l;
+            x.slot = rest - sum - __shfl_sync(~0u, upto - mine, l);
+            break;
+          }
+          sum += __shfl_sync(~0u, upto, 31);
+        }
+      }
+    }
+    if (lane == 0) *w = x;
+  }
+  __syncthreads();
+}
+
+// To the first slot of the next unit.
+__device__ __forceinline__ void next_unit(const AttnParams& p, Request& r, Walk& w) {
+  w.slot = 0;
+  if (++w.qt < (r.rows + p.R - 1) / p.R) return;
+  w.qt = 0;
+  if (++w.h < p.Hk) return;
+  w.h = 0;
+  do {
+    ++w.b;
+    if (w.b >= p.batch) return;
+    r = request_of(p, w.b);
+  } while (r.rows == 0);
+}
+
+// The part of a unit that a CTA does, and where its result goes.
+struct Segment {
+  int first, n;     // slots
+  bool opens, ends;
+  __device__ bool whole() const { return opens && ends; }
+};
+
+__device__ __forceinline__ Segment segment_of(const Walk& w, int slots) {
+  Segment s;
+  s.first = w.slot;
+  s.n = static_cast<int>(min(w.left, static_cast<long long>(slots - w.slot)));
+  s.opens = w.slot == 0;
+  s.ends = w.slot + s.n == slots;
+  return s;
+}
+
+// The CTA whose range holds global slot s.
+__device__ __forceinline__ int cta_of(const AttnParams& p, long long s, long long total) {
+  return static_cast<int>(((s + 1) * min(total, static_cast<long long>(p.ncta)) - 1) / total);
+}
+
+// Token i (0..127) of a unit's tile: its page (-1: none), slot in the page, place in the request.
+struct Token { int page, slot; long long place; };
+
+__device__ __forceinline__ Token token_of(const AttnParams& p, const Request& r, int b, int tile, int i) {
+  Token t{-1, 0, -1};
+  int entry;
+  if (p.tpp) {
+    entry = tile / p.tpp;
+    t.slot = tile % p.tpp * kTile + i;
+    if (t.slot >= p.P) return t;
+  } else {
+    if (i >= p.ppt * p.P) return t;
+    entry = tile * p.ppt + i / p.P;
+    t.slot = i % p.P;
+  }
+  const long long place = 1ll * entry * p.P + t.slot;
+  if (p.counts ? entry >= r.len : place >= r.len) return t;
+  const int page = p.table[1ll * b * p.table_stride + entry];
+  if (page < 0 || page >= p.num_pages) {
+    if (p.status) atomicOr(p.status, DSD_SCALED_BAD_PAGE);
+    return t;
+  }
+  if (p.counts && t.slot >= p.counts[page]) return t;
+  t.page = page;
+  t.place = p.counts ? 0 : place;
+  return t;
+}
+
+// Whether query row `row` of the request sees the token at `place`.
+__device__ __forceinline__ bool sees(const AttnParams& p, const Request& r, int row, long long place) {
+  if (row >= r.rows) return false;
+  const long long pos = static_cast<long long>(r.len) - r.nq + row / p.G;
+  if (p.causal && place > pos) return false;
+  return !p.window || place > pos - p.window;
+}
+
+__device__ __forceinline__ long long scale_index(const AttnParams& p, int page, int h, int slot) {
+  return (1ll * page * p.Hk + h) * p.nblk + slot / p.bt;
+}
+
+// Weights carry the value scale: w = 2^(s + log2 vs - m) <= 1 for the running
+// maximum m of s + log2 vs, so that the largest CONTRIBUTION, not the largest
+// probability, is 1 when weights are cut into 8-bit pieces; the softmax sum gets
+// w / vs.  A scale below 2^-64 counts as 2^-64 in the exponent and keeps its own
+// value through the factor, so the sum cannot overflow and a zero scale adds
+// nothing to the output.
+struct TokenScale { float log2, inverse, factor; };
+
+__device__ __forceinline__ TokenScale token_scale(float vs) {
+  const float v = vs < kTinyScale ? kTinyScale : vs;   // NaN stays
+  return {log2f(v), 1.0f / v, vs < kTinyScale ? vs * (1.0f / kTinyScale) : 1.0f};
+}
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+// One output row from its (m, l, O) state; thread-wise over elements d.
+__device__ __forceinline__ void write_row_elem(const AttnParams& p, const Request& r, int h, int row,
+                                               int d, float o, float l) {
+  const int qi = row / p.G, head = h * p.G + row % p.G;
+  const long long i = 1ll * (r.q0 + qi) * p.ost[0] + 1ll * head * p.ost[1] + d;
+  store_elem(p.out, i, p.dtype, l == 0.0f ? 0.0f : o / l);
+}
+__device__ __forceinline__ void write_row_lse(const AttnParams& p, const Request& r, int h, int row,
+                                              float m, float l) {
+  if (!p.lse) return;
+  const int qi = row / p.G, head = h * p.G + row % p.G;
+  p.lse[1ll * (r.q0 + qi) * p.H + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Joins the partial results of the units that span CTAs.  Block (c, g) looks
+// after rows g, g + gridDim.y, ... of the unit CTA c leaves open: the opener's
+// piece is its slot 1, every following CTA's is its slot 0, added in CTA order,
+// so the result does not depend on timing.  256 threads cover head_dim <= 256.
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, d = threadIdx.x;
+  const int4 u = p.meta[c];
+  if (u.w < 0) return;
+  const Request r = request_of(p, u.x);
+  for (int row = blockIdx.y; row < p.R; row += gridDim.y) {
+    const int global_row = u.z * p.R + row;
+    if (global_row >= r.rows) return;
+    const auto piece = [&](int cta) { return (2ll * cta + (cta == c)) * p.R + row; };
+    float m = -INFINITY;
+    for (int i = c; i <= u.w; ++i) m = fmaxf(m, p.part_ml[2 * piece(i)]);
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o = 0.0f;
+#pragma unroll 4
+    for (int i = c; i <= u.w; ++i) {
+      const long long at = piece(i);
+      const float f = exp2f(p.part_ml[2 * at] - m0);
+      l += f * p.part_ml[2 * at + 1];
+      // a piece none of whose tokens this row saw holds zeros: f is 0 there
+      if (d < p.D) o += f * p.part_o[at * p.D + d];
+    }
+    if (d < p.D) write_row_elem(p, r, u.y, global_row, d, o, l);
+    if (d == 0) write_row_lse(p, r, u.y, global_row, m0, l);
+  }
+}
+
+}  // namespace dsds

@@ -1,0 +1,280 @@
+"""Scaled 8-bit paged KV cache: append with the position rotation, attention (torch tensors).
+
+The binding of ``dsd_scaled_append`` / ``dsd_scaled_attention``
+(``include/dsd_b200.h``) for programs that keep their tensors in torch.  A
+stored key or value is ``code * scale``: an e4m3 or int8 code under one fp32
+scale for each page, key head and run of ``block_tokens`` tokens of a page.
+
+Every call runs on the current torch stream of the cache's device, allocates
+only what it returns plus the attention's workspace (from torch's allocator),
+never synchronises, and can be captured into a CUDA graph.  What only the device
+can see (page ids, lengths, positions) is checked there: see
+:meth:`ScaledKVCache.check`.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import (DSD_EINVAL, KV_FP8_SCALED, KV_I8_SCALED, InvalidArgument, OutOfRange, ScaledAppendArgs,
+               ScaledAttentionArgs, ScaledCacheDesc, _check, load_library)
+
+_FORMATS = {torch.float8_e4m3fn: KV_FP8_SCALED, torch.int8: KV_I8_SCALED}
+_CODES = {v: k for k, v in _FORMATS.items()}
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_BAD = ((8, "a device-side wait exceeded its budget"),
+        (1, "a page id is outside the pool or a page is beyond the page-table row"),
+        (2, "a position is outside the rotation table"),
+        (4, "seq_lens or offsets that fit no token"))
+
+
+def _invalid(message: str):
+    raise InvalidArgument(int(DSD_EINVAL), message)
+
+
+class RotaryTable:
+    """Cosines and sines of the position rotation, fp32 ``[positions, rotary_dim / 2]``.
+
+    ``interleaved`` turns neighbouring elements (2i, 2i+1); otherwise the pairs
+    are (i, i + rotary_dim / 2).  Elements from ``rotary_dim`` on stay.
+    """
+
+    def __init__(self, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False):
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1 or cos.shape[1] < 1:
+            _invalid("cos and sin must have the same shape [positions, rotary_dim / 2]")
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            _invalid("cos and sin must be float32")
+        if not (cos.is_contiguous() and sin.is_contiguous()) or cos.device != sin.device:
+            _invalid("cos and sin must be contiguous and on one device")
+        self.cos, self.sin, self.interleaved = cos, sin, bool(interleaved)
+
+    @classmethod
+    def from_base(cls, positions: int, rotary_dim: int, base: float = 10000.0, interleaved: bool = False,
+                  device="cuda") -> "RotaryTable":
+        """Angles position * base^(-2i / rotary_dim), computed in 64 bits."""
+        if rotary_dim < 2 or rotary_dim % 2 or positions < 1:
+            _invalid("rotary_dim must be even and positive, positions positive")
+        i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+        angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * base ** (-i / rotary_dim)
+        return cls(angle.cos().float(), angle.sin().float(), interleaved)
+
+
+class ScaledKVCache:
+    """A pool of pages of 8-bit keys and values with their scales.
+
+    ``k_codes`` / ``v_codes``: float8_e4m3fn or int8 ``[num_pages, page_size,
+    num_kv_heads, head_dim]``, any positive strides with adjacent elements (a
+    head-major pool is its transposed view).  ``k_scales`` / ``v_scales``: float32
+    ``[num_pages, num_kv_heads, page_size / block_tokens]``, contiguous.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 kv_format: int = KV_FP8_SCALED, block_tokens: int | None = None, head_major: bool = False,
+                 device="cuda"):
+        if kv_format not in _CODES:
+            _invalid("kv_format must be KV_FP8_SCALED or KV_I8_SCALED")
+        block = page_size if block_tokens is None else block_tokens
+        if min(num_pages, page_size, num_kv_heads, head_dim, block) < 1 or page_size % block:
+            _invalid("sizes must be positive and block_tokens must divide page_size")
+        if head_dim % 8 or head_dim > 256:
+            _invalid("head_dim must be a multiple of 8 in [8, 256]")
+        shape = (num_pages, num_kv_heads, page_size, head_dim) if head_major else (
+            num_pages, page_size, num_kv_heads, head_dim)
+        codes = [torch.zeros(shape, dtype=torch.int8, device=device).view(_CODES[kv_format]) for _ in range(2)]
+        if head_major:
+            codes = [c.transpose(1, 2) for c in codes]
+        scales = [torch.zeros((num_pages, num_kv_heads, page_size // block), device=device) for _ in range(2)]
+        self._adopt(*codes, *scales)
+
+    @classmethod
+    def from_tensors(cls, k_codes, v_codes, k_scales, v_scales) -> "ScaledKVCache":
+        """A cache over the caller's tensors (kept, not copied)."""
+        self = cls.__new__(cls)
+        self._adopt(k_codes, v_codes, k_scales, v_scales)
+        return self
+
+    def _adopt(self, k_codes, v_codes, k_scales, v_scales):
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape or k_codes.dtype != v_codes.dtype:
+            _invalid("k_codes and v_codes must have one shape [num_pages, page_size, num_kv_heads, head_dim] and type")
+        if k_codes.dtype not in _FORMATS:
+            _invalid("codes must be float8_e4m3fn or int8")
+        pages, page_size, heads, dim = k_codes.shape
+        for c in (k_codes, v_codes):
+            if dim > 1 and c.stride(3) != 1:
+                _invalid("the elements of a code row must be adjacent")
+            if any(n > 1 and s < 1 for n, s in zip(c.shape, c.stride())):
+                _invalid("code strides must be positive")
+        if k_scales.dim() != 3 or k_scales.shape != v_scales.shape or tuple(k_scales.shape[:2]) != (pages, heads):
+            _invalid("scales must be [num_pages, num_kv_heads, page_size / block_tokens]")
+        blocks = k_scales.shape[2]
+        if blocks < 1 or page_size % blocks:
+            _invalid("the number of scales per page must divide page_size")
+        for s in (k_scales, v_scales):
+            if s.dtype != torch.float32 or not s.is_contiguous():
+                _invalid("scales must be contiguous float32")
+        device = k_codes.device
+        if device.type != "cuda" or any(t.device != device for t in (v_codes, k_scales, v_scales)):
+            _invalid("codes and scales must be on one CUDA device")
+        self.lib = load_library()
+        self.device = device
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+        self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = pages, page_size, heads, dim
+        self.block_tokens = page_size // blocks
+        self.kv_format = _FORMATS[k_codes.dtype]
+        strides = lambda c: [max(1, s) for s in c.stride()[:3]]  # noqa: E731  (a dimension of one may have any)
+        self._desc = ScaledCacheDesc(self.kv_format, pages, page_size, heads, dim, self.block_tokens,
+                                     k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                                     (ctypes.c_int64 * 3)(*strides(k_codes)), (ctypes.c_int64 * 3)(*strides(v_codes)))
+        self._desc_ref = ctypes.byref(self._desc)
+        self._workspace = {}
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    # ---- checks
+    def _ints(self, name, t, n=None):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.device != self.device or (t.numel() > 1 and t.stride(0) != 1):
+            _invalid(f"{name} must be a contiguous int32 vector on {self.device}")
+        if n is not None and t.shape[0] != n:
+            _invalid(f"{name} must have {n} entries")
+        return t.data_ptr()
+
+    def _rows(self, name, t, dtype=None, shape=None):
+        if t.dim() != 3 or t.device != self.device or t.dtype not in _TYPES or (
+                t.shape[2] > 1 and t.stride(2) != 1):
+            _invalid(f"{name} must be [rows, heads, head_dim] float32, bfloat16 or float16 on {self.device}, elements adjacent")
+        if t.shape[2] != self.head_dim:
+            _invalid(f"{name} must have head_dim {self.head_dim}")
+        if dtype is not None and t.dtype != dtype:
+            _invalid(f"{name} must be {dtype}")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            _invalid(f"{name} must be {tuple(shape)}")
+        return t.data_ptr()
+
+    def _table(self, table, batch):
+        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or table.shape[0] != batch or (
+                table.shape[1] > 1 and table.stride(1) != 1):
+            _invalid(f"the page table must be int32 [{batch}, pages] on {self.device}, rows contiguous")
+        return table.data_ptr(), table.stride(0) if batch > 1 else table.shape[1]
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def check(self) -> None:
+        """Waits for the device and raises if a call since the last check met bad device data."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            for bit, message in _BAD:
+                if bits & bit:
+                    if bit == 8:
+                        raise RuntimeError(message)
+                    raise OutOfRange(2, message)
+
+    # ---- operators
+    def append(self, k, v, page_table, seq_lens, token_offsets=None, rotary: RotaryTable | None = None,
+               positions=None, q=None, q_out=None, token_counts=None):
+        """Writes the new tokens' keys and values; returns the rotated queries (or None).
+
+        ``k`` / ``v`` ``[tokens, num_kv_heads, head_dim]`` and ``q`` ``[tokens, num_q_heads,
+        head_dim]`` hold the requests' new tokens back to back: request b's are rows
+        ``token_offsets[b] : token_offsets[b + 1]`` (None: one token for each request).
+        ``seq_lens`` counts each request's tokens with the new ones; ``page_table`` ``[batch,
+        pages]`` lists its pages.  ``rotary`` turns keys and queries by ``positions`` (None: the
+        token's place in its request).  ``q_out`` may be ``q``.  ``token_counts`` ``[num_pages]``
+        receives the tokens that the touched pages hold (what :meth:`attend_pages` reads).
+        """
+        batch = seq_lens.shape[0]
+        tokens, heads = k.shape[0], self.num_kv_heads
+        kp = self._rows("k", k, None, (tokens, heads, self.head_dim))
+        vp = self._rows("v", v, k.dtype, (tokens, heads, self.head_dim))
+        table, stride = self._table(page_table, batch)
+        a = ScaledAppendArgs()
+        a.dtype, a.batch, a.total_tokens, a.max_pages_per_request = _TYPES[k.dtype], batch, tokens, page_table.shape[1]
+        a.k, a.v, a.k_stride[:], a.v_stride[:] = kp, vp, k.stride()[:2], v.stride()[:2]
+        if token_offsets is not None:
+            a.token_offsets = self._ints("token_offsets", token_offsets, batch + 1)
+        a.seq_lens = self._ints("seq_lens", seq_lens)
+        a.page_table, a.page_table_stride = table, stride
+        if rotary is not None:
+            if rotary.cos.device != self.device:
+                _invalid(f"the rotation table must be on {self.device}")
+            a.cos, a.sin = rotary.cos.data_ptr(), rotary.sin.data_ptr()
+            a.rotary_positions, a.rotary_dim, a.interleaved = rotary.cos.shape[0], 2 * rotary.cos.shape[1], rotary.interleaved
+        if positions is not None:
+            a.positions = self._ints("positions", positions, tokens)
+        if q is not None:
+            a.q = self._rows("q", q, k.dtype)
+            if q.shape[0] != tokens:
+                _invalid("q must have a row for each token")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            a.q_out = self._rows("q_out", q_out, q.dtype, q.shape)
+            a.num_q_heads, a.q_stride[:], a.q_out_stride[:] = q.shape[1], q.stride()[:2], q_out.stride()[:2]
+        elif q_out is not None:
+            _invalid("q_out needs q")
+        if token_counts is not None:
+            a.token_counts = self._ints("token_counts", token_counts, self.num_pages)
+        a.status = self.status.data_ptr()
+        _check(self.lib.dsd_scaled_append(self.device.index, self._desc_ref, ctypes.byref(a), self._stream()))
+        return q_out
+
+    def _attend(self, q, table, lens, q_offsets, counts, scale, causal, window, out, return_lse):
+        batch = lens.shape[0]
+        rows = q.shape[0]
+        a = ScaledAttentionArgs()
+        a.q = self._rows("q", q)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        a.out = self._rows("out", out, q.dtype, q.shape)
+        a.dtype, a.batch, a.total_queries, a.num_q_heads = _TYPES[q.dtype], batch, rows, q.shape[1]
+        a.q_stride[:], a.out_stride[:] = q.stride()[:2], out.stride()[:2]
+        a.lens = self._ints("lens", lens)
+        a.page_table, a.page_table_stride = self._table(table, batch)
+        a.max_pages_per_request = table.shape[1]
+        if q_offsets is not None:
+            a.q_offsets = self._ints("q_offsets", q_offsets, batch + 1)
+        if counts is not None:
+            a.page_counts = self._ints("page_counts", counts, self.num_pages)
+        a.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
+        a.causal, a.window = causal, window
+        a.status = self.status.data_ptr()
+        lse = None
+        if return_lse:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+            a.lse = lse.data_ptr()
+        key = (batch, rows, q.shape[1], q_offsets is None, q.dtype)
+        need = self._workspace.get(key)   # bytes, a function of the sizes alone
+        if need is None:
+            if len(self._workspace) >= 1024:
+                self._workspace.clear()
+            n = ctypes.c_int64()
+            _check(self.lib.dsd_scaled_attention_workspace(self.device.index, self._desc_ref, ctypes.byref(a),
+                                                           ctypes.byref(n)))
+            need = self._workspace[key] = n.value
+        # a new block each call: torch orders its reuse by stream, and a captured graph keeps its own
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
+        _check(self.lib.dsd_scaled_attention(self.device.index, self._desc_ref, ctypes.byref(a), self._stream()))
+        return (out, lse) if return_lse else out
+
+    def attend(self, q, page_table, seq_lens, q_offsets=None, scale: float | None = None, causal: bool = True,
+               window: int = 0, out=None, return_lse: bool = False):
+        """Attention of each request's last queries over its first ``seq_lens[b]`` tokens.
+
+        ``q`` ``[queries, num_q_heads, head_dim]``: request b's are rows ``q_offsets[b] :
+        q_offsets[b + 1]`` (None: one query for each request), its last tokens.  ``scale`` defaults
+        to ``head_dim ** -0.5``.  ``window`` > 0 lets a query see that many tokens, itself
+        included.  A query that sees nothing gets zeros and -inf.  Returns ``out`` or
+        ``(out, lse)``, lse float32 ``[queries, num_q_heads]``.
+        """
+        return self._attend(q, page_table, seq_lens, q_offsets, None, scale, causal, window, out, return_lse)
+
+    def attend_pages(self, q, page_lists, list_lens, page_counts, q_offsets=None, scale: float | None = None,
+                     out=None, return_lse: bool = False):
+        """Attention over listed pages in any order, such as a top-k selection.
+
+        Request b attends to the tokens of the pages ``page_lists[b, :list_lens[b]]``; page p holds
+        ``page_counts[p]`` tokens (:meth:`append` keeps them in ``token_counts``).
+        """
+        return self._attend(q, page_lists, list_lens, q_offsets, page_counts, scale, False, 0, out, return_lse)

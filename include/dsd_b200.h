@@ -314,6 +314,164 @@ int dsd_decode_batch_noalloc(int device, const dsd_model_config* config, int cap
                              const float* d_keys, const float* d_values,
                              const int32_t* d_token_counts, float* d_outputs, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Scaled 8-bit paged cache: append with the position rotation, attention.
+ *
+ * No counterpart in the reference (its pool is fp32 and its attention reads one
+ * query token and one key head per query head).  These calls keep no state: the
+ * caller owns every device array and passes the stream, as in
+ * dsd_decode_batch_noalloc, so they can be captured into CUDA graphs, used on
+ * any stream and called from several threads at once.  They launch kernels and
+ * return; nothing is copied, allocated or synchronised.
+ *
+ * A stored key or value is code * scale: an 8-bit code (e4m3 or int8) under one
+ * fp32 scale for each page, key head and run of block_tokens tokens of the page
+ * ("block").  Query heads share key heads in groups: head h reads key head
+ * h / (num_q_heads / num_kv_heads).
+ * ------------------------------------------------------------------------- */
+#define DSD_KV_FP8_SCALED 3   /* e4m3 codes, |code| <= 448 */
+#define DSD_KV_I8_SCALED 4    /* int8 codes, |code| <= 127 */
+
+/* Element types of the device rows these calls read and write. */
+#define DSD_TYPE_F32 0
+#define DSD_TYPE_BF16 1
+#define DSD_TYPE_F16 2
+
+/* Bits the kernels OR into the caller's status word (see `status` below). */
+#define DSD_SCALED_BAD_PAGE 1      /* a page id outside [0, num_pages), or a page
+                                      beyond the request's page-table row       */
+#define DSD_SCALED_BAD_POSITION 2  /* a position outside the rotation table     */
+#define DSD_SCALED_BAD_LENGTH 4    /* seq_lens or offsets that fit no token     */
+#define DSD_SCALED_TIMEOUT 8       /* a bounded device-side wait gave up        */
+
+/* The cache.  Code (page p, token t, head h, element d) is at byte
+ * p*stride[0] + t*stride[1] + h*stride[2] + d of k_codes / v_codes; strides are
+ * positive, so pages may hold token-major or head-major rows and K and V may be
+ * interleaved.  Scales are [num_pages][num_kv_heads][page_size / block_tokens],
+ * finite and >= 0. */
+typedef struct dsd_scaled_cache {
+  int32_t kv_format;      /* DSD_KV_FP8_SCALED or DSD_KV_I8_SCALED */
+  int32_t num_pages;
+  int32_t page_size;      /* 1..4096 tokens */
+  int32_t num_kv_heads;
+  int32_t head_dim;       /* a multiple of 8, 8..256 */
+  int32_t block_tokens;   /* divides page_size, at most 256 */
+  void* k_codes;
+  void* v_codes;
+  float* k_scales;
+  float* v_scales;
+  int64_t k_stride[3];    /* bytes per page, token, head */
+  int64_t v_stride[3];
+} dsd_scaled_cache;
+
+/* dsd_scaled_append: the new tokens' keys (rotated by their position) and
+ * values go into the cache, quantised; queries of the same tokens may be rotated
+ * in the same launch.
+ *
+ * Request b's new tokens are rows token_offsets[b] .. token_offsets[b+1] of
+ * k / v / q (token_offsets NULL: one token per request, row b).  seq_lens[b]
+ * counts the request's tokens INCLUDING the new ones; the j-th of n new tokens
+ * is token seq_lens[b] - n + j of the request, in page
+ * page_table[b*page_table_stride + place / page_size].
+ *
+ * Rotation (cos == NULL: none): position = positions[row], or the token's place
+ * in its request when positions is NULL; element pairs (i, i + rotary_dim/2), or
+ * (2i, 2i+1) when interleaved, i < rotary_dim/2, turn by the angle whose cosine
+ * and sine are cos/sin[position*(rotary_dim/2) + i]; elements from rotary_dim on
+ * stay.  Products and their sum are each rounded to fp32.
+ *
+ * Scales: a block that gets its first token in this call takes
+ * amax * (1/448 or 1/127) over its new tokens' finite values (0 when amax <
+ * 2^-100; whatever the scale array held is ignored).  A block that holds older
+ * tokens keeps its scale unless the new tokens need a larger one; then the older
+ * codes are rounded again to the larger scale.  code = round-to-nearest-even(
+ * value * (1/scale)), saturating; infinities saturate, NaN is stored as NaN
+ * (e4m3) or 0 (int8).
+ *
+ * A token whose page, position or length is bad is left out (its status bit is
+ * set) and nothing outside the arrays is touched.  Two requests that append into
+ * the same block in one call race: their codes and its scale are unspecified. */
+typedef struct dsd_scaled_append_args {
+  int32_t dtype;                 /* DSD_TYPE_* of k, v, q, q_out */
+  int32_t batch;
+  int32_t total_tokens;          /* rows of k, v, q */
+  int32_t max_pages_per_request; /* entries of a page-table row */
+  const void* k;                 /* [total_tokens][num_kv_heads][head_dim] */
+  const void* v;
+  int64_t k_stride[2];           /* elements per token, head; elements are adjacent */
+  int64_t v_stride[2];
+  const int32_t* token_offsets;  /* device [batch+1], non-decreasing from 0, or NULL */
+  const int32_t* seq_lens;       /* device [batch] */
+  const int32_t* page_table;     /* device [batch][page_table_stride] */
+  int64_t page_table_stride;
+  const float* cos;              /* device [rotary_positions][rotary_dim/2], or NULL */
+  const float* sin;
+  const int32_t* positions;      /* device [total_tokens], or NULL */
+  int32_t rotary_positions;
+  int32_t rotary_dim;            /* even, <= head_dim */
+  int32_t interleaved;
+  int32_t num_q_heads;           /* 0: no queries */
+  const void* q;                 /* [total_tokens][num_q_heads][head_dim] */
+  void* q_out;                   /* rotated queries, rounded to dtype; may be q itself */
+  int64_t q_stride[2];
+  int64_t q_out_stride[2];
+  int32_t* token_counts;         /* device [num_pages] or NULL: counts[page] becomes the
+                                    number of the request's tokens in the page */
+  int32_t* status;               /* device word or NULL */
+} dsd_scaled_append_args;
+
+int dsd_scaled_append(int device, const dsd_scaled_cache* cache,
+                      const dsd_scaled_append_args* args, void* stream);
+
+/* dsd_scaled_attention: softmax(scale * q.k) v over the cache in fp32.
+ *
+ * Request b's queries are rows q_offsets[b] .. q_offsets[b+1] of q / out / lse
+ * (q_offsets NULL: one query per request, row b).  Two ways to name its tokens:
+ *  page_counts == NULL: the first lens[b] tokens of the pages its page-table row
+ *    lists.  The request's queries are its LAST tokens: with `causal`, query j of
+ *    n sees tokens up to lens[b] - n + j; with window > 0 only the last `window`
+ *    of those (without `causal`: tokens from lens[b] - n + j - window + 1 on).
+ *  page_counts != NULL: lens[b] is the number of pages its row lists, in any
+ *    order (the pages a selection picked), and a listed page p holds
+ *    min(page_counts[p], page_size) tokens; causal and window must be 0.
+ * A query that sees no token gets zeros and lse = -inf.  Rows behind the last
+ * request's are left as they were.  A listed page outside [0, num_pages) counts
+ * as masked and sets the status bit.
+ *
+ * lse (nullable) is the natural log of the softmax denominator.  The workspace
+ * (16-byte aligned, dsd_scaled_attention_workspace bytes) holds partial results
+ * between the call's two kernels: calls that may run at the same time, graph
+ * replays included, need one each. */
+typedef struct dsd_scaled_attention_args {
+  int32_t dtype;                 /* DSD_TYPE_* of q and out */
+  int32_t batch;                 /* <= 4096 */
+  int32_t total_queries;         /* rows of q, out, lse */
+  int32_t num_q_heads;           /* a multiple of num_kv_heads */
+  const void* q;                 /* [total_queries][num_q_heads][head_dim] */
+  void* out;
+  float* lse;                    /* [total_queries][num_q_heads], contiguous, or NULL */
+  int64_t q_stride[2];           /* elements per row, head */
+  int64_t out_stride[2];
+  const int32_t* q_offsets;      /* device [batch+1] or NULL */
+  const int32_t* lens;           /* device [batch] */
+  const int32_t* page_table;     /* device [batch][page_table_stride] */
+  int64_t page_table_stride;
+  const int32_t* page_counts;    /* device [num_pages] or NULL */
+  int32_t max_pages_per_request; /* entries of a page-table row */
+  float scale;
+  int32_t causal;
+  int32_t window;                /* 0: none */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;               /* device word or NULL */
+} dsd_scaled_attention_args;
+
+/* Bytes of workspace a call with these arguments needs (pointers are not looked at). */
+int dsd_scaled_attention_workspace(int device, const dsd_scaled_cache* cache,
+                                   const dsd_scaled_attention_args* args, int64_t* bytes);
+int dsd_scaled_attention(int device, const dsd_scaled_cache* cache,
+                         const dsd_scaled_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
