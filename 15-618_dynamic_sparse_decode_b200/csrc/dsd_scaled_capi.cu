@@ -13,6 +13,7 @@
 #include "dsd_internal.h"
 #include "dsd_scaled_append.cuh"
 #include "dsd_scaled_attn.cuh"
+#include "dsd_scaled_attn_tc.cuh"
 
 namespace {
 
@@ -30,7 +31,7 @@ struct Device {
 std::mutex g_mutex;
 Device g_devices[kMaxDevices];
 
-void SetSimpleAttributes();
+void SetAttentionAttributes();
 
 const Device& DeviceOf(int device) {
   if (device < 0 || device >= kMaxDevices) Fail(DSD_EINVAL, "device index out of range");
@@ -41,7 +42,7 @@ const Device& DeviceOf(int device) {
     Check(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device), "device");
     if (major != 10) Fail(DSD_EUNAVAILABLE, "no sm_100 GPU at this device index");
     Check(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device), "SM count");
-    SetSimpleAttributes();
+    SetAttentionAttributes();
     d.ready = true;
   }
   return d;
@@ -202,9 +203,45 @@ void SetSimple() {
   Check(cudaFuncSetAttribute(dsds::attn_simple_kernel<I8, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kSimpleMaxSmem), "shared memory attribute");
 }
-void SetSimpleAttributes() {
+
+// f(kernel, shape) for the tensor-core kernel of R query rows
+template <typename T>
+struct Tag { using type = T; };
+template <bool I8, int PIECES, int R, typename F>
+void WithTcRows(F&& f) { f(dsds::attn_tc_kernel<I8, R, PIECES>, Tag<dsds::TcShape<R, PIECES>>{}); }
+template <bool I8, int PIECES, typename F>
+void WithTc(int R, F&& f) {
+  switch (R) {
+    case 1: return WithTcRows<I8, PIECES, 1>(f);
+    case 2: return WithTcRows<I8, PIECES, 2>(f);
+    case 4: return WithTcRows<I8, PIECES, 4>(f);
+    case 8: return WithTcRows<I8, PIECES, 8>(f);
+    case 16: return WithTcRows<I8, PIECES, 16>(f);
+    default:
+      if constexpr (PIECES == 3) return WithTcRows<I8, PIECES, 32>(f);
+      else Fail(DSD_EINVAL, "no kernel for this row count");
+  }
+}
+template <typename F>
+void WithTc(bool i8, bool fp32, int R, F&& f) {
+  if (i8 && fp32) return WithTc<true, 4>(R, f);
+  if (i8) return WithTc<true, 3>(R, f);
+  if (fp32) return WithTc<false, 6>(R, f);
+  return WithTc<false, 3>(R, f);
+}
+constexpr int TcMaxRows(bool fp32) { return fp32 ? 16 : 32; }
+
+void SetAttentionAttributes() {
   SetSimple<false, 1>(); SetSimple<false, 2>(); SetSimple<false, 4>(); SetSimple<false, 8>();
   SetSimple<true, 1>(); SetSimple<true, 2>(); SetSimple<true, 4>(); SetSimple<true, 8>();
+  for (int i8 = 0; i8 < 2; ++i8)
+    for (int fp32 = 0; fp32 < 2; ++fp32)
+      for (int R = 1; R <= TcMaxRows(fp32); R *= 2)
+        WithTc(i8, fp32, R, [](auto kernel, auto tag) {
+          using Shape = typename decltype(tag)::type;
+          Check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape::kSmem)),
+                "shared memory attribute");
+        });
 }
 
 template <bool I8>
@@ -218,7 +255,84 @@ void LaunchSimple(const AttnParams& p, cudaStream_t s) {
   }
 }
 
+// TMA's view of one code array: elements, then tokens and heads by their stride,
+// then pages.  Only such orders can be encoded: every stride a multiple of 16
+// bytes and of the one before it.
+struct CodeOrder {
+  bool ok = false, head_first = false;
+  int64_t stride[3];   // of dimensions 1, 2, 3
+};
+
+CodeOrder OrderOf(const dsd_scaled_cache* c, const void* codes, const int64_t* st, bool head_first) {
+  CodeOrder o;
+  o.head_first = head_first;
+  const int64_t sizes[3] = {head_first ? c->num_kv_heads : c->page_size, head_first ? c->page_size : c->num_kv_heads,
+                            c->num_pages};
+  const int64_t given[3] = {head_first ? st[2] : st[1], head_first ? st[1] : st[2], st[0]};
+  // a dimension of one may have any stride: it takes the least that fits
+  int64_t before = 16, span = (c->head_dim + 15) / 16 * 16;
+  for (int i = 0; i < 3; ++i) {
+    o.stride[i] = sizes[i] > 1 ? given[i] : span;
+    if (o.stride[i] % before || o.stride[i] < c->head_dim || o.stride[i] >= (int64_t(1) << 40)) return o;
+    before = o.stride[i];
+    span = std::max(span, o.stride[i] * sizes[i]);
+  }
+  o.ok = Aligned(codes, 16);
+  return o;
+}
+
+struct TcMaps { CodeOrder k, v; };
+
+// The rule of the tensor-core path: rows of 16 to 128 bytes in 16-byte steps (one
+// 128-byte operand row, the rest of it zero-filled by TMA), pages of whole
+// 8-row swizzle groups, and strides that TMA takes.  Everything else runs on the
+// fp32 pipes.
+bool TensorCores(const dsd_scaled_cache* c, TcMaps* maps) {
+  if (c->head_dim % 16 || c->head_dim > 128 || c->page_size % 8) return false;
+  for (const bool head_first : {true, false}) {
+    maps->k = OrderOf(c, c->k_codes, c->k_stride, head_first);
+    maps->v = OrderOf(c, c->v_codes, c->v_stride, head_first);
+    if (maps->k.ok && maps->v.ok) return true;
+  }
+  return false;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled Encoder() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  if (!fn) Fail(DSD_ECUDA, "the driver has no cuTensorMapEncodeTiled");
+  return fn;
+}
+
+CUtensorMap MapOf(const dsd_scaled_cache* c, const void* codes, const CodeOrder& o) {
+  const cuuint32_t rows = cuuint32_t(std::min(c->page_size, dsds::kTile));
+  const cuuint64_t tokens = cuuint64_t(c->page_size), heads = cuuint64_t(c->num_kv_heads);
+  const cuuint64_t dims[4] = {cuuint64_t(c->head_dim), o.head_first ? heads : tokens, o.head_first ? tokens : heads,
+                              cuuint64_t(c->num_pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(o.stride[0]), cuuint64_t(o.stride[1]), cuuint64_t(o.stride[2])};
+  const cuuint32_t box[4] = {128, o.head_first ? 1 : rows, o.head_first ? rows : 1, 1};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  CUtensorMap map;
+  const CUresult r = Encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(codes), dims, strides, box,
+                               ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) Fail(DSD_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+  return map;
+}
+
 struct AttnPlan {
+  bool tc = false;
+  TcMaps maps;
   int R = 1, ncta = 0;
   int64_t ml_at = 0, o_at = 0, bytes = 0;   // workspace: meta, then ml, then O
 };
@@ -226,11 +340,17 @@ struct AttnPlan {
 AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_scaled_attention_args* a) {
   AttnPlan pl;
   const int group = a->num_q_heads / c->num_kv_heads;
+  const bool i8 = c->kv_format == DSD_KV_I8_SCALED, fp32 = a->dtype == DSD_TYPE_F32;
+  pl.tc = TensorCores(c, &pl.maps);
   // query rows of a request: exact for one query each, the average otherwise
   const int64_t queries = a->q_offsets ? (int64_t(a->total_queries) + a->batch - 1) / a->batch : 1;
   const int64_t rows = queries * group;
-  while (pl.R < 8 && pl.R < rows) pl.R *= 2;
-  pl.ncta = 8 * dev.sms;
+  const int most = pl.tc ? TcMaxRows(fp32) : 8;
+  while (pl.R < most && pl.R < rows) pl.R *= 2;
+  int per_sm = 8;
+  if (pl.tc)
+    WithTc(i8, fp32, pl.R, [&](auto, auto tag) { per_sm = decltype(tag)::type::kCtas; });
+  pl.ncta = per_sm * dev.sms;
   pl.ml_at = (int64_t(pl.ncta) * 16 + 255) / 256 * 256;
   pl.o_at = pl.ml_at + (int64_t(pl.ncta) * 2 * pl.R * 8 + 255) / 256 * 256;
   pl.bytes = pl.o_at + int64_t(pl.ncta) * 2 * pl.R * c->head_dim * 4;
@@ -306,7 +426,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   p.table_stride = a->page_table_stride;
   p.max_pages = a->max_pages_per_request;
   p.counts = a->page_counts;
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.scale_log2 = static_cast<float>(double(a->scale) * 1.4426950408889634);
   p.causal = a->causal != 0;
   p.window = a->window;
   p.status = a->status;
@@ -319,8 +439,17 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   p.part_ml = reinterpret_cast<float*>(ws + pl.ml_at);
   p.part_o = reinterpret_cast<float*>(ws + pl.o_at);
 
-  if (c->kv_format == DSD_KV_I8_SCALED) LaunchSimple<true>(p, s);
-  else LaunchSimple<false>(p, s);
+  const bool i8 = c->kv_format == DSD_KV_I8_SCALED;
+  if (pl.tc) {
+    const CUtensorMap k_map = MapOf(c, c->k_codes, pl.maps.k), v_map = MapOf(c, c->v_codes, pl.maps.v);
+    WithTc(i8, a->dtype == DSD_TYPE_F32, p.R, [&](auto kernel, auto tag) {
+      kernel<<<p.ncta, dsds::kTcThreads, decltype(tag)::type::kSmem, s>>>(p, k_map, v_map, pl.maps.k.head_first);
+    });
+  } else if (i8) {
+    LaunchSimple<true>(p, s);
+  } else {
+    LaunchSimple<false>(p, s);
+  }
   Check(cudaGetLastError(), "attention launch");
 
   // the join may be scheduled while the last CTAs of the attention run; it waits
