@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
   extern __shared__ float smem[];
   float* q_s = smem;                       // [R][D]
   float* w_s = q_s + R * p.D;              // [R][128] logits, then weights
-  float* inv_s = w_s + R * kTile;          // [128] 1 / value scale
+  float* inv_s = w_s + R * kTile;          // [128] 2^-e and f of the value scales
   float* fac_s = inv_s + kTile;            // [128]
   int* page_s = reinterpret_cast<int*>(fac_s + kTile);   // [128]
   int* slot_s = page_s + kTile;            // [128]
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
       const int row = row0 + i / p.D, d = i % p.D;
       float x = 0.0f;
       if (row < r.rows)
-        x = load_elem(p.q, 1ll * (r.q0 + row / p.G) * p.qst[0] + 1ll * (w.h * p.G + row % p.G) * p.qst[1] + d, p.dtype);
+        x = load_elem(p.q, 1ll * (r.q0 + row / p.by_group) * p.qst[0] + 1ll * (w.h * p.G + row % p.by_group) * p.qst[1] + d, p.dtype);
       q_s[i] = x;
     }
     if (tid < R) {
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
         }
 #pragma unroll
         for (int j = 0; j < R; ++j)
-          s[j] = sees(p, r, row0 + j, t.place) ? fmaf(s[j] * ks, p.scale_log2, ts.log2) : -INFINITY;
+          s[j] = sees(p, r, row0 + j, t.place) ? fmaf(s[j] * ks, p.scale_log2, ts.e) : -INFINITY;
       }
 #pragma unroll
       for (int j = 0; j < R; ++j) w_s[j * kTile + tid] = t.page >= 0 ? s[j] : -INFINITY;
@@ -158,9 +158,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
       if (seg.opens && tid == 0)
         p.meta[cta] = make_int4(w.b, w.h, w.qt, cta_of(p, w.at + slots - 1, w.total));
     }
-    w.at += seg.n;
-    w.left -= seg.n;
-    if (w.left > 0) next_unit(p, r, w);
+    next_unit(p, seg, r, w);
     __syncthreads();
   }
 }

@@ -17,9 +17,12 @@
 // with 8 query rows per key head, S and O have 24 of their up to 256 columns.
 //
 // Roles: warps 0-3 softmax (thread = token for S^T, = element d for O^T), warp 4
-// TMA, warp 5 MMA issue.  S and O are double-buffered in TMEM: S of the next tile
-// is issued before the weights of this one are ready.  O^T leaves TMEM every tile
-// and adds up in registers in fp32, rescaled by the running maximum there.
+// TMA, warp 5 MMA issue, warp 6 token data (page, scales, masks of a tile), warp 7
+// the next unit's queries.  Warps 4, 6 and 7 walk the CTA's range ahead of the
+// softmax, across units, so that a unit's first tile finds its operands ready.
+// S and O are double-buffered in TMEM: S of the next tile is issued before the
+// weights of this one are ready.  O^T leaves TMEM every tile and adds up in
+// registers in fp32, rescaled by the running maximum there.
 #pragma once
 
 #include <cuda.h>
@@ -29,7 +32,9 @@
 
 namespace dsds {
 
-constexpr int kTcThreads = 192;
+constexpr int kTcThreads = 256;
+constexpr int kTokenBytes = 3072;   // shared memory for token data, see TokenRing
+constexpr int kTokenStages = 8;     // tiles of token data ahead at most
 constexpr int kTcTileBytes = kTile * 128;
 
 __host__ __device__ constexpr int pad16(int n) { return (n + 15) / 16 * 16; }
@@ -39,11 +44,11 @@ template <int R, int PIECES>
 struct TcShape {
   static constexpr int N = pad16(R * PIECES);           // columns of S and of O
   static constexpr int kColumns = pow2_at_least(4 * N);
-  static constexpr int kOperand = N * 128;              // bytes of Q' (and of one P')
+  static constexpr int kOperand = (R * PIECES + 7) / 8 * 1024;   // bytes of Q' (and of one P')
   // CTAs per SM and ring stages that 512 TMEM columns and 227 KiB allow
-  static constexpr int kCtas = N <= 64 ? 2 : 1;
-  static constexpr int kStages = N <= 32 ? 3 : N <= 64 ? 2 : 4;
-  static constexpr size_t kSmem = 1024 + size_t(kStages) * 2 * kTcTileBytes + 3 * kOperand;
+  static constexpr int kCtas = 2;
+  static constexpr int kStages = N <= 32 ? 3 : 2;
+  static constexpr size_t kSmem = 1024 + size_t(kStages) * 2 * kTcTileBytes + 4 * kOperand;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -148,7 +153,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float warp_max(float x) {
   float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
 // The four softmax warps; returns whether any thread's flag was set.
@@ -205,52 +210,105 @@ __device__ __forceinline__ bool row_has_nan(const uint4* row, int lane) {
   return hit != 0;
 }
 
-// What a softmax thread knows of its token one tile ahead.
-struct TokenAhead {
-  int page, slot, held;   // held: tokens the page holds (page lists)
-  long long place;
-  float ks, vs;
+// What the softmax warps know of a unit, from warp 7.
+struct UnitInfo {
+  int tiles;          // -1: the range ends
+  int b, h, qt;
+  int rows;           // query rows from the unit's first on
+  int opens, ends;    // the segment has the unit's first / last slot
+  int last_cta;
 };
 
-// Page-table entry of token i of a tile, -1 where there is none.
-__device__ __forceinline__ int entry_of(const AttnParams& p, const Request& r, int b, int tile, int i) {
-  int entry, slot;
-  if (p.tpp) {
-    entry = tile / p.tpp;
-    slot = tile % p.tpp * kTile + i;
-    if (slot >= p.P) return -1;
-  } else {
-    if (i >= p.ppt * p.P) return -1;
-    entry = tile * p.ppt + i / p.P;
-    slot = i % p.P;
+// Token data of a tile, from warp 6.  A scale covers a block of bt tokens, so a
+// tile has at most 128 / bt + 1 entries: the two scales and how many of the
+// block's tokens are there.  As many tiles ahead as the ring has room for: the
+// scales come from far apart in memory, and one tile ahead left the softmax
+// waiting for them (64 requests x 16-32k: 1.01 ms, with eight ahead see DESIGN).
+struct TokenRing {
+  float2* scales;    // [stages][entries]
+  int* limit;        // [stages][entries]
+  int entries, stages;
+
+  __device__ __forceinline__ TokenRing(uint8_t* smem, const AttnParams& p) {
+    entries = p.token_entries;
+    stages = p.token_stages;
+    scales = reinterpret_cast<float2*>(smem);
+    limit = reinterpret_cast<int*>(scales + stages * entries);
   }
-  if (p.counts ? entry >= r.len : 1ll * entry * p.P + slot >= r.len) return -1;
-  const int page = p.table[1ll * b * p.table_stride + entry];
-  return page < 0 ? INT_MAX : page;
+};
+struct TileInfo { int place, lead, open; };   // of the first token; its index in its block; every row sees all
+
+__device__ __forceinline__ void copy4_async(const void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_after_copies(uint64_t* b) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
 }
 
-__device__ __forceinline__ TokenAhead resolve(const AttnParams& p, int h, int tile, int i, int page) {
-  TokenAhead t{-1, 0, INT_MAX, -1, 0.0f, 0.0f};
-  if (page < 0) return t;
-  if (page >= p.num_pages) {
-    if (p.status) atomicOr(p.status, DSD_SCALED_BAD_PAGE);
-    return t;
-  }
-  long long entry;
-  if (p.tpp) {
-    entry = tile / p.tpp;
-    t.slot = tile % p.tpp * kTile + i;
+// Page-table entry of box i of a tile, -1 where there is none.
+__device__ __forceinline__ int box_page(const AttnParams& p, const Request& r, int b, int tile, int i) {
+  const int entry = p.tpp ? tile / p.by_tpp : tile * p.ppt + i;
+  const int slot = p.tpp ? tile % p.by_tpp * kTile : 0;
+  if (p.counts ? entry >= r.len : 1ll * entry * p.P + slot >= r.len) return -1;
+  return p.table[1ll * b * p.table_stride + entry];
+}
+
+// Row `row` of a unit's queries, a lane four elements, as pieces in the operand;
+// returns the row's factor.
+template <bool I8, int R, int PIECES>
+__device__ __noinline__ float cut_row(float4 x, int row, uint8_t* op, float scale_log2) {
+  const int lane = threadIdx.x & 31;
+  uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
+                     max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
+  top = __reduce_max_sync(~0u, top);
+  // the row's power of two: 2^e <= largest < 2^(e+1)
+  const int e = max(static_cast<int>(top >> 23) - 127, -100);
+  uint16_t lo[PIECES], hi[PIECES];
+  const float f = __uint_as_float(uint32_t((I8 ? 7 * PIECES - 2 : 7) - e + 127) << 23);
+  if constexpr (I8) {
+    cut_int<PIECES>(__float2int_rn(x.x * f), __float2int_rn(x.y * f), lo);
+    cut_int<PIECES>(__float2int_rn(x.z * f), __float2int_rn(x.w * f), hi);
   } else {
-    entry = 1ll * tile * p.ppt + i / p.P;
-    t.slot = i % p.P;
+    cut_e4m3<PIECES>(x.x * f, x.y * f, lo);
+    cut_e4m3<PIECES>(x.z * f, x.w * f, hi);
   }
-  t.page = page;
-  t.place = p.counts ? 0 : entry * p.P + t.slot;
-  if (p.counts) t.held = p.counts[page];
-  const long long si = scale_index(p, page, h, t.slot);
-  t.ks = p.ks[si];
-  t.vs = p.vs[si];
-  return t;
+#pragma unroll
+  for (int j = 0; j < PIECES; ++j) {
+    const int n = j * R + row;
+    *reinterpret_cast<uint32_t*>(op + n * 128 + (4 * lane ^ (n & 7) << 4)) = uint32_t(lo[j]) | uint32_t(hi[j]) << 16;
+  }
+  // the first piece's unit: e4m3 2^(e - 7), int8 2^(e - 5); a row that is not finite is NaN
+  const float unit = __uint_as_float(uint32_t(e - (I8 ? 5 : 7) + 127) << 23);
+  return top >= 0x7f800000u ? NAN : scale_log2 * unit;
+}
+
+// Four elements of a row as they lie; aligned: one access.
+__device__ __forceinline__ uint4 load_four(const uint8_t* at, int elem, bool aligned) {
+  uint4 y{0, 0, 0, 0};
+  if (elem == 4) {
+    if (aligned) return __ldg(reinterpret_cast<const uint4*>(at));
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(at);
+    return {p[0], p[1], p[2], p[3]};
+  }
+  if (aligned) {
+    const uint2 z = __ldg(reinterpret_cast<const uint2*>(at));
+    y.x = z.x;
+    y.y = z.y;
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(at);
+    y.x = p[0] | uint32_t(p[1]) << 16;
+    y.y = p[2] | uint32_t(p[3]) << 16;
+  }
+  return y;
+}
+__device__ __forceinline__ float4 widen_four(uint4 y, int dtype) {
+  if (dtype == DSD_TYPE_F32)
+    return make_float4(__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w));
+  if (dtype == DSD_TYPE_BF16)
+    return make_float4(__uint_as_float(y.x << 16), __uint_as_float(y.x & 0xffff0000u), __uint_as_float(y.y << 16),
+                       __uint_as_float(y.y & 0xffff0000u));
+  const float2 a = __half22float2(*reinterpret_cast<__half2*>(&y.x)), b = __half22float2(*reinterpret_cast<__half2*>(&y.y));
+  return make_float4(a.x, a.y, b.x, b.y);
 }
 
 template <bool I8, int R, int PIECES>
@@ -261,13 +319,21 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
   constexpr int N = Shape::N, STAGES = Shape::kStages;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* base = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
-  uint8_t* k_ring = base;
+  // the operands first: a product's padding columns read on behind its operand
+  uint8_t* q_op = base;
+  uint8_t* p_op = q_op + 2 * Shape::kOperand;
+  uint8_t* k_ring = p_op + 2 * Shape::kOperand;
   uint8_t* v_ring = k_ring + STAGES * kTcTileBytes;
-  uint8_t* q_op = v_ring + STAGES * kTcTileBytes;
-  uint8_t* p_op = q_op + Shape::kOperand;
   __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-  __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], q_full, drained;
-  __shared__ float red[2][4][R], row_factor[R];
+  __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], unit_full[2], unit_empty[2];
+  __shared__ uint64_t token_full[kTokenStages], token_empty[kTokenStages], drained;
+  __shared__ TileInfo info[kTokenStages];
+  __shared__ __align__(16) uint8_t token_smem[kTokenBytes];
+  __shared__ float4 red[2][R];   // a row's four warps
+  __shared__ float row_factor[2][R];
+  __shared__ int row_pos[2][R], row_lse[2][R];   // a row's place; its element of lse
+  __shared__ long long row_out[2][R];            // its first element of out
+  __shared__ UnitInfo units[2];
   __shared__ uint32_t tmem_base;
   __shared__ int stop;
   __shared__ Walk walk_s;
@@ -287,8 +353,13 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 4);
+      mbar_init(&unit_full[i], 1);
+      mbar_init(&unit_empty[i], 5);   // the softmax warps and the MMA warp
     }
-    mbar_init(&q_full, 4);
+    for (int i = 0; i < kTokenStages; ++i) {
+      mbar_init(&token_full[i], 64);   // every lane, and every lane's copies
+      mbar_init(&token_empty[i], 4);
+    }
     mbar_init(&drained, 1);
     stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -308,26 +379,29 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
-  Request r = request_of(p, w.b);
 
   if (warp == 4) {
     // ---- TMA: the pages of a tile, one box each, K then V
+    Request r = request_of(p, w.b);
     const int rows = p.tpp ? kTile : p.P, boxes = p.tpp ? 1 : p.ppt;
     uint32_t g = 0;
     bool ok = true;
+#pragma unroll 1
     while (w.left > 0 && ok) {
       const Span span = span_of(p, r, w.qt);
-      const int slots = slots_of(span);
-      const Segment seg = segment_of(w, slots);
+      const Segment seg = segment_of(w, slots_of(span));
       const int tiles = span.n == 0 ? 0 : seg.n;
+      int next = -1;
+      if (tiles > 0 && lane < boxes) next = box_page(p, r, w.b, span.first + seg.first, lane);
+#pragma unroll 1
       for (int i = 0; i < tiles && ok; ++i, ++g) {
         const int tile = span.first + seg.first + i;
-        int page = -1;
-        if (lane < boxes) page = entry_of(p, r, w.b, tile, lane * p.P);
+        const int page = next;
+        if (i + 1 < tiles && lane < boxes) next = box_page(p, r, w.b, tile + 1, lane);
         const bool good = page >= 0 && page < p.num_pages;
         const int bytes = __popc(__ballot_sync(~0u, good)) * rows * 128;
         const int s = g % STAGES, parity = (g / STAGES & 1) ^ 1;
-        const int slot = p.tpp ? tile % p.tpp * kTile : 0;
+        const int slot = p.tpp ? tile % p.by_tpp * kTile : 0;
         const int c1 = head_first ? w.h : slot, c2 = head_first ? slot : w.h;
         const uint32_t at = s * kTcTileBytes + lane * rows * 128;
 #pragma unroll
@@ -341,13 +415,12 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
           if (good) tma_box(kv ? &v_map : &k_map, smem_addr(kv ? v_ring : k_ring) + at, full, c1, c2, page);
         }
       }
-      w.at += seg.n;
-      w.left -= seg.n;
-      if (w.left > 0) next_unit(p, r, w);
+      next_unit(p, seg, r, w);
     }
     // after a time-out: the copies still in flight land before the block's memory is given back
     if (!ok && lane == 0) {
       int never = 0;
+#pragma unroll 1
       for (uint32_t i = g > STAGES ? g - STAGES : 0; i <= g; ++i) {
         mbar_wait_slow(&k_full[i % STAGES], i / STAGES & 1, &never, nullptr);
         never = 0;
@@ -359,8 +432,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
     // ---- MMA issue (one lane)
     if (lane == 0) {
       constexpr uint32_t s_desc = mma_desc<I8, N>(false), o_desc = mma_desc<I8, N>(true);
-      const uint64_t q_d = operand_desc(smem_addr(q_op));
-      uint32_t g = 0, unit = 0;
+      uint32_t g = 0;
       bool ok = true;
       const auto weigh = [&](uint32_t t) {   // O^T of tile t
         const int s = t % STAGES, buf = t & 1;
@@ -371,40 +443,43 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         tc_fence_after();
         const uint64_t a = operand_desc(smem_addr(v_ring + s * kTcTileBytes));
         const uint64_t b = operand_desc(smem_addr(p_op + buf * Shape::kOperand));
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 4; ++k) mma<I8>(tmem + 2 * N + buf * N, a + 256 * k, b + 2 * k, o_desc, k > 0);
         mma_commit(&v_empty[s]);
         mma_commit(&o_full[buf]);
       };
-      while (w.left > 0 && ok) {
-        const Span span = span_of(p, r, w.qt);
-        const int slots = slots_of(span);
-        const Segment seg = segment_of(w, slots);
-        const int tiles = span.n == 0 ? 0 : seg.n;
+      bool owed = false;   // the last tile's O^T is still to be issued
+#pragma unroll 1
+      for (uint32_t unit = 0; ok; ++unit) {
+        const int u = unit & 1;
+        // the queries are ready ahead of time, except for the first units
+        if (owed && !mbar_try(&unit_full[u], unit >> 1 & 1)) {
+          weigh(g - 1);
+          owed = false;
+        }
+        ok = ok && mbar_wait(&unit_full[u], unit >> 1 & 1, &stop, p.status);
+        if (!ok) break;
+        const int tiles = units[u].tiles;
+        mbar_arrive(&unit_empty[u]);
+        if (tiles < 0) break;
+        const uint64_t q_d = operand_desc(smem_addr(q_op + u * Shape::kOperand));
+#pragma unroll 1
         for (int i = 0; i < tiles && ok; ++i, ++g) {
-          if (i == 0) {
-            // the softmax warps write the next queries after the last unit's tiles
-            if (g > 0) weigh(g - 1);
-            ok = ok && mbar_wait(&q_full, unit & 1, &stop, p.status);
-            ++unit;
-          }
           const int s = g % STAGES, buf = g & 1;
           ok = ok && mbar_wait(&k_full[s], g / STAGES & 1, &stop, p.status) &&
                mbar_wait(&s_empty[buf], (g >> 1 & 1) ^ 1, &stop, p.status);
           if (!ok) break;
           tc_fence_after();
           const uint64_t a = operand_desc(smem_addr(k_ring + s * kTcTileBytes));
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < 4; ++k) mma<I8>(tmem + buf * N, a + 2 * k, q_d + 2 * k, s_desc, k > 0);
           mma_commit(&k_empty[s]);
           mma_commit(&s_full[buf]);
-          if (i > 0) weigh(g - 1);
+          if (owed) weigh(g - 1);
+          owed = true;
         }
-        w.at += seg.n;
-        w.left -= seg.n;
-        if (w.left > 0) next_unit(p, r, w);
       }
-      if (ok && g > 0) weigh(g - 1);
+      if (owed) weigh(g - 1);
       if (!ok) {
         // after a time-out: what was issued ends before TMEM is given back
         int never = 0;
@@ -413,69 +488,150 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
       }
     }
     __syncwarp();
-  } else {
-    // ---- softmax
-    uint32_t g = 0;
+  } else if (warp == 6) {
+    // ---- token data; a lane has every 32nd entry of a tile
+    const TokenRing ring(token_smem, p);
+    Request r = request_of(p, w.b);
+    int s = 0, phase = 0;   // of the token ring
     bool ok = true;
-    const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
+#pragma unroll 1
     while (w.left > 0 && ok) {
       const Span span = span_of(p, r, w.qt);
+      const Segment seg = segment_of(w, slots_of(span));
+      const int tiles = span.n == 0 ? 0 : seg.n;
+      const int* table = p.table + 1ll * w.b * p.table_stride;
+      const int row0 = w.qt * R;
+      const int base_pos = r.len - r.nq;
+      // every row sees the tokens at all_from .. all_to
+      int all_from = 0, all_to = INT_MAX;
+      if (p.causal) all_to = max(base_pos + row0 / p.by_group, -1);
+      if (p.window) all_from = max(max(base_pos + (min(row0 + R, r.rows) - 1) / p.by_group, -1) - p.window + 1, 0);
+#pragma unroll 1
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int tile = span.first + seg.first + i;
+        const int first = p.tpp ? tile / p.by_tpp : tile * p.ppt;       // page-table entry of the first token
+        const int off = p.tpp ? tile % p.by_tpp * kTile : 0;            // and its slot in that page
+        const int lead = off % p.by_block;
+        const int here = p.tpp ? min(kTile, p.P - off) : p.ppt * p.P;   // places of the tile
+        ok = mbar_wait(&token_empty[s], phase ^ 1, &stop, p.status);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        // one pass unless block_tokens < 5; the table's lines are in L1 then
+#pragma unroll 1
+        for (int e = lane; e < ring.entries; e += 32) {
+          const int t = e * p.bt - lead;   // the block's first token in the tile; below 0 only where tpp
+          int limit = 0;
+          if (t < here) {
+            const int entry = p.tpp ? first : first + t / p.by_page, slot = p.tpp ? off + t : t % p.by_page;
+            if (!p.counts) limit = static_cast<int>(min(max(r.len - 1ll * entry * p.P - slot, 0ll), static_cast<long long>(p.bt)));
+            if (p.counts ? entry < r.len : limit > 0) {
+              const int page = table[entry];
+              if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
+                if (p.status) atomicOr(p.status, DSD_SCALED_BAD_PAGE);
+                limit = 0;
+              } else {
+                if (p.counts) limit = min(max(p.counts[page] - slot, 0), p.bt);
+                const long long si = (1ll * page * p.Hk + w.h) * p.nblk + slot / p.by_block;
+                float2* to = ring.scales + s * ring.entries + e;
+                copy4_async(&to->x, p.ks + si);
+                copy4_async(&to->y, p.vs + si);
+              }
+            }
+          }
+          ring.limit[s * ring.entries + e] = limit;
+        }
+        if (lane == 0) {
+          const int place = p.tpp ? first * p.P + off : tile * p.ppt * p.P;
+          info[s] = {place, lead, p.counts || (place >= all_from && place <= all_to - (kTile - 1))};
+        }
+        mbar_arrive_after_copies(&token_full[s]);
+        mbar_arrive(&token_full[s]);
+        if (++s == ring.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+      next_unit(p, seg, r, w);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 7) {
+    // ---- queries, cut into pieces; a lane takes four elements of every row
+    Request r = request_of(p, w.b);
+    const int elem = p.dtype == DSD_TYPE_F32 ? 4 : 2;
+    const bool aligned = reinterpret_cast<uintptr_t>(p.q) % (4 * elem) == 0 && p.qst[0] % 4 == 0 && p.qst[1] % 4 == 0;
+    bool ok = true;
+#pragma unroll 1
+    for (uint32_t unit = 0; ok; ++unit) {
+      const int u = unit & 1;
+      const bool end = w.left <= 0;
+      Span span{0, 0};
+      if (!end) span = span_of(p, r, w.qt);
       const int slots = slots_of(span);
       const Segment seg = segment_of(w, slots);
-      const int tiles = span.n == 0 ? 0 : seg.n;
-      const int first = span.first + seg.first;
-      const int row0 = w.qt * R;
-      const long long base_pos = static_cast<long long>(r.len) - r.nq;
-
-      // token data: the page-table entry two tiles ahead, the scales one
-      TokenAhead ahead{-1, 0, INT_MAX, -1, 0.0f, 0.0f};
-      int entry = -1;
-      if (tiles > 0) ahead = resolve(p, w.h, first, tid, entry_of(p, r, w.b, first, tid));
-      if (tiles > 1) entry = entry_of(p, r, w.b, first + 1, tid);
-
-      if (tiles > 0) {
-        // queries, cut into pieces; a warp takes a row, a lane four elements
-        for (int row = warp; row < R; row += 4) {
-          float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const int gr = row0 + row;
-          if (gr < r.rows) {
-            const long long at = 1ll * (r.q0 + gr / p.G) * p.qst[0] + 1ll * (w.h * p.G + gr % p.G) * p.qst[1];
+      const int row0 = w.qt * R, base_pos = r.len - r.nq;
+      // lane = row: where it lies and what it sees
+      const int gr = min(row0 + lane, r.rows - 1);
+      const int qi = gr / p.by_group, head = w.h * p.G + gr % p.by_group;
+      const long long at = 1ll * (r.q0 + qi) * p.qst[0] + 1ll * head * p.qst[1];
+      const bool in_row = 4 * lane < p.D;   // head_dim is a multiple of 16 here
+      uint4 raw[R];
+      if (!end) {
+        // every address is a valid one: the loads are in flight together
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (4 * lane + j < p.D) x[j] = load_elem(p.q, at + 4 * lane + j, p.dtype);
-          }
-          uint32_t top = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(fabsf(x[j])));
-          top = __reduce_max_sync(~0u, top);
-          // the row's power of two: 2^e <= largest < 2^(e+1); not finite: the row is NaN
-          const int e = max(static_cast<int>(top >> 23) - 127, -100);
-          uint16_t lo[PIECES], hi[PIECES];
-          if constexpr (I8) {
-            constexpr int kBits = 7 * PIECES - 2;
-            const float f = __uint_as_float(uint32_t(kBits - e + 127) << 23);
-            cut_int<PIECES>(__float2int_rn(x[0] * f), __float2int_rn(x[1] * f), lo);
-            cut_int<PIECES>(__float2int_rn(x[2] * f), __float2int_rn(x[3] * f), hi);
-          } else {
-            const float f = __uint_as_float(uint32_t(7 - e + 127) << 23);
-            cut_e4m3<PIECES>(x[0] * f, x[1] * f, lo);
-            cut_e4m3<PIECES>(x[2] * f, x[3] * f, hi);
-          }
-#pragma unroll
-          for (int j = 0; j < PIECES; ++j) {
-            const int n = j * R + row;
-            *reinterpret_cast<uint32_t*>(q_op + n * 128 + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4) =
-                uint32_t(lo[j]) | uint32_t(hi[j]) << 16;
-          }
-          // first piece's unit: e4m3 2^(e-7); int8 2^(e - 5)
-          if (lane == 0)
-            row_factor[row] = top >= 0x7f800000u ? NAN : ldexpf(p.scale_log2, I8 ? e - 5 : e - 7);
-        }
-        proxy_fence();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full);
+        for (int row = 0; row < R; ++row)
+          raw[row] = load_four(static_cast<const uint8_t*>(p.q) + (__shfl_sync(~0u, at, row) + (in_row ? 4 * lane : 0)) * elem,
+                               elem, aligned);
       }
-
+      ok = mbar_wait(&unit_empty[u], (unit >> 1 & 1) ^ 1, &stop, p.status);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      if (!end) {
+#pragma unroll
+        for (int row = 0; row < R; ++row) {
+          float4 x = widen_four(raw[row], p.dtype);
+          if (!in_row || row0 + row >= r.rows) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const float factor = cut_row<I8, R, PIECES>(x, row, q_op + u * Shape::kOperand, p.scale_log2);
+          if (lane == 0) row_factor[u][row] = factor;
+        }
+        if (lane < R) {
+          row_pos[u][lane] = base_pos + qi;
+          row_out[u][lane] = 1ll * (r.q0 + qi) * p.ost[0] + 1ll * head * p.ost[1];
+          row_lse[u][lane] = (r.q0 + qi) * p.H + head;
+        }
+      }
+      if (lane == 0) {
+        UnitInfo& x = units[u];
+        x.tiles = end ? -1 : span.n == 0 ? 0 : seg.n;
+        x.b = w.b;
+        x.h = w.h;
+        x.qt = w.qt;
+        x.rows = r.rows - row0;
+        x.opens = seg.opens;
+        x.ends = seg.ends;
+        x.last_cta = end ? 0 : cta_of(p, w.at - w.slot + slots - 1, w.total);
+      }
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_full[u]);
+      if (end) break;
+      next_unit(p, seg, r, w);
+    }
+  } else {
+    // ---- softmax
+    const TokenRing ring(token_smem, p);
+    const int here = p.tpp ? kTile : p.ppt * p.P;   // a tile's places (a page's last tile: entries have limit 0 behind it)
+    const int my_entry = tid / p.by_block, my_place = tid % p.by_block;
+    uint32_t g = 0;
+    int ts_at = 0, ts_phase = 0;   // of the token ring
+    bool ok = true;
+    const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
+#pragma unroll 1
+    for (uint32_t unit = 0; ok; ++unit) {
+      const int u = unit & 1;
+      ok = !softmax_sync_or(!mbar_wait(&unit_full[u], unit >> 1 & 1, &stop, p.status));
+      if (!ok) break;
+      const int tiles = units[u].tiles;
+      if (tiles < 0) break;
       float m[R], l[R], alpha[R], acc[R];
 #pragma unroll
       for (int j = 0; j < R; ++j) {
@@ -506,24 +662,30 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         }
         return in;
       };
+#pragma unroll 1
       for (int i = 0; i < tiles && ok; ++i, ++g) {
-        const int buf = g & 1, tile = first + i;
-        const TokenAhead t = ahead;
-        if (i + 1 < tiles) ahead = resolve(p, w.h, tile + 1, tid, entry);
-        if (i + 2 < tiles) entry = entry_of(p, r, w.b, tile + 2, tid);
-        const bool valid = t.page >= 0 && t.slot < t.held;
-        // whether every row sees every token that is there
-        bool open = true;
-        if (!p.counts) {
-          const long long t0 = p.tpp ? 1ll * (tile / p.tpp) * p.P + tile % p.tpp * kTile : 1ll * tile * p.ppt * p.P;
-          const long long last_row = min(row0 + R, r.rows) - 1;
-          open = (!p.causal || t0 + kTile - 1 <= base_pos + row0 / p.G) &&
-                 (!p.window || t0 > base_pos + last_row / p.G - p.window);
+        const int buf = g & 1;
+        bool in = mbar_wait(&token_full[ts_at], ts_phase, &stop, p.status);
+        const TileInfo tile = info[ts_at];
+        int entry = my_entry, in_block = my_place;
+        if (tile.lead) {
+          entry = (tile.lead + tid) / p.by_block;
+          in_block = (tile.lead + tid) % p.by_block;
         }
-        const TokenScale ts = token_scale(valid ? t.vs : 0.0f);
+        entry += ts_at * ring.entries;
+        const int place = tile.place + tid;
+        const bool open = tile.open != 0;
+        const bool valid = tid < here && in_block < ring.limit[entry];
+        const float2 scales = ring.scales[entry];
+        const TokenScale ts = token_scale(valid ? scales.y : 0.0f);
 
-        bool in = mbar_wait(&s_full[buf], g >> 1 & 1, &stop, p.status);
+        in = mbar_wait(&s_full[buf], g >> 1 & 1, &stop, p.status) && in;
         __syncwarp();
+        if (lane == 0) mbar_arrive(&token_empty[ts_at]);
+        if (++ts_at == ring.stages) {
+          ts_at = 0;
+          ts_phase ^= 1;
+        }
         tc_fence_after();
         float s[R];
         {
@@ -539,15 +701,20 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
             float sum = 0.0f;
 #pragma unroll
             for (int j = PIECES - 1; j >= 0; --j) sum = add_pieces<I8, PIECES>(sum, x[j][row], j);
-            s[row] = sum;
+            s[row] = valid ? fmaf(sum * scales.x, row_factor[u][row], ts.e) : -INFINITY;
+          }
+        }
+        if (!open) {
+#pragma unroll
+          for (int row = 0; row < R; ++row) {
+            const int pos = row_pos[u][row];
+            if ((p.causal && place > pos) || (p.window && 1ll * place + p.window <= pos)) s[row] = -INFINITY;
           }
         }
 #pragma unroll
         for (int row = 0; row < R; ++row) {
-          s[row] = valid ? fmaf(s[row] * t.ks, row_factor[row], ts.log2) : -INFINITY;
-          if (!open && valid && !sees(p, r, row0 + row, t.place)) s[row] = -INFINITY;
           const float top = warp_max(s[row]);
-          if (lane == 0) red[buf][warp][row] = top;
+          if (lane == 0) reinterpret_cast<float*>(&red[buf][row])[warp] = top;
         }
         // A tile with places that a row must not see: what lies there may be NaN,
         // and 0 * NaN is NaN, so such a value row becomes zeros; rows that do see
@@ -572,7 +739,8 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         }
 #pragma unroll
         for (int row = 0; row < R; ++row) {
-          const float top = fmaxf(fmaxf(red[buf][0][row], red[buf][1][row]), fmaxf(red[buf][2][row], red[buf][3][row]));
+          const float4 tops = red[buf][row];
+          const float top = fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w));
           const float now = fmaxf(m[row], top), m0 = now == -INFINITY ? 0.0f : now;
           alpha[row] = ex2(m[row] - m0);
           m[row] = now;
@@ -582,18 +750,17 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
           s[row] = x * ts.factor;
         }
         uint8_t* op = p_op + buf * Shape::kOperand;
-        const auto put = [&](int n, uint32_t byte) {
-          op[n * 128 + (((tid >> 4) ^ (n & 7)) << 4) + (tid & 15)] = static_cast<uint8_t>(byte);
-        };
+        // byte tid of row n, its 16-byte pieces swizzled within groups of 8 rows
+        const auto put = [&](int n, uint32_t byte) { op[n * 128 + (tid ^ (n & 7) << 4)] = static_cast<uint8_t>(byte); };
 #pragma unroll
         for (int row = 0; row < R; row += 2) {
           const float x = s[row], y = row + 1 < R ? s[row + 1] : 0.0f;
           uint16_t piece[PIECES];
           if constexpr (I8) {
-            constexpr float kOne = float(1 << (7 * PIECES - 1));
+            constexpr float kOne = float(1 << (7 * PIECES - 2));
             cut_int<PIECES>(__float2int_rn(x * kOne), __float2int_rn(y * kOne), piece);
           } else {
-            cut_e4m3<PIECES>(x * 256.0f, y * 256.0f, piece);
+            cut_e4m3<PIECES>(x * 128.0f, y * 128.0f, piece);
           }
 #pragma unroll
           for (int j = 0; j < PIECES; ++j) {
@@ -613,36 +780,37 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         float x = l[row];
 #pragma unroll
         for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-        if (lane == 0) red[0][warp][row] = x;
+        if (lane == 0) reinterpret_cast<float*>(&red[0][row])[warp] = x;
       }
       ok = !softmax_sync_or(!ok);
-      // weight 1 is 256 (e4m3) or 2^6 in the first piece's unit (int8: 2^(7 PIECES - 1) over 2^(7 (PIECES - 1)))
-      constexpr float kUnit = I8 ? 1.0f / 64 : 1.0f / 256;
+      // weight 1 is 128 (e4m3) or 2^5 in the first piece's unit (int8: 2^(7 PIECES - 2) over 2^(7 (PIECES - 1)))
+      constexpr float kUnit = I8 ? 1.0f / 32 : 1.0f / 128;
+      const UnitInfo x = units[u];
+      const bool whole = x.opens && x.ends;
+      const long long piece = (2ll * cta + x.opens) * R;
 #pragma unroll
       for (int row = 0; row < R; ++row) {
-        const float sum = (red[0][0][row] + red[0][1][row]) + (red[0][2][row] + red[0][3][row]);
-        const float o = acc[row] * kUnit;
-        if (seg.whole()) {
-          if (row0 + row < r.rows) {
-            if (tid < p.D) write_row_elem(p, r, w.h, row0 + row, tid, o, sum);
-            if (tid == 0) write_row_lse(p, r, w.h, row0 + row, m[row] == -INFINITY ? 0.0f : m[row], sum);
-          }
+        const float4 sums = red[0][row];
+        const float sum = (sums.x + sums.y) + (sums.z + sums.w);
+        float o = acc[row] * kUnit;
+        if (whole) {
+          if (row >= x.rows) continue;
+          o = sum == 0.0f ? 0.0f : o / sum;
+          if (tid < p.D) store_elem(p.out, row_out[u][row] + tid, p.dtype, o);
+          if (tid == 0 && p.lse)
+            p.lse[row_lse[u][row]] = sum == 0.0f ? -INFINITY : ((m[row] == -INFINITY ? 0.0f : m[row]) + log2f(sum)) * kLn2;
         } else {
-          const long long at = (2ll * cta + seg.opens) * R + row;
-          if (tid < p.D) p.part_o[at * p.D + tid] = o;
+          if (tid < p.D) p.part_o[(piece + row) * p.D + tid] = o;
           if (tid == 0) {
-            p.part_ml[2 * at] = m[row];
-            p.part_ml[2 * at + 1] = sum;
+            p.part_ml[2 * (piece + row)] = m[row];
+            p.part_ml[2 * (piece + row) + 1] = sum;
           }
         }
       }
-      if (!seg.whole() && seg.opens && tid == 0)
-        p.meta[cta] = make_int4(w.b, w.h, w.qt, cta_of(p, w.at + slots - 1, w.total));
-      // nobody writes `red` or the row factors of the next unit before all have read these
-      ok = !softmax_sync_or(!ok) && ok;
-      w.at += seg.n;
-      w.left -= seg.n;
-      if (w.left > 0) next_unit(p, r, w);
+      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.h, x.qt, x.last_cta);
+      // `red` is written again behind the barrier at the next unit's start
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_empty[u]);
     }
   }
   tc_fence_before();

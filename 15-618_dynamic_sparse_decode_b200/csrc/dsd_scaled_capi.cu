@@ -215,11 +215,7 @@ void WithTc(int R, F&& f) {
     case 1: return WithTcRows<I8, PIECES, 1>(f);
     case 2: return WithTcRows<I8, PIECES, 2>(f);
     case 4: return WithTcRows<I8, PIECES, 4>(f);
-    case 8: return WithTcRows<I8, PIECES, 8>(f);
-    case 16: return WithTcRows<I8, PIECES, 16>(f);
-    default:
-      if constexpr (PIECES == 3) return WithTcRows<I8, PIECES, 32>(f);
-      else Fail(DSD_EINVAL, "no kernel for this row count");
+    default: return WithTcRows<I8, PIECES, 8>(f);
   }
 }
 template <typename F>
@@ -229,14 +225,14 @@ void WithTc(bool i8, bool fp32, int R, F&& f) {
   if (fp32) return WithTc<false, 6>(R, f);
   return WithTc<false, 3>(R, f);
 }
-constexpr int TcMaxRows(bool fp32) { return fp32 ? 16 : 32; }
+constexpr int kTcMaxRows = 8;
 
 void SetAttentionAttributes() {
   SetSimple<false, 1>(); SetSimple<false, 2>(); SetSimple<false, 4>(); SetSimple<false, 8>();
   SetSimple<true, 1>(); SetSimple<true, 2>(); SetSimple<true, 4>(); SetSimple<true, 8>();
   for (int i8 = 0; i8 < 2; ++i8)
     for (int fp32 = 0; fp32 < 2; ++fp32)
-      for (int R = 1; R <= TcMaxRows(fp32); R *= 2)
+      for (int R = 1; R <= kTcMaxRows; R *= 2)
         WithTc(i8, fp32, R, [](auto kernel, auto tag) {
           using Shape = typename decltype(tag)::type;
           Check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape::kSmem)),
@@ -345,7 +341,7 @@ AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_s
   // query rows of a request: exact for one query each, the average otherwise
   const int64_t queries = a->q_offsets ? (int64_t(a->total_queries) + a->batch - 1) / a->batch : 1;
   const int64_t rows = queries * group;
-  const int most = pl.tc ? TcMaxRows(fp32) : 8;
+  const int most = pl.tc ? kTcMaxRows : 8;
   while (pl.R < most && pl.R < rows) pl.R *= 2;
   int per_sm = 8;
   if (pl.tc)
@@ -428,11 +424,19 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   p.counts = a->page_counts;
   p.scale_log2 = static_cast<float>(double(a->scale) * 1.4426950408889634);
   p.causal = a->causal != 0;
-  p.window = a->window;
+  // a window of all places is none
+  p.window = a->window >= 1ll * a->max_pages_per_request * c->page_size ? 0 : a->window;
   p.status = a->status;
   p.ppt = p.P <= dsds::kTile ? dsds::kTile / p.P : 0;
   p.tpp = p.P <= dsds::kTile ? 0 : (p.P + dsds::kTile - 1) / dsds::kTile;
   p.R = pl.R;
+  p.by_page = dsds::divisor_of(p.P);
+  p.by_group = dsds::divisor_of(p.G);
+  p.by_block = dsds::divisor_of(p.bt);
+  p.by_tpp = dsds::divisor_of(std::max(1, p.tpp));
+  p.by_tile = dsds::divisor_of(std::max(1, p.ppt * p.P));
+  p.token_entries = (dsds::kTile + p.bt - 1) / p.bt + 1;
+  p.token_stages = std::min(dsds::kTokenStages, dsds::kTokenBytes / (12 * p.token_entries));
   p.ncta = pl.ncta;
   char* ws = static_cast<char*>(a->workspace);
   p.meta = reinterpret_cast<int4*>(ws);

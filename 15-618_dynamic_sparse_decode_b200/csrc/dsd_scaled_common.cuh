@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include "dsd_b200.h"
@@ -24,7 +25,25 @@ namespace dsds {
 
 constexpr int kTile = 128;          // tokens of a tile at most
 constexpr int kMaxBatch = 4096;     // plan: one int per request in shared memory
-constexpr float kTinyScale = 5.421010862427522e-20f;  // 2^-64, see token_scale()
+
+// Division of n < 2^31 by a fixed d >= 1: with 2^(l-1) < d <= 2^l and
+// m = ceil(2^(31+l) / d), floor(n m / 2^(31+l)) = floor(n / d), since the excess
+// n (m d - 2^(31+l)) / (d 2^(31+l)) stays below 1 / d.  Three instructions in
+// place of thirty: the walkers divide by these sizes all over.
+struct Divisor {
+  int d;
+  uint32_t m;
+  int shift;
+};
+inline Divisor divisor_of(int d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return {d, static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), 31 + l};
+}
+__device__ __forceinline__ int operator/(int n, const Divisor& v) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * v.m) >> v.shift);
+}
+__device__ __forceinline__ int operator%(int n, const Divisor& v) { return n - n / v * v.d; }
 
 struct AttnParams {
   const uint8_t* k;
@@ -50,6 +69,8 @@ struct AttnParams {
   int ppt;            // pages per tile (page_size <= 128), else 0
   int tpp;            // tiles per page (page_size > 128), else 0
   int R;              // query rows of a unit
+  Divisor by_page, by_group, by_block, by_tpp, by_tile;   // P, G, bt, tpp, ppt * P (1 where 0)
+  int token_entries, token_stages;   // of TokenRing
   int ncta;
   float* part_ml;     // [ncta][2][R][2]  running maximum (log2) and sum
   float* part_o;      // [ncta][2][R][D]
@@ -82,7 +103,7 @@ struct Request {
   int len;            // tokens, or listed pages when page_counts is given
 };
 
-__device__ __forceinline__ Request request_of(const AttnParams& p, int b) {
+__device__ __noinline__ Request request_of(const AttnParams& p, int b) {
   Request r;
   r.q0 = b;
   r.nq = 1;
@@ -99,28 +120,29 @@ __device__ __forceinline__ Request request_of(const AttnParams& p, int b) {
 
 // Tiles that hold `tokens` tokens of a request, and the tile of token t.
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int tokens) {
-  if (p.tpp) return tokens / p.P * p.tpp + (tokens % p.P + kTile - 1) / kTile;
-  const int tt = p.ppt * p.P;
-  return (tokens + tt - 1) / tt;
+  if (p.tpp) return tokens / p.by_page * p.tpp + (tokens % p.by_page + kTile - 1) / kTile;
+  return tokens == 0 ? 0 : (tokens - 1) / p.by_tile + 1;
 }
 __device__ __forceinline__ int tile_at(const AttnParams& p, int t) {
-  if (p.tpp) return t / p.P * p.tpp + t % p.P / kTile;
-  return t / (p.ppt * p.P);
+  if (p.tpp) return t / p.by_page * p.tpp + t % p.by_page / kTile;
+  return t / p.by_tile;
 }
 
-// The tiles that row tile qt (R rows) sees: the first one and how many.
+// The tiles that row tile qt (R rows) sees: the first one and how many.  Out of
+// line, as next_unit: several warp roles walk the units, and their code would
+// otherwise fill the instruction cache (200 KiB a kernel; a unit's first pass
+// through it took 15 us).
 struct Span { int first, n; };
 
-__device__ __forceinline__ Span span_of(const AttnParams& p, const Request& r, int qt) {
+__device__ __noinline__ Span span_of(const AttnParams& p, Request r, int qt) {
   if (p.counts) return {0, p.tpp ? r.len * p.tpp : (r.len + p.ppt - 1) / p.ppt};
-  const long long base = static_cast<long long>(r.len) - r.nq;
-  const long long row0 = 1ll * qt * p.R, row1 = min(static_cast<long long>(r.rows), row0 + p.R) - 1;
-  long long hi = r.len, lo = 0;
-  if (p.causal) hi = min(hi, max(0ll, base + row1 / p.G + 1));
-  if (p.window) lo = max(0ll, base + row0 / p.G - p.window + 1);
+  const int base = r.len - r.nq, row0 = qt * p.R, row1 = min(r.rows, row0 + p.R) - 1;
+  int hi = r.len, lo = 0;
+  if (p.causal) hi = min(hi, max(0, base + row1 / p.by_group + 1));
+  if (p.window) lo = max(0, max(base + row0 / p.by_group, -1) - p.window + 1);
   if (lo >= hi) return {0, 0};
-  const int t0 = tile_at(p, static_cast<int>(lo));
-  return {t0, tiles_of(p, static_cast<int>(hi)) - t0};
+  const int t0 = tile_at(p, lo);
+  return {t0, tiles_of(p, hi) - t0};
 }
 
 // A unit without a tile still takes a slot of the axis: its rows get zeros.
@@ -129,15 +151,30 @@ __device__ __forceinline__ int slots_of(const Span& s) { return max(1, s.n); }
 // Where a CTA stands: unit (b, h, qt), slot within the unit, slots left in its range.
 struct Walk {
   int b, h, qt, slot;
-  long long at, left;   // global slot, slots left
-  long long total;
+  int at, left;   // global slot, slots left
+  int total;
 };
+
+// The axis in p.ncta parts that differ by one slot at most (fewer where there are
+// fewer slots, so that no part between two that work is empty).
+struct Cut { int each, more, parts; };   // the first `more` parts have each + 1 slots
+__device__ __forceinline__ Cut cut_of(const AttnParams& p, int total) {
+  const int parts = min(total, p.ncta);
+  return {total / max(parts, 1), total % max(parts, 1), parts};
+}
+// The CTA whose range holds global slot s.
+__device__ __forceinline__ int cta_of(const AttnParams& p, int s, int total) {
+  const Cut c = cut_of(p, total);
+  const int wide = c.more * (c.each + 1);
+  return s < wide ? s / (c.each + 1) : c.more + (s - wide) / c.each;
+}
 
 // Every thread of the CTA calls it; wb has room for p.batch ints, w is shared.
 template <int THREADS>
 __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned bad = 0;
+#pragma unroll 1
   for (int b = p.q_off ? warp : tid; b < p.batch; b += p.q_off ? THREADS / 32 : THREADS) {
     const Request r = request_of(p, b);
     if (cta == 0 && p.status && (p.q_off == nullptr || lane == 0)) {
@@ -147,40 +184,49 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
       if (p.q_off && (p.q_off[b] != r.q0 || p.q_off[b + 1] != r.q0 + r.nq)) bad |= DSD_SCALED_BAD_LENGTH;
     }
     const int qts = (r.rows + p.R - 1) / p.R;
-    if (!p.q_off) {
-      // one query: every row tile sees the same tokens
-      wb[b] = qts * slots_of(span_of(p, r, 0));
-    } else {
-      int sum = 0;
-      for (int qt = lane; qt < qts; qt += 32) sum += slots_of(span_of(p, r, qt));
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      if (lane == 0) wb[b] = sum;
+    // one query: every row tile sees the same tokens; several: the lanes share the row tiles
+    int sum = 0;
+#pragma unroll 1
+    for (int qt = p.q_off ? lane : 0; qt < qts; qt += 32) {
+      sum += slots_of(span_of(p, r, qt));
+      if (!p.q_off) {
+        sum *= qts;
+        break;
+      }
     }
+    if (p.q_off) sum = __reduce_add_sync(~0u, sum);
+    if (!p.q_off || lane == 0) wb[b] = sum;
   }
-  if (bad) atomicOr(p.status, static_cast<int>(bad));
   __syncthreads();
   if (warp == 0) {
-    long long total = 0;
-    for (int b = lane; b < p.batch; b += 32) total += wb[b];
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-    total *= p.Hk;
-    // no CTA between the first and the last that works is without a slot
-    const long long parts = min(total, static_cast<long long>(p.ncta));
-    const long long lo = cta < parts ? total * cta / parts : 0, hi = cta < parts ? total * (cta + 1) / parts : 0;
+    long long all = 0;
+#pragma unroll 1
+    for (int b = lane; b < p.batch; b += 32) all += wb[b];
+#pragma unroll 1
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+    all *= p.Hk;
+    if (all > INT_MAX) {   // more than hours of work: refused
+      bad |= DSD_SCALED_BAD_LENGTH;
+      all = 0;
+    }
+    const int total = static_cast<int>(all);
+    const Cut c = cut_of(p, total);
     Walk x{};
-    x.at = lo;
-    x.left = hi - lo;
     x.total = total;
-    if (x.left > 0) {
-      long long before = 0;
+    if (cta < c.parts) {
+      x.at = cta * c.each + min(cta, c.more);
+      x.left = c.each + (cta < c.more);
+      int before = 0;
+#pragma unroll 1
       for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const long long mine = b0 + lane < p.batch ? 1ll * wb[b0 + lane] * p.Hk : 0;
-        long long upto = mine;
+        const int mine = b0 + lane < p.batch ? wb[b0 + lane] * p.Hk : 0;
+        int upto = mine;
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-          const long long y = __shfl_up_sync(~0u, upto, o);
+          const int y = __shfl_up_sync(~0u, upto, o);
           if (lane >= o) upto += y;
         }
-        const unsigned past = __ballot_sync(~0u, before + upto > lo);
+        const unsigned past = __ballot_sync(~0u, before + upto > x.at);
         if (past) {
           const int l = __ffs(past) - 1;
           x.b = b0 + l;
@@ -190,8 +236,8 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
         before += __shfl_sync(~0u, upto, 31);
       }
       const int w1 = wb[x.b];
-      const int rest = static_cast<int>((lo - before) % w1);
-      x.h = static_cast<int>((lo - before) / w1);
+      const int rest = (x.at - before) % w1;
+      x.h = (x.at - before) / w1;
       const Request r = request_of(p, x.b);
       const int qts = (r.rows + p.R - 1) / p.R;
       if (!p.q_off) {
@@ -200,9 +246,11 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
         x.slot = rest % per;
       } else {
         int sum = 0;
+#pragma unroll 1
         for (int q0 = 0; q0 < qts; q0 += 32) {
           const int mine = q0 + lane < qts ? slots_of(span_of(p, r, q0 + lane)) : 0;
           int upto = mine;
+#pragma unroll 1
           for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(~0u, upto, o);
             if (lane >= o) upto += y;
@@ -220,21 +268,8 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
     }
     if (lane == 0) *w = x;
   }
+  if (bad && cta == 0 && p.status) atomicOr(p.status, static_cast<int>(bad));
   __syncthreads();
-}
-
-// To the first slot of the next unit.
-__device__ __forceinline__ void next_unit(const AttnParams& p, Request& r, Walk& w) {
-  w.slot = 0;
-  if (++w.qt < (r.rows + p.R - 1) / p.R) return;
-  w.qt = 0;
-  if (++w.h < p.Hk) return;
-  w.h = 0;
-  do {
-    ++w.b;
-    if (w.b >= p.batch) return;
-    r = request_of(p, w.b);
-  } while (r.rows == 0);
 }
 
 // The part of a unit that a CTA does, and where its result goes.
@@ -247,15 +282,27 @@ struct Segment {
 __device__ __forceinline__ Segment segment_of(const Walk& w, int slots) {
   Segment s;
   s.first = w.slot;
-  s.n = static_cast<int>(min(w.left, static_cast<long long>(slots - w.slot)));
+  s.n = min(w.left, slots - w.slot);
   s.opens = w.slot == 0;
   s.ends = w.slot + s.n == slots;
   return s;
 }
 
-// The CTA whose range holds global slot s.
-__device__ __forceinline__ int cta_of(const AttnParams& p, long long s, long long total) {
-  return static_cast<int>(((s + 1) * min(total, static_cast<long long>(p.ncta)) - 1) / total);
+// Past a segment, to the first slot of the next unit.
+__device__ __noinline__ void next_unit(const AttnParams& p, const Segment& seg, Request& r, Walk& w) {
+  w.at += seg.n;
+  w.left -= seg.n;
+  if (w.left <= 0) return;
+  w.slot = 0;
+  if (++w.qt < (r.rows + p.R - 1) / p.R) return;
+  w.qt = 0;
+  if (++w.h < p.Hk) return;
+  w.h = 0;
+  do {
+    ++w.b;
+    if (w.b >= p.batch) return;
+    r = request_of(p, w.b);
+  } while (r.rows == 0);
 }
 
 // Token i (0..127) of a unit's tile: its page (-1: none), slot in the page, place in the request.
@@ -265,13 +312,13 @@ __device__ __forceinline__ Token token_of(const AttnParams& p, const Request& r,
   Token t{-1, 0, -1};
   int entry;
   if (p.tpp) {
-    entry = tile / p.tpp;
-    t.slot = tile % p.tpp * kTile + i;
+    entry = tile / p.by_tpp;
+    t.slot = tile % p.by_tpp * kTile + i;
     if (t.slot >= p.P) return t;
   } else {
     if (i >= p.ppt * p.P) return t;
-    entry = tile * p.ppt + i / p.P;
-    t.slot = i % p.P;
+    entry = tile * p.ppt + i / p.by_page;
+    t.slot = i % p.by_page;
   }
   const long long place = 1ll * entry * p.P + t.slot;
   if (p.counts ? entry >= r.len : place >= r.len) return t;
@@ -289,26 +336,30 @@ __device__ __forceinline__ Token token_of(const AttnParams& p, const Request& r,
 // Whether query row `row` of the request sees the token at `place`.
 __device__ __forceinline__ bool sees(const AttnParams& p, const Request& r, int row, long long place) {
   if (row >= r.rows) return false;
-  const long long pos = static_cast<long long>(r.len) - r.nq + row / p.G;
+  const long long pos = static_cast<long long>(r.len) - r.nq + row / p.by_group;
   if (p.causal && place > pos) return false;
   return !p.window || place > pos - p.window;
 }
 
 __device__ __forceinline__ long long scale_index(const AttnParams& p, int page, int h, int slot) {
-  return (1ll * page * p.Hk + h) * p.nblk + slot / p.bt;
+  return (1ll * page * p.Hk + h) * p.nblk + slot / p.by_block;
 }
 
-// Weights carry the value scale: w = 2^(s + log2 vs - m) <= 1 for the running
-// maximum m of s + log2 vs, so that the largest CONTRIBUTION, not the largest
-// probability, is 1 when weights are cut into 8-bit pieces; the softmax sum gets
-// w / vs.  A scale below 2^-64 counts as 2^-64 in the exponent and keeps its own
-// value through the factor, so the sum cannot overflow and a zero scale adds
-// nothing to the output.
-struct TokenScale { float log2, inverse, factor; };
+// Weights carry the value scale: with vs = f 2^e, 1 <= f < 2, and the running
+// maximum m of s + e, w = 2^(s + e - m) <= 1 is the size of a token's CONTRIBUTION:
+// its value codes are weighted by w f, and the softmax sum gets w 2^-e.  Cut into
+// 8-bit pieces, a weight thus keeps its bits where the output needs them.  All of
+// it is exact.  e stays in [-64, 100], so that the sum cannot overflow: a smaller
+// scale makes f small, a zero scale adds nothing.  A scale that is not finite
+// makes e NaN, and with it the logit of a row that sees the token; f stays finite
+// for the rows that do not.
+struct TokenScale { float e, inverse, factor; };
 
 __device__ __forceinline__ TokenScale token_scale(float vs) {
-  const float v = vs < kTinyScale ? kTinyScale : vs;   // NaN stays
-  return {log2f(v), 1.0f / v, vs < kTinyScale ? vs * (1.0f / kTinyScale) : 1.0f};
+  const int e = min(max(static_cast<int>(__float_as_uint(vs) >> 23 & 255) - 127, -64), 100);
+  const float inverse = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  const float off = vs - vs;   // 0 or NaN
+  return {static_cast<float>(e) + off, inverse, off == 0.0f ? vs * inverse : 1.0f};
 }
 
 constexpr float kLn2 = 0.6931471805599453f;
@@ -316,14 +367,14 @@ constexpr float kLn2 = 0.6931471805599453f;
 // One output row from its (m, l, O) state; thread-wise over elements d.
 __device__ __forceinline__ void write_row_elem(const AttnParams& p, const Request& r, int h, int row,
                                                int d, float o, float l) {
-  const int qi = row / p.G, head = h * p.G + row % p.G;
+  const int qi = row / p.by_group, head = h * p.G + row % p.by_group;
   const long long i = 1ll * (r.q0 + qi) * p.ost[0] + 1ll * head * p.ost[1] + d;
   store_elem(p.out, i, p.dtype, l == 0.0f ? 0.0f : o / l);
 }
 __device__ __forceinline__ void write_row_lse(const AttnParams& p, const Request& r, int h, int row,
                                               float m, float l) {
   if (!p.lse) return;
-  const int qi = row / p.G, head = h * p.G + row % p.G;
+  const int qi = row / p.by_group, head = h * p.G + row % p.by_group;
   p.lse[1ll * (r.q0 + qi) * p.H + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
