@@ -36,12 +36,13 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cta = blockIdx.x;
 
-  plan_walk<kSimpleThreads>(p, cta, wb, &walk_s);
+  const int head = cta % p.Hk;
+  plan_walk<kSimpleThreads>(p, cta / p.Hk, wb, &walk_s);
   Walk w = walk_s;
-  if (tid == 0) p.meta[cta] = make_int4(0, 0, 0, -1);
+  if (tid == 0) p.meta[cta] = make_int4(0, 0, -1, 0);
   if (w.left == 0) return;
-  Request r = request_of(p, w.b);
   while (w.left > 0) {
+    const Request r = w.r;
     const Span span = span_of(p, r, w.qt);
     const int slots = slots_of(span);
     const Segment seg = segment_of(w, slots);
@@ -50,7 +51,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
       const int row = row0 + i / p.D, d = i % p.D;
       float x = 0.0f;
       if (row < r.rows)
-        x = load_elem(p.q, 1ll * (r.q0 + row / p.by_group) * p.qst[0] + 1ll * (w.h * p.G + row % p.by_group) * p.qst[1] + d, p.dtype);
+        x = load_elem(p.q, 1ll * (r.q0 + row / p.by_group) * p.qst[0] + 1ll * (head * p.G + row % p.by_group) * p.qst[1] + d, p.dtype);
       q_s[i] = x;
     }
     if (tid < R) {
@@ -67,10 +68,10 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
       for (int j = 0; j < R; ++j) s[j] = 0.0f;
       TokenScale ts{0.0f, 0.0f, 0.0f};
       if (t.page >= 0) {
-        const long long si = scale_index(p, t.page, w.h, t.slot);
+        const long long si = scale_index(p, t.page, head, t.slot);
         ts = token_scale(p.vs[si]);
         const float ks = p.ks[si];
-        const uint8_t* row = p.k + t.page * p.kst[0] + t.slot * p.kst[1] + w.h * p.kst[2];
+        const uint8_t* row = p.k + t.page * p.kst[0] + t.slot * p.kst[1] + head * p.kst[2];
         for (int d = 0; d < p.D; ++d) {
           const float x = code_value<I8>(row[d]);
 #pragma unroll
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
       for (int k = 0; k < kTile; ++k) {
         const int page = page_s[k];
         if (page < 0) continue;
-        const uint8_t* row = p.v + page * p.vst[0] + slot_s[k] * p.vst[1] + w.h * p.vst[2];
+        const uint8_t* row = p.v + page * p.vst[0] + slot_s[k] * p.vst[1] + head * p.vst[2];
         const float x0 = tid < p.D ? code_value<I8>(row[tid]) : 0.0f;
         const float x1 = tid + kSimpleThreads < p.D ? code_value<I8>(row[tid + kSimpleThreads]) : 0.0f;
 #pragma unroll
@@ -135,14 +136,14 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
     if (seg.whole()) {
       for (int j = 0; j < R && row0 + j < r.rows; ++j) {
         const float l = l_s[j];
-        if (tid == 0) write_row_lse(p, r, w.h, row0 + j, m_s[j], l);
+        if (tid == 0) write_row_lse(p, r, head, row0 + j, m_s[j], l);
       }
 #pragma unroll
       for (int j = 0; j < R; ++j)
         if (row0 + j < r.rows) {
-          if (tid < p.D) write_row_elem(p, r, w.h, row0 + j, tid, acc[j][0], l_s[j]);
+          if (tid < p.D) write_row_elem(p, r, head, row0 + j, tid, acc[j][0], l_s[j]);
           if (tid + kSimpleThreads < p.D)
-            write_row_elem(p, r, w.h, row0 + j, tid + kSimpleThreads, acc[j][1], l_s[j]);
+            write_row_elem(p, r, head, row0 + j, tid + kSimpleThreads, acc[j][1], l_s[j]);
         }
     } else {
       const long long at = (2ll * cta + seg.opens) * R;
@@ -156,9 +157,9 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
         }
       }
       if (seg.opens && tid == 0)
-        p.meta[cta] = make_int4(w.b, w.h, w.qt, cta_of(p, w.at + slots - 1, w.total));
+        p.meta[cta] = make_int4(w.b, w.qt, gang_of(p, w.at + slots - 1, w.total), 0);
     }
-    next_unit(p, seg, r, w);
+    next_unit(p, seg, w);
     __syncthreads();
   }
 }

@@ -213,10 +213,10 @@ __device__ __forceinline__ bool row_has_nan(const uint4* row, int lane) {
 // What the softmax warps know of a unit, from warp 7.
 struct UnitInfo {
   int tiles;          // -1: the range ends
-  int b, h, qt;
+  int b, qt;
   int rows;           // query rows from the unit's first on
   int opens, ends;    // the segment has the unit's first / last slot
-  int last_cta;
+  int last_gang;
 };
 
 // Token data of a tile, from warp 6.  A scale covers a block of bt tokens, so a
@@ -338,7 +338,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
   __shared__ int stop;
   __shared__ Walk walk_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cta = blockIdx.x;
+  const int cta = blockIdx.x, head = cta % p.Hk;
 
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -363,10 +363,10 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
     mbar_init(&drained, 1);
     stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    p.meta[cta] = make_int4(0, 0, 0, -1);
+    p.meta[cta] = make_int4(0, 0, -1, 0);
   }
   // the plan's scratch lies in the ring, which nothing fills before the barrier in it
-  plan_walk<kTcThreads>(p, cta, reinterpret_cast<int*>(k_ring), &walk_s);
+  plan_walk<kTcThreads>(p, cta / p.Hk, reinterpret_cast<int*>(k_ring), &walk_s);
   Walk w = walk_s;
   if (w.left == 0) return;
   proxy_fence();   // the scratch's generic writes, before TMA writes the same bytes
@@ -382,12 +382,12 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
 
   if (warp == 4) {
     // ---- TMA: the pages of a tile, one box each, K then V
-    Request r = request_of(p, w.b);
     const int rows = p.tpp ? kTile : p.P, boxes = p.tpp ? 1 : p.ppt;
     uint32_t g = 0;
     bool ok = true;
 #pragma unroll 1
     while (w.left > 0 && ok) {
+      const Request r = w.r;
       const Span span = span_of(p, r, w.qt);
       const Segment seg = segment_of(w, slots_of(span));
       const int tiles = span.n == 0 ? 0 : seg.n;
@@ -402,7 +402,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         const int bytes = __popc(__ballot_sync(~0u, good)) * rows * 128;
         const int s = g % STAGES, parity = (g / STAGES & 1) ^ 1;
         const int slot = p.tpp ? tile % p.by_tpp * kTile : 0;
-        const int c1 = head_first ? w.h : slot, c2 = head_first ? slot : w.h;
+        const int c1 = head_first ? head : slot, c2 = head_first ? slot : head;
         const uint32_t at = s * kTcTileBytes + lane * rows * 128;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -415,7 +415,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
           if (good) tma_box(kv ? &v_map : &k_map, smem_addr(kv ? v_ring : k_ring) + at, full, c1, c2, page);
         }
       }
-      next_unit(p, seg, r, w);
+      next_unit(p, seg, w);
     }
     // after a time-out: the copies still in flight land before the block's memory is given back
     if (!ok && lane == 0) {
@@ -491,11 +491,11 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
   } else if (warp == 6) {
     // ---- token data; a lane has every 32nd entry of a tile
     const TokenRing ring(token_smem, p);
-    Request r = request_of(p, w.b);
     int s = 0, phase = 0;   // of the token ring
     bool ok = true;
 #pragma unroll 1
     while (w.left > 0 && ok) {
+      const Request r = w.r;
       const Span span = span_of(p, r, w.qt);
       const Segment seg = segment_of(w, slots_of(span));
       const int tiles = span.n == 0 ? 0 : seg.n;
@@ -531,7 +531,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
                 limit = 0;
               } else {
                 if (p.counts) limit = min(max(p.counts[page] - slot, 0), p.bt);
-                const long long si = (1ll * page * p.Hk + w.h) * p.nblk + slot / p.by_block;
+                const long long si = (1ll * page * p.Hk + head) * p.nblk + slot / p.by_block;
                 float2* to = ring.scales + s * ring.entries + e;
                 copy4_async(&to->x, p.ks + si);
                 copy4_async(&to->y, p.vs + si);
@@ -551,12 +551,11 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
           phase ^= 1;
         }
       }
-      next_unit(p, seg, r, w);
+      next_unit(p, seg, w);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 7) {
     // ---- queries, cut into pieces; a lane takes four elements of every row
-    Request r = request_of(p, w.b);
     const int elem = p.dtype == DSD_TYPE_F32 ? 4 : 2;
     const bool aligned = reinterpret_cast<uintptr_t>(p.q) % (4 * elem) == 0 && p.qst[0] % 4 == 0 && p.qst[1] % 4 == 0;
     bool ok = true;
@@ -564,6 +563,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
     for (uint32_t unit = 0; ok; ++unit) {
       const int u = unit & 1;
       const bool end = w.left <= 0;
+      const Request r = w.r;
       Span span{0, 0};
       if (!end) span = span_of(p, r, w.qt);
       const int slots = slots_of(span);
@@ -571,8 +571,8 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
       const int row0 = w.qt * R, base_pos = r.len - r.nq;
       // lane = row: where it lies and what it sees
       const int gr = min(row0 + lane, r.rows - 1);
-      const int qi = gr / p.by_group, head = w.h * p.G + gr % p.by_group;
-      const long long at = 1ll * (r.q0 + qi) * p.qst[0] + 1ll * head * p.qst[1];
+      const int qi = gr / p.by_group, q_head = head * p.G + gr % p.by_group;
+      const long long at = 1ll * (r.q0 + qi) * p.qst[0] + 1ll * q_head * p.qst[1];
       const bool in_row = 4 * lane < p.D;   // head_dim is a multiple of 16 here
       uint4 raw[R];
       if (!end) {
@@ -595,26 +595,25 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         }
         if (lane < R) {
           row_pos[u][lane] = base_pos + qi;
-          row_out[u][lane] = 1ll * (r.q0 + qi) * p.ost[0] + 1ll * head * p.ost[1];
-          row_lse[u][lane] = (r.q0 + qi) * p.H + head;
+          row_out[u][lane] = 1ll * (r.q0 + qi) * p.ost[0] + 1ll * q_head * p.ost[1];
+          row_lse[u][lane] = (r.q0 + qi) * p.H + q_head;
         }
       }
       if (lane == 0) {
         UnitInfo& x = units[u];
         x.tiles = end ? -1 : span.n == 0 ? 0 : seg.n;
         x.b = w.b;
-        x.h = w.h;
         x.qt = w.qt;
         x.rows = r.rows - row0;
         x.opens = seg.opens;
         x.ends = seg.ends;
-        x.last_cta = end ? 0 : cta_of(p, w.at - w.slot + slots - 1, w.total);
+        x.last_gang = end ? 0 : gang_of(p, w.at - w.slot + slots - 1, w.total);
       }
       proxy_fence();
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_full[u]);
       if (end) break;
-      next_unit(p, seg, r, w);
+      next_unit(p, seg, w);
     }
   } else {
     // ---- softmax
@@ -807,7 +806,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
           }
         }
       }
-      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.h, x.qt, x.last_cta);
+      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.qt, x.last_gang, 0);
       // `red` is written again behind the barrier at the next unit's start
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[u]);

@@ -57,7 +57,7 @@ void CheckCache(const dsd_scaled_cache* c) {
     Fail(DSD_EINVAL, "kv_format must be DSD_KV_FP8_SCALED or DSD_KV_I8_SCALED");
   if (c->num_pages <= 0) Fail(DSD_EINVAL, "num_pages must be positive");
   if (c->page_size < 1 || c->page_size > 4096) Fail(DSD_EINVAL, "page_size must be in [1, 4096]");
-  if (c->num_kv_heads < 1 || c->num_kv_heads > 1024) Fail(DSD_EINVAL, "num_kv_heads must be in [1, 1024]");
+  if (c->num_kv_heads < 1 || c->num_kv_heads > 128) Fail(DSD_EINVAL, "num_kv_heads must be in [1, 128]");
   if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8)
     Fail(DSD_EINVAL, "head_dim must be a multiple of 8 in [8, 256]");
   if (c->block_tokens < 1 || c->block_tokens > 256 || c->page_size % c->block_tokens)
@@ -329,7 +329,7 @@ CUtensorMap MapOf(const dsd_scaled_cache* c, const void* codes, const CodeOrder&
 struct AttnPlan {
   bool tc = false;
   TcMaps maps;
-  int R = 1, ncta = 0;
+  int R = 1, ncta = 0, gangs = 0;
   int64_t ml_at = 0, o_at = 0, bytes = 0;   // workspace: meta, then ml, then O
 };
 
@@ -346,7 +346,8 @@ AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_s
   int per_sm = 8;
   if (pl.tc)
     WithTc(i8, fp32, pl.R, [&](auto, auto tag) { per_sm = decltype(tag)::type::kCtas; });
-  pl.ncta = per_sm * dev.sms;
+  pl.gangs = std::max(1, per_sm * dev.sms / c->num_kv_heads);
+  pl.ncta = pl.gangs * c->num_kv_heads;
   pl.ml_at = (int64_t(pl.ncta) * 16 + 255) / 256 * 256;
   pl.o_at = pl.ml_at + (int64_t(pl.ncta) * 2 * pl.R * 8 + 255) / 256 * 256;
   pl.bytes = pl.o_at + int64_t(pl.ncta) * 2 * pl.R * c->head_dim * 4;
@@ -438,6 +439,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   p.token_entries = (dsds::kTile + p.bt - 1) / p.bt + 1;
   p.token_stages = std::min(dsds::kTokenStages, dsds::kTokenBytes / (12 * p.token_entries));
   p.ncta = pl.ncta;
+  p.gangs = pl.gangs;
   char* ws = static_cast<char*>(a->workspace);
   p.meta = reinterpret_cast<int4*>(ws);
   p.part_ml = reinterpret_cast<float*>(ws + pl.ml_at);

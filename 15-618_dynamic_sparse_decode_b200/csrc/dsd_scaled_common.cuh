@@ -4,12 +4,17 @@
 //
 // Attention splits the KEY axis: a unit is one request, one key head and R
 // consecutive query rows (row = query * group + head of the group); it walks the
-// tiles of up to 128 tokens that its rows see.  All units' tiles in a row form
-// one axis, which is cut into equal contiguous ranges, one per CTA, so that one
-// long request fills the machine and a ragged batch leaves no CTA idle.  A CTA
-// derives its range from the lengths on the device (no host knowledge of them,
-// so a captured graph follows them); a unit that spans CTAs leaves partial
-// results, at most two per CTA, which combine_kernel joins in tile order.
+// tiles of up to 128 tokens that its rows see.  All units' tiles of a head in a
+// row form one axis, which is cut into equal contiguous ranges, so that one long
+// request fills the machine and a ragged batch leaves no CTA idle.  A range is
+// walked by a gang of CTAs at once, one for each key head: in a token-major pool
+// the heads' rows of a token are neighbours in memory, and CTAs that read them at
+// about the same time keep DRAM in its open pages (64 requests x 16-32k: 595 us
+// with the heads one after another along the axis, see the table in the design
+// notes for the gang's).  A CTA derives its range from the lengths on the device
+// (no host knowledge of them, so a captured graph follows them); a unit that spans
+// ranges leaves partial results, at most two per CTA, which combine_kernel joins
+// in tile order.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -71,10 +76,10 @@ struct AttnParams {
   int R;              // query rows of a unit
   Divisor by_page, by_group, by_block, by_tpp, by_tile;   // P, G, bt, tpp, ppt * P (1 where 0)
   int token_entries, token_stages;   // of TokenRing
-  int ncta;
+  int ncta, gangs;    // ncta = gangs * Hk; CTA = gang * Hk + head
   float* part_ml;     // [ncta][2][R][2]  running maximum (log2) and sum
   float* part_o;      // [ncta][2][R][D]
-  int4* meta;         // [ncta]  unit a CTA leaves open: request, head, row tile, last CTA (-1: none)
+  int4* meta;         // [ncta]  unit a CTA leaves open: request, row tile, last gang (-1: none)
 };
 
 __device__ __forceinline__ float load_elem(const void* p, long long i, int dtype) {
@@ -148,22 +153,23 @@ __device__ __noinline__ Span span_of(const AttnParams& p, Request r, int qt) {
 // A unit without a tile still takes a slot of the axis: its rows get zeros.
 __device__ __forceinline__ int slots_of(const Span& s) { return max(1, s.n); }
 
-// Where a CTA stands: unit (b, h, qt), slot within the unit, slots left in its range.
+// Where a gang stands: unit (b, qt), slot within the unit, slots left in its range.
 struct Walk {
-  int b, h, qt, slot;
-  int at, left;   // global slot, slots left
+  int b, qt, slot;
+  int at, left;   // slot of the axis, slots left
   int total;
+  Request r;      // of b
 };
 
-// The axis in p.ncta parts that differ by one slot at most (fewer where there are
+// The axis in p.gangs parts that differ by one slot at most (fewer where there are
 // fewer slots, so that no part between two that work is empty).
 struct Cut { int each, more, parts; };   // the first `more` parts have each + 1 slots
 __device__ __forceinline__ Cut cut_of(const AttnParams& p, int total) {
-  const int parts = min(total, p.ncta);
+  const int parts = min(total, p.gangs);
   return {total / max(parts, 1), total % max(parts, 1), parts};
 }
-// The CTA whose range holds global slot s.
-__device__ __forceinline__ int cta_of(const AttnParams& p, int s, int total) {
+// The gang whose range holds slot s.
+__device__ __forceinline__ int gang_of(const AttnParams& p, int s, int total) {
   const Cut c = cut_of(p, total);
   const int wide = c.more * (c.each + 1);
   return s < wide ? s / (c.each + 1) : c.more + (s - wide) / c.each;
@@ -171,13 +177,13 @@ __device__ __forceinline__ int cta_of(const AttnParams& p, int s, int total) {
 
 // Every thread of the CTA calls it; wb has room for p.batch ints, w is shared.
 template <int THREADS>
-__device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
+__device__ void plan_walk(const AttnParams& p, int gang, int* wb, Walk* w) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned bad = 0;
 #pragma unroll 1
   for (int b = p.q_off ? warp : tid; b < p.batch; b += p.q_off ? THREADS / 32 : THREADS) {
     const Request r = request_of(p, b);
-    if (cta == 0 && p.status && (p.q_off == nullptr || lane == 0)) {
+    if (blockIdx.x == 0 && p.status && (p.q_off == nullptr || lane == 0)) {
       const long long most = p.counts ? p.max_pages : 1ll * p.max_pages * p.P;
       if (p.lens[b] < 0) bad |= DSD_SCALED_BAD_LENGTH;
       if (p.lens[b] > most) bad |= DSD_SCALED_BAD_PAGE;
@@ -204,7 +210,6 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
     for (int b = lane; b < p.batch; b += 32) all += wb[b];
 #pragma unroll 1
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
-    all *= p.Hk;
     if (all > INT_MAX) {   // more than hours of work: refused
       bad |= DSD_SCALED_BAD_LENGTH;
       all = 0;
@@ -213,13 +218,13 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
     const Cut c = cut_of(p, total);
     Walk x{};
     x.total = total;
-    if (cta < c.parts) {
-      x.at = cta * c.each + min(cta, c.more);
-      x.left = c.each + (cta < c.more);
+    if (gang < c.parts) {
+      x.at = gang * c.each + min(gang, c.more);
+      x.left = c.each + (gang < c.more);
       int before = 0;
 #pragma unroll 1
       for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int mine = b0 + lane < p.batch ? wb[b0 + lane] * p.Hk : 0;
+        const int mine = b0 + lane < p.batch ? wb[b0 + lane] : 0;
         int upto = mine;
 #pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
@@ -235,13 +240,11 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
         }
         before += __shfl_sync(~0u, upto, 31);
       }
-      const int w1 = wb[x.b];
-      const int rest = (x.at - before) % w1;
-      x.h = (x.at - before) / w1;
-      const Request r = request_of(p, x.b);
+      const int rest = x.at - before;
+      const Request r = x.r = request_of(p, x.b);
       const int qts = (r.rows + p.R - 1) / p.R;
       if (!p.q_off) {
-        const int per = w1 / qts;
+        const int per = wb[x.b] / qts;
         x.qt = rest / per;
         x.slot = rest % per;
       } else {
@@ -268,7 +271,7 @@ __device__ void plan_walk(const AttnParams& p, int cta, int* wb, Walk* w) {
     }
     if (lane == 0) *w = x;
   }
-  if (bad && cta == 0 && p.status) atomicOr(p.status, static_cast<int>(bad));
+  if (bad && blockIdx.x == 0 && p.status) atomicOr(p.status, static_cast<int>(bad));
   __syncthreads();
 }
 
@@ -289,20 +292,18 @@ __device__ __forceinline__ Segment segment_of(const Walk& w, int slots) {
 }
 
 // Past a segment, to the first slot of the next unit.
-__device__ __noinline__ void next_unit(const AttnParams& p, const Segment& seg, Request& r, Walk& w) {
+__device__ __noinline__ void next_unit(const AttnParams& p, const Segment& seg, Walk& w) {
   w.at += seg.n;
   w.left -= seg.n;
   if (w.left <= 0) return;
   w.slot = 0;
-  if (++w.qt < (r.rows + p.R - 1) / p.R) return;
+  if (++w.qt < (w.r.rows + p.R - 1) / p.R) return;
   w.qt = 0;
-  if (++w.h < p.Hk) return;
-  w.h = 0;
   do {
     ++w.b;
     if (w.b >= p.batch) return;
-    r = request_of(p, w.b);
-  } while (r.rows == 0);
+    w.r = request_of(p, w.b);
+  } while (w.r.rows == 0);
 }
 
 // Token i (0..127) of a unit's tile: its page (-1: none), slot in the page, place in the request.
@@ -378,34 +379,36 @@ __device__ __forceinline__ void write_row_lse(const AttnParams& p, const Request
   p.lse[1ll * (r.q0 + qi) * p.H + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// Joins the partial results of the units that span CTAs.  Block (c, g) looks
+// Joins the partial results of the units that span ranges.  Block (c, g) looks
 // after rows g, g + gridDim.y, ... of the unit CTA c leaves open: the opener's
-// piece is its slot 1, every following CTA's is its slot 0, added in CTA order,
-// so the result does not depend on timing.  256 threads cover head_dim <= 256.
+// piece is its slot 1, the slot 0 of the same head's CTA in every following gang
+// the rest, added in that order, so the result does not depend on timing.
+// head_dim <= 256 threads.
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x, d = threadIdx.x;
   const int4 u = p.meta[c];
-  if (u.w < 0) return;
+  if (u.z < 0) return;
   const Request r = request_of(p, u.x);
+  const int head = c % p.Hk, pieces = u.z - c / p.Hk + 1;
   for (int row = blockIdx.y; row < p.R; row += gridDim.y) {
-    const int global_row = u.z * p.R + row;
+    const int global_row = u.y * p.R + row;
     if (global_row >= r.rows) return;
-    const auto piece = [&](int cta) { return (2ll * cta + (cta == c)) * p.R + row; };
+    const auto piece = [&](int i) { return (2ll * (c + i * p.Hk) + (i == 0)) * p.R + row; };
     float m = -INFINITY;
-    for (int i = c; i <= u.w; ++i) m = fmaxf(m, p.part_ml[2 * piece(i)]);
+    for (int i = 0; i < pieces; ++i) m = fmaxf(m, p.part_ml[2 * piece(i)]);
     const float m0 = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o = 0.0f;
 #pragma unroll 4
-    for (int i = c; i <= u.w; ++i) {
+    for (int i = 0; i < pieces; ++i) {
       const long long at = piece(i);
       const float f = exp2f(p.part_ml[2 * at] - m0);
       l += f * p.part_ml[2 * at + 1];
       // a piece none of whose tokens this row saw holds zeros: f is 0 there
       if (d < p.D) o += f * p.part_o[at * p.D + d];
     }
-    if (d < p.D) write_row_elem(p, r, u.y, global_row, d, o, l);
-    if (d == 0) write_row_lse(p, r, u.y, global_row, m0, l);
+    if (d < p.D) write_row_elem(p, r, head, global_row, d, o, l);
+    if (d == 0) write_row_lse(p, r, head, global_row, m0, l);
   }
 }
 

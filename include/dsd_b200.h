@@ -353,7 +353,7 @@ typedef struct dsd_scaled_cache {
   int32_t kv_format;      /* DSD_KV_FP8_SCALED or DSD_KV_I8_SCALED */
   int32_t num_pages;
   int32_t page_size;      /* 1..4096 tokens */
-  int32_t num_kv_heads;
+  int32_t num_kv_heads;   /* 1..128 */
   int32_t head_dim;       /* a multiple of 8, 8..256 */
   int32_t block_tokens;   /* divides page_size, at most 256 */
   void* k_codes;
