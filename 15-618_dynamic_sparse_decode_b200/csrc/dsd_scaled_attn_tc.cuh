@@ -146,6 +146,12 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -429,65 +435,92 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
       }
     }
   } else if (warp == 5) {
-    // ---- MMA issue (one lane)
-    if (lane == 0) {
-      constexpr uint32_t s_desc = mma_desc<I8, N>(false), o_desc = mma_desc<I8, N>(true);
-      uint32_t g = 0;
-      bool ok = true;
-      const auto weigh = [&](uint32_t t) {   // O^T of tile t
-        const int s = t % STAGES, buf = t & 1;
-        ok = ok && mbar_wait(&p_full[buf], t >> 1 & 1, &stop, p.status) &&
-             mbar_wait(&v_full[s], t / STAGES & 1, &stop, p.status) &&
-             mbar_wait(&o_empty[buf], (t >> 1 & 1) ^ 1, &stop, p.status);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t a = operand_desc(smem_addr(v_ring + s * kTcTileBytes));
-        const uint64_t b = operand_desc(smem_addr(p_op + buf * Shape::kOperand));
-#pragma unroll 1
+    // ---- MMA issue: the warp waits as one, so that descriptors stay in uniform
+    // registers, and one lane issues
+    constexpr uint32_t s_desc = mma_desc<I8, N>(false), o_desc = mma_desc<I8, N>(true);
+    const bool leader = elect_one();
+    const uint64_t k_d = operand_desc(smem_addr(k_ring)), v_d = operand_desc(smem_addr(v_ring));
+    const uint64_t q_d = operand_desc(smem_addr(q_op)), p_d = operand_desc(smem_addr(p_op));
+    const auto all = [&](uint64_t* bar, int parity) { return __all_sync(~0u, mbar_wait(bar, parity, &stop, p.status)) != 0; };
+    uint32_t g = 0;
+    int ks = 0, kp = 0, vs = 0, vp = 0;   // ring stage and phase of K and of V
+    bool ok = true, owed = false;         // owed: O^T of tile g - 1 is still to be issued
+    const auto weigh = [&]() {
+      const int t = g - 1, buf = t & 1;
+      owed = false;
+      ok = ok && all(&p_full[buf], t >> 1 & 1) && all(&v_full[vs], vp) && all(&o_empty[buf], (t >> 1 & 1) ^ 1);
+      if (!ok) return;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t a = v_d + vs * (kTcTileBytes >> 4), b = p_d + buf * (Shape::kOperand >> 4);
+#pragma unroll
         for (int k = 0; k < 4; ++k) mma<I8>(tmem + 2 * N + buf * N, a + 256 * k, b + 2 * k, o_desc, k > 0);
-        mma_commit(&v_empty[s]);
+        mma_commit(&v_empty[vs]);
         mma_commit(&o_full[buf]);
-      };
-      bool owed = false;   // the last tile's O^T is still to be issued
-#pragma unroll 1
-      for (uint32_t unit = 0; ok; ++unit) {
-        const int u = unit & 1;
-        // the queries are ready ahead of time, except for the first units
-        if (owed && !mbar_try(&unit_full[u], unit >> 1 & 1)) {
-          weigh(g - 1);
-          owed = false;
-        }
-        ok = ok && mbar_wait(&unit_full[u], unit >> 1 & 1, &stop, p.status);
-        if (!ok) break;
-        const int tiles = units[u].tiles;
-        mbar_arrive(&unit_empty[u]);
-        if (tiles < 0) break;
-        const uint64_t q_d = operand_desc(smem_addr(q_op + u * Shape::kOperand));
-#pragma unroll 1
-        for (int i = 0; i < tiles && ok; ++i, ++g) {
-          const int s = g % STAGES, buf = g & 1;
-          ok = ok && mbar_wait(&k_full[s], g / STAGES & 1, &stop, p.status) &&
-               mbar_wait(&s_empty[buf], (g >> 1 & 1) ^ 1, &stop, p.status);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t a = operand_desc(smem_addr(k_ring + s * kTcTileBytes));
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) mma<I8>(tmem + buf * N, a + 2 * k, q_d + 2 * k, s_desc, k > 0);
-          mma_commit(&k_empty[s]);
-          mma_commit(&s_full[buf]);
-          if (owed) weigh(g - 1);
-          owed = true;
-        }
       }
-      if (owed) weigh(g - 1);
-      if (!ok) {
-        // after a time-out: what was issued ends before TMEM is given back
-        int never = 0;
-        mma_commit(&drained);
-        mbar_wait_slow(&drained, 0, &never, nullptr);
+      __syncwarp();
+      if (++vs == STAGES) {
+        vs = 0;
+        vp ^= 1;
+      }
+    };
+    int left = 0, u = 1;
+    uint32_t unit = 0;
+    bool end = false;
+    // one step issues S^T of a tile, then O^T of the tile before it
+#pragma unroll 1
+    while (ok && !(end && !owed)) {
+      if (left == 0 && !end) {
+        // the next unit's queries are ready ahead of time, except for the first
+        // units: the owed product goes before a wait for them
+        const int at = unit & 1, parity = unit >> 1 & 1;
+        if (owed && !__all_sync(~0u, mbar_try(&unit_full[at], parity))) {
+          weigh();
+          continue;
+        }
+        ok = all(&unit_full[at], parity);
+        if (!ok) break;
+        u = at;
+        left = units[u].tiles;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&unit_empty[u]);
+        ++unit;
+        end = left < 0;
+        continue;
+      }
+      const bool more = !end;
+      if (more) {
+        const int buf = g & 1;
+        ok = all(&k_full[ks], kp) && all(&s_empty[buf], (g >> 1 & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t a = k_d + ks * (kTcTileBytes >> 4), b = q_d + u * (Shape::kOperand >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma<I8>(tmem + buf * N, a + 2 * k, b + 2 * k, s_desc, k > 0);
+          mma_commit(&k_empty[ks]);
+          mma_commit(&s_full[buf]);
+        }
+        __syncwarp();
+        if (++ks == STAGES) {
+          ks = 0;
+          kp ^= 1;
+        }
+        --left;
+      }
+      if (owed) weigh();
+      if (more) {
+        owed = true;
+        ++g;
       }
     }
-    __syncwarp();
+    if (!ok) {
+      // after a time-out: what was issued ends before TMEM is given back
+      int never = 0;
+      if (leader) mma_commit(&drained);
+      mbar_wait_slow(&drained, 0, &never, nullptr);
+      __syncwarp();
+    }
   } else if (warp == 6) {
     // ---- token data; a lane has every 32nd entry of a tile
     const TokenRing ring(token_smem, p);
