@@ -143,13 +143,11 @@ SIGNATURES = [
     ("dsd_decode_batch_noalloc", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ModelConfig),
                                                 ctypes.c_int, ctypes.c_int, _I32P, _VP, _VP,
                                                 _VP, _VP, _VP, _VP, _VP, _VP]),
-    ("dsd_scaled_append", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ScaledCacheDesc),
-                                         ctypes.POINTER(ScaledAppendArgs), _VP]),
-    ("dsd_scaled_attention_workspace", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ScaledCacheDesc),
-                                                      ctypes.POINTER(ScaledAttentionArgs),
+    # (device, ScaledCacheDesc*, Scaled...Args*, ...): the structs by reference, address or packed bytes
+    ("dsd_scaled_append", ctypes.c_int, [ctypes.c_int, _VP, _VP, _VP]),
+    ("dsd_scaled_attention_workspace", ctypes.c_int, [ctypes.c_int, _VP, _VP,
                                                       ctypes.POINTER(ctypes.c_int64)]),
-    ("dsd_scaled_attention", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ScaledCacheDesc),
-                                            ctypes.POINTER(ScaledAttentionArgs), _VP]),
+    ("dsd_scaled_attention", ctypes.c_int, [ctypes.c_int, _VP, _VP, _VP]),
 ]
 
 _lib = None

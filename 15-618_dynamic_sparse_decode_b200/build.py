@@ -23,11 +23,12 @@ LIB = os.path.join(PKG, "libdsd_b200.so")
 
 SOURCES = ["dsd_capi.cu", "dsd_scaled_capi.cu"]
 HEADERS = ["dsd_internal.h", "dsd_kernels.cuh", "dsd_scaled_common.cuh", "dsd_scaled_append.cuh",
-           "dsd_scaled_attn.cuh", "dsd_scaled_attn_tc.cuh"]
+           "dsd_scaled_attn.cuh", "dsd_scaled_attn_tc.cuh", "dsd_scaled_attn_wide.cuh"]
 # headers of one source only: the other need not be compiled again for them
 ONLY = {"dsd_kernels.cuh": "dsd_capi.cu", "dsd_scaled_common.cuh": "dsd_scaled_capi.cu",
         "dsd_scaled_append.cuh": "dsd_scaled_capi.cu", "dsd_scaled_attn.cuh": "dsd_scaled_capi.cu",
-        "dsd_scaled_attn_tc.cuh": "dsd_scaled_capi.cu"}
+        "dsd_scaled_attn_tc.cuh": "dsd_scaled_capi.cu",
+        "dsd_scaled_attn_wide.cuh": "dsd_scaled_capi.cu"}
 
 
 def _newer(target: str, deps: list[str]) -> bool:

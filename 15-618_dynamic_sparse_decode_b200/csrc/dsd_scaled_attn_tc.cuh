@@ -220,7 +220,8 @@ __device__ __forceinline__ bool row_has_nan(const uint4* row, int lane) {
 struct UnitInfo {
   int tiles;          // -1: the range ends
   int b, qt;
-  int rows;           // query rows from the unit's first on
+  int rows;           // query rows from the unit's first on (wide: the request's)
+  int q0, base_pos;   // wide: first query row, place of the first query
   int opens, ends;    // the segment has the unit's first / last slot
   int last_gang;
 };
@@ -257,6 +258,131 @@ __device__ __forceinline__ int box_page(const AttnParams& p, const Request& r, i
   const int slot = p.tpp ? tile % p.by_tpp * kTile : 0;
   if (p.counts ? entry >= r.len : 1ll * entry * p.P + slot >= r.len) return -1;
   return p.table[1ll * b * p.table_stride + entry];
+}
+
+// TMA warp: the pages of the CTA's tiles, one box each, K then V, as far ahead as
+// the ring has room.
+template <int STAGES>
+__device__ __forceinline__ void walk_boxes(const AttnParams& p, Walk w, int head, const CUtensorMap& k_map,
+                                           const CUtensorMap& v_map, int head_first, uint8_t* k_ring, uint8_t* v_ring,
+                                           uint64_t* k_full, uint64_t* k_empty, uint64_t* v_full, uint64_t* v_empty,
+                                           volatile int* stop) {
+  const int lane = threadIdx.x & 31;
+  const int rows = p.tpp ? kTile : p.P, boxes = p.tpp ? 1 : p.ppt;
+  uint32_t g = 0;
+  bool ok = true;
+#pragma unroll 1
+  while (w.left > 0 && ok) {
+    const Request r = w.r;
+    const Span span = span_of(p, r, w.qt);
+    const Segment seg = segment_of(w, slots_of(span));
+    const int tiles = span.n == 0 ? 0 : seg.n;
+    int next = -1;
+    if (tiles > 0 && lane < boxes) next = box_page(p, r, w.b, span.first + seg.first, lane);
+#pragma unroll 1
+    for (int i = 0; i < tiles && ok; ++i, ++g) {
+      const int tile = span.first + seg.first + i;
+      const int page = next;
+      if (i + 1 < tiles && lane < boxes) next = box_page(p, r, w.b, tile + 1, lane);
+      const bool good = page >= 0 && page < p.num_pages;
+      const int bytes = __popc(__ballot_sync(~0u, good)) * rows * 128;
+      const int s = g % STAGES, parity = (g / STAGES & 1) ^ 1;
+      const int slot = p.tpp ? tile % p.by_tpp * kTile : 0;
+      const int c1 = head_first ? head : slot, c2 = head_first ? slot : head;
+      const uint32_t at = s * kTcTileBytes + lane * rows * 128;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        uint64_t* full = kv ? &v_full[s] : &k_full[s];
+        ok = ok && mbar_wait(kv ? &v_empty[s] : &k_empty[s], parity, stop, p.status);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect(full, bytes);
+        __syncwarp();
+        if (good) tma_box(kv ? &v_map : &k_map, smem_addr(kv ? v_ring : k_ring) + at, full, c1, c2, page);
+      }
+    }
+    next_unit(p, seg, w);
+  }
+  // after a time-out: the copies still in flight land before the block's memory is given back
+  if (!ok && lane == 0) {
+    int never = 0;
+#pragma unroll 1
+    for (uint32_t i = g > STAGES ? g - STAGES : 0; i <= g; ++i) {
+      mbar_wait_slow(&k_full[i % STAGES], i / STAGES & 1, &never, nullptr);
+      never = 0;
+      mbar_wait_slow(&v_full[i % STAGES], i / STAGES & 1, &never, nullptr);
+      never = 0;
+    }
+  }
+}
+
+// Token-data warp; a lane has every 32nd entry of a tile.
+__device__ __forceinline__ void walk_tokens(const AttnParams& p, Walk w, int head, const TokenRing& ring, TileInfo* info,
+                                            uint64_t* token_full, uint64_t* token_empty, volatile int* stop) {
+  const int lane = threadIdx.x & 31;
+  int s = 0, phase = 0;   // of the token ring
+  bool ok = true;
+#pragma unroll 1
+  while (w.left > 0 && ok) {
+    const Request r = w.r;
+    const Span span = span_of(p, r, w.qt);
+    const Segment seg = segment_of(w, slots_of(span));
+    const int tiles = span.n == 0 ? 0 : seg.n;
+    const int* table = p.table + 1ll * w.b * p.table_stride;
+    const int row0 = w.qt * p.R;
+    const int base_pos = r.len - r.nq;
+    // every row sees the tokens at all_from .. all_to
+    int all_from = 0, all_to = INT_MAX;
+    if (p.causal) all_to = max(base_pos + row0 / p.by_group, -1);
+    if (p.window) all_from = max(max(base_pos + (min(row0 + p.R, r.rows) - 1) / p.by_group, -1) - p.window + 1, 0);
+#pragma unroll 1
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int tile = span.first + seg.first + i;
+      const int first = p.tpp ? tile / p.by_tpp : tile * p.ppt;       // page-table entry of the first token
+      const int off = p.tpp ? tile % p.by_tpp * kTile : 0;            // and its slot in that page
+      const int lead = off % p.by_block;
+      const int here = p.tpp ? min(kTile, p.P - off) : p.ppt * p.P;   // places of the tile
+      ok = mbar_wait(&token_empty[s], phase ^ 1, stop, p.status);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      // one pass unless block_tokens < 5; the table's lines are in L1 then
+#pragma unroll 1
+      for (int e = lane; e < ring.entries; e += 32) {
+        const int t = e * p.bt - lead;   // the block's first token in the tile; below 0 only where tpp
+        int limit = 0;
+        if (t < here) {
+          const int entry = p.tpp ? first : first + t / p.by_page, slot = p.tpp ? off + t : t % p.by_page;
+          if (!p.counts) limit = static_cast<int>(min(max(r.len - 1ll * entry * p.P - slot, 0ll), static_cast<long long>(p.bt)));
+          if (p.counts ? entry < r.len : limit > 0) {
+            const int page = table[entry];
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
+              if (p.status) atomicOr(p.status, DSD_SCALED_BAD_PAGE);
+              limit = 0;
+            } else {
+              if (p.counts) limit = min(max(p.counts[page] - slot, 0), p.bt);
+              const long long si = (1ll * page * p.Hk + head) * p.nblk + slot / p.by_block;
+              float2* to = ring.scales + s * ring.entries + e;
+              copy4_async(&to->x, p.ks + si);
+              copy4_async(&to->y, p.vs + si);
+            }
+          }
+        }
+        ring.limit[s * ring.entries + e] = limit;
+      }
+      if (lane == 0) {
+        const int place = p.tpp ? first * p.P + off : tile * p.ppt * p.P;
+        info[s] = {place, lead, p.counts || (place >= all_from && place <= all_to - (kTile - 1))};
+      }
+      mbar_arrive_after_copies(&token_full[s]);
+      mbar_arrive(&token_full[s]);
+      if (++s == ring.stages) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+    next_unit(p, seg, w);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Row `row` of a unit's queries, a lane four elements, as pieces in the operand;
@@ -387,53 +513,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
   const uint32_t tmem = tmem_base;
 
   if (warp == 4) {
-    // ---- TMA: the pages of a tile, one box each, K then V
-    const int rows = p.tpp ? kTile : p.P, boxes = p.tpp ? 1 : p.ppt;
-    uint32_t g = 0;
-    bool ok = true;
-#pragma unroll 1
-    while (w.left > 0 && ok) {
-      const Request r = w.r;
-      const Span span = span_of(p, r, w.qt);
-      const Segment seg = segment_of(w, slots_of(span));
-      const int tiles = span.n == 0 ? 0 : seg.n;
-      int next = -1;
-      if (tiles > 0 && lane < boxes) next = box_page(p, r, w.b, span.first + seg.first, lane);
-#pragma unroll 1
-      for (int i = 0; i < tiles && ok; ++i, ++g) {
-        const int tile = span.first + seg.first + i;
-        const int page = next;
-        if (i + 1 < tiles && lane < boxes) next = box_page(p, r, w.b, tile + 1, lane);
-        const bool good = page >= 0 && page < p.num_pages;
-        const int bytes = __popc(__ballot_sync(~0u, good)) * rows * 128;
-        const int s = g % STAGES, parity = (g / STAGES & 1) ^ 1;
-        const int slot = p.tpp ? tile % p.by_tpp * kTile : 0;
-        const int c1 = head_first ? head : slot, c2 = head_first ? slot : head;
-        const uint32_t at = s * kTcTileBytes + lane * rows * 128;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          uint64_t* full = kv ? &v_full[s] : &k_full[s];
-          ok = ok && mbar_wait(kv ? &v_empty[s] : &k_empty[s], parity, &stop, p.status);
-          ok = __all_sync(~0u, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_expect(full, bytes);
-          __syncwarp();
-          if (good) tma_box(kv ? &v_map : &k_map, smem_addr(kv ? v_ring : k_ring) + at, full, c1, c2, page);
-        }
-      }
-      next_unit(p, seg, w);
-    }
-    // after a time-out: the copies still in flight land before the block's memory is given back
-    if (!ok && lane == 0) {
-      int never = 0;
-#pragma unroll 1
-      for (uint32_t i = g > STAGES ? g - STAGES : 0; i <= g; ++i) {
-        mbar_wait_slow(&k_full[i % STAGES], i / STAGES & 1, &never, nullptr);
-        never = 0;
-        mbar_wait_slow(&v_full[i % STAGES], i / STAGES & 1, &never, nullptr);
-        never = 0;
-      }
-    }
+    walk_boxes<STAGES>(p, w, head, k_map, v_map, head_first, k_ring, v_ring, k_full, k_empty, v_full, v_empty, &stop);
   } else if (warp == 5) {
     // ---- MMA issue: the warp waits as one, so that descriptors stay in uniform
     // registers, and one lane issues
@@ -522,71 +602,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
       __syncwarp();
     }
   } else if (warp == 6) {
-    // ---- token data; a lane has every 32nd entry of a tile
-    const TokenRing ring(token_smem, p);
-    int s = 0, phase = 0;   // of the token ring
-    bool ok = true;
-#pragma unroll 1
-    while (w.left > 0 && ok) {
-      const Request r = w.r;
-      const Span span = span_of(p, r, w.qt);
-      const Segment seg = segment_of(w, slots_of(span));
-      const int tiles = span.n == 0 ? 0 : seg.n;
-      const int* table = p.table + 1ll * w.b * p.table_stride;
-      const int row0 = w.qt * R;
-      const int base_pos = r.len - r.nq;
-      // every row sees the tokens at all_from .. all_to
-      int all_from = 0, all_to = INT_MAX;
-      if (p.causal) all_to = max(base_pos + row0 / p.by_group, -1);
-      if (p.window) all_from = max(max(base_pos + (min(row0 + R, r.rows) - 1) / p.by_group, -1) - p.window + 1, 0);
-#pragma unroll 1
-      for (int i = 0; i < tiles && ok; ++i) {
-        const int tile = span.first + seg.first + i;
-        const int first = p.tpp ? tile / p.by_tpp : tile * p.ppt;       // page-table entry of the first token
-        const int off = p.tpp ? tile % p.by_tpp * kTile : 0;            // and its slot in that page
-        const int lead = off % p.by_block;
-        const int here = p.tpp ? min(kTile, p.P - off) : p.ppt * p.P;   // places of the tile
-        ok = mbar_wait(&token_empty[s], phase ^ 1, &stop, p.status);
-        ok = __all_sync(~0u, ok);
-        if (!ok) break;
-        // one pass unless block_tokens < 5; the table's lines are in L1 then
-#pragma unroll 1
-        for (int e = lane; e < ring.entries; e += 32) {
-          const int t = e * p.bt - lead;   // the block's first token in the tile; below 0 only where tpp
-          int limit = 0;
-          if (t < here) {
-            const int entry = p.tpp ? first : first + t / p.by_page, slot = p.tpp ? off + t : t % p.by_page;
-            if (!p.counts) limit = static_cast<int>(min(max(r.len - 1ll * entry * p.P - slot, 0ll), static_cast<long long>(p.bt)));
-            if (p.counts ? entry < r.len : limit > 0) {
-              const int page = table[entry];
-              if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
-                if (p.status) atomicOr(p.status, DSD_SCALED_BAD_PAGE);
-                limit = 0;
-              } else {
-                if (p.counts) limit = min(max(p.counts[page] - slot, 0), p.bt);
-                const long long si = (1ll * page * p.Hk + head) * p.nblk + slot / p.by_block;
-                float2* to = ring.scales + s * ring.entries + e;
-                copy4_async(&to->x, p.ks + si);
-                copy4_async(&to->y, p.vs + si);
-              }
-            }
-          }
-          ring.limit[s * ring.entries + e] = limit;
-        }
-        if (lane == 0) {
-          const int place = p.tpp ? first * p.P + off : tile * p.ppt * p.P;
-          info[s] = {place, lead, p.counts || (place >= all_from && place <= all_to - (kTile - 1))};
-        }
-        mbar_arrive_after_copies(&token_full[s]);
-        mbar_arrive(&token_full[s]);
-        if (++s == ring.stages) {
-          s = 0;
-          phase ^= 1;
-        }
-      }
-      next_unit(p, seg, w);
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    walk_tokens(p, w, head, TokenRing(token_smem, p), info, token_full, token_empty, &stop);
   } else if (warp == 7) {
     // ---- queries, cut into pieces; a lane takes four elements of every row
     const int elem = p.dtype == DSD_TYPE_F32 ? 4 : 2;

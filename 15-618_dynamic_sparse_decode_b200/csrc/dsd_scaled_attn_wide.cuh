@@ -1,0 +1,651 @@
+// dsd_scaled_attn_wide.cuh -- attention over the scaled 8-bit cache for many query
+// rows per key head (prompt chunks, drafted tokens, large groups): 128 rows at a
+// time on the fp16 tensor cores.
+//
+//   S[row][token] = Q[row][d] K[token][d]^T      O[row][d] += P[row][token] V[token][d]
+//
+// With many rows the tile's codes are worth widening once: e4m3 and int8 are exact
+// in fp16, so four warps write each K and V tile as fp16 operands and one product
+// does what the narrow kernel needs three 8-bit pieces for.  Queries are scaled by
+// a power of two of their row into fp16's range (exact for fp16 and for bf16 within
+// 2^-29 of the row's largest; fp32 rows take two fp16 pieces, 22 bits, added by the
+// accumulator).  Weights go back to TMEM as fp16 (2^-12 of their value) and are the
+// A operand of the second product there.
+//
+// A thread owns half a row of S: the running maximum and sum are its own, two
+// threads meet once a tile for the row's maximum.  O stays in TMEM and is rescaled
+// only when a row's maximum has grown by more than 2^8, which fp16 weights bear.
+//
+// Roles: warps 0-7 softmax, 8-11 widen the codes, 12 TMA, 13 MMA issue, 14 token
+// data, 15 units.
+#pragma once
+
+#include "dsd_scaled_attn_tc.cuh"
+
+namespace dsds {
+
+constexpr int kWideThreads = 512;
+constexpr int kWideRows = 128;
+constexpr float kWideGrow = 8.0f;     // log2 of how far a maximum may run behind
+constexpr float kWideOne = 64.0f;     // fp16 value of weight 1: 2^6 2^8 f < 2^15
+
+template <int PIECES>
+struct WideShape {
+  static constexpr int kStages = PIECES == 1 ? 3 : 2;
+  static constexpr int kTile16 = 2 * kTcTileBytes;   // a tile of 128 x 128 fp16
+  static constexpr size_t kSmem = 1024 + size_t(kStages) * 2 * kTcTileBytes + (2 + PIECES) * size_t(kTile16);
+  // TMEM columns: S twice, O, P
+  static constexpr int kO = 256, kP = 384, kColumns = 512;
+};
+
+__device__ __forceinline__ bool wide_sync_or(bool flag) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"(uint32_t(flag)) : "memory");
+  return any != 0;
+}
+
+// D (fp32) [128][n], A and B fp16; b_n_major: B's columns are adjacent.
+__device__ __forceinline__ uint32_t wide_desc(int n, bool b_n_major) {
+  return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"(uint32_t(add)) : "memory");
+}
+__device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(desc), "r"(uint32_t(add)) : "memory");
+}
+// 64 fp16 columns (128 bytes) a row, swizzled; the second 64 lie 16 KiB behind.
+__device__ __forceinline__ uint64_t operand16_desc(uint32_t addr) {
+  return (uint64_t(addr >> 4) & 0x3FFF) | (uint64_t(kTcTileBytes >> 4) << 16) | (uint64_t(64) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&x)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&x)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]),
+               "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 codes as fp16, exactly.
+template <bool I8>
+__device__ __forceinline__ void widen16(uint4 c, uint4& lo, uint4& hi) {
+  const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+  uint32_t out[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (I8) {
+      // 0x64uu is 1024 + u: with u = code + 128, less 1152
+      const uint32_t u = in[i] ^ 0x80808080u;
+      const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+      uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+      const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+      out[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+      out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+      const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(in[i] & 0xffff), __NV_E4M3);
+      const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(in[i] >> 16), __NV_E4M3);
+      out[2 * i] = uint32_t(x.x) | uint32_t(x.y) << 16;
+      out[2 * i + 1] = uint32_t(y.x) | uint32_t(y.y) << 16;
+    }
+  }
+  lo = make_uint4(out[0], out[1], out[2], out[3]);
+  hi = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+// Row `t` of a swizzled code tile into the fp16 tile.
+template <bool I8>
+__device__ __forceinline__ void widen_row(const uint8_t* codes, uint8_t* wide, int t, bool zero) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    if (!zero) widen16<I8>(*reinterpret_cast<const uint4*>(codes + t * 128 + ((j ^ (t & 7)) << 4)), lo, hi);
+    uint8_t* to = wide + (j >> 2) * kTcTileBytes + t * 128;
+    const int piece = 2 * (j & 3);
+    *reinterpret_cast<uint4*>(to + ((piece ^ (t & 7)) << 4)) = lo;
+    *reinterpret_cast<uint4*>(to + (((piece + 1) ^ (t & 7)) << 4)) = hi;
+  }
+}
+
+// A tile's tokens as the softmax reads them, four at a time.
+struct __align__(16) Columns {   // its size too: float4 reads of the second one
+  float ks[kTile], e[kTile], f[kTile], inverse[kTile];
+  int place, open;
+};
+
+template <bool I8, int PIECES>
+__global__ void __launch_bounds__(kWideThreads, 1)
+attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap k_map,
+                 const __grid_constant__ CUtensorMap v_map, int head_first) {
+  using Shape = WideShape<PIECES>;
+  constexpr int STAGES = Shape::kStages;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* base = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+  uint8_t* k_ring = base;
+  uint8_t* v_ring = k_ring + STAGES * kTcTileBytes;
+  uint8_t* k16 = v_ring + STAGES * kTcTileBytes;
+  uint8_t* v16 = k16 + Shape::kTile16;
+  uint8_t* q16 = v16 + Shape::kTile16;   // PIECES of them
+  __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+  __shared__ uint64_t k16_full, k16_empty, v16_full, v16_empty, s_full[2], s_empty[2], p_full, o_full, q_full;
+  __shared__ uint64_t cols_full[2], cols_empty[2], unit_full[2], unit_empty[2];
+  __shared__ uint64_t token_full[kTokenStages], token_empty[kTokenStages], drained;
+  __shared__ TileInfo info[kTokenStages];
+  __shared__ __align__(16) uint8_t token_smem[kTokenBytes];
+  __shared__ __align__(16) Columns cols[2];
+  __shared__ float red[2][2][kWideRows];
+  __shared__ UnitInfo units[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int stop;
+  __shared__ Walk walk_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cta = blockIdx.x, head = cta % p.Hk;
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 4);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 8);
+      mbar_init(&cols_full[i], 4);
+      mbar_init(&cols_empty[i], 8);
+      mbar_init(&unit_full[i], 1);
+      mbar_init(&unit_empty[i], 9);   // the softmax warps and the MMA warp
+    }
+    mbar_init(&k16_full, 4);
+    mbar_init(&k16_empty, 1);
+    mbar_init(&v16_full, 4);
+    mbar_init(&v16_empty, 1);
+    mbar_init(&p_full, 8);
+    mbar_init(&o_full, 1);
+    mbar_init(&q_full, 8);
+    for (int i = 0; i < kTokenStages; ++i) {
+      mbar_init(&token_full[i], 64);
+      mbar_init(&token_empty[i], 4);
+    }
+    mbar_init(&drained, 1);
+    stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    p.meta[cta] = make_int4(0, 0, -1, 0);
+  }
+  plan_walk<kWideThreads>(p, cta / p.Hk, reinterpret_cast<int*>(k_ring), &walk_s);
+  Walk w = walk_s;
+  if (w.left == 0) return;
+  proxy_fence();   // the plan's scratch lay in the ring
+  if (warp == 13) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                 "r"(Shape::kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  if (warp == 12) {
+    walk_boxes<STAGES>(p, w, head, k_map, v_map, head_first, k_ring, v_ring, k_full, k_empty, v_full, v_empty, &stop);
+  } else if (warp == 14) {
+    walk_tokens(p, w, head, TokenRing(token_smem, p), info, token_full, token_empty, &stop);
+  } else if (warp == 15) {
+    // ---- units
+    bool ok = true;
+#pragma unroll 1
+    for (uint32_t unit = 0; ok; ++unit) {
+      const int u = unit & 1;
+      const bool end = w.left <= 0;
+      const Request r = w.r;
+      Span span{0, 0};
+      if (!end) span = span_of(p, r, w.qt);
+      const int slots = slots_of(span);
+      const Segment seg = segment_of(w, slots);
+      ok = __all_sync(~0u, mbar_wait(&unit_empty[u], (unit >> 1 & 1) ^ 1, &stop, p.status));
+      if (!ok) break;
+      if (lane == 0) {
+        UnitInfo& x = units[u];
+        x.tiles = end ? -1 : span.n == 0 ? 0 : seg.n;
+        x.b = w.b;
+        x.qt = w.qt;
+        x.rows = r.rows;
+        x.q0 = r.q0;
+        x.base_pos = r.len - r.nq;
+        x.opens = seg.opens;
+        x.ends = seg.ends;
+        x.last_gang = end ? 0 : gang_of(p, w.at - w.slot + slots - 1, w.total);
+        mbar_arrive(&unit_full[u]);
+      }
+      __syncwarp();
+      if (end) break;
+      next_unit(p, seg, w);
+    }
+  } else if (warp == 13) {
+    // ---- MMA issue
+    const bool leader = elect_one();
+    const uint32_t s_desc = wide_desc(kTile, false), o_desc = wide_desc(p.D, true);
+    const uint64_t k_d = operand16_desc(smem_addr(k16)), v_d = operand16_desc(smem_addr(v16)), q_d = operand16_desc(smem_addr(q16));
+    const auto all = [&](uint64_t* bar, int parity) { return __all_sync(~0u, mbar_wait(bar, parity, &stop, p.status)) != 0; };
+    uint32_t g = 0, unit = 0, with_tiles = 0;
+    int left = 0;
+    bool ok = true, owed = false, owed_first = false, first = false, end = false;
+    const auto weigh = [&]() {   // O of tile g - 1
+      const int t = g - 1;
+      owed = false;
+      ok = ok && all(&p_full, t & 1) && all(&v16_full, t & 1);
+      if (!ok) return;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int piece = 0; piece < PIECES; ++piece)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_f16_tmem(tmem + Shape::kO, tmem + Shape::kP + piece * 64 + 8 * k, v_d + 128 * k, o_desc, !owed_first || k > 0 || piece > 0);
+        mma_commit(&v16_empty);
+        mma_commit(&o_full);
+      }
+      __syncwarp();
+    };
+#pragma unroll 1
+    while (ok && !(end && !owed)) {
+      if (left == 0 && !end) {
+        if (owed) {
+          weigh();   // the next queries overwrite nothing that it reads, but wait for its result
+          continue;
+        }
+        const int u = unit & 1;
+        ok = all(&unit_full[u], unit >> 1 & 1);
+        if (!ok) break;
+        left = units[u].tiles;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&unit_empty[u]);
+        ++unit;
+        end = left < 0;
+        first = true;
+        if (left > 0) {
+          ok = all(&q_full, with_tiles & 1);
+          ++with_tiles;
+        }
+        continue;
+      }
+      const bool more = !end;
+      if (more) {
+        const int buf = g & 1;
+        ok = all(&k16_full, g & 1) && all(&s_empty[buf], (g >> 1 & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const int steps = p.D / 16;
+#pragma unroll
+          for (int piece = 0; piece < PIECES; ++piece)
+#pragma unroll 1
+            for (int k = 0; k < steps; ++k) {
+              const uint64_t at = (k >> 2) * (kTcTileBytes >> 4) + 2 * (k & 3);
+              mma_f16(tmem + buf * kTile, q_d + piece * (Shape::kTile16 >> 4) + at, k_d + at, s_desc, k > 0 || piece > 0);
+            }
+          mma_commit(&k16_empty);
+          mma_commit(&s_full[buf]);
+        }
+        __syncwarp();
+        --left;
+      }
+      if (owed) weigh();
+      if (more) {
+        owed = true;
+        owed_first = first;
+        first = false;
+        ++g;
+      }
+    }
+    if (!ok) {
+      int never = 0;
+      if (leader) mma_commit(&drained);
+      mbar_wait_slow(&drained, 0, &never, nullptr);
+      __syncwarp();
+    }
+  } else if (warp >= 8) {
+    // ---- widen: thread = token; its data, then its K row, then its V row
+    const TokenRing ring(token_smem, p);
+    const int t = tid - 256, here = p.tpp ? kTile : p.ppt * p.P;
+    const int my_entry = t / p.by_block, my_place = t % p.by_block;
+    int ts = 0, tp = 0, s = 0, sp = 0;   // stage and phase of the token and code rings
+    uint32_t g = 0;
+    bool ok = true;
+    // of the units only the number of tiles matters here
+    int tiles_left = 0;
+#pragma unroll 1
+    while (w.left > 0) {
+      const Span span = span_of(p, w.r, w.qt);
+      const Segment seg = segment_of(w, slots_of(span));
+      tiles_left += span.n == 0 ? 0 : seg.n;
+      next_unit(p, seg, w);
+    }
+#pragma unroll 1
+    for (; tiles_left > 0 && ok; --tiles_left, ++g) {
+      const int cb = g & 1;
+      ok = ok && mbar_wait(&token_full[ts], tp, &stop, p.status);
+      const TileInfo tile = info[ts];
+      int entry = my_entry, in_block = my_place;
+      if (tile.lead) {
+        entry = (tile.lead + t) / p.by_block;
+        in_block = (tile.lead + t) % p.by_block;
+      }
+      entry += ts * ring.entries;
+      const bool valid = t < here && in_block < ring.limit[entry];
+      const float2 scales = ring.scales[entry];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&token_empty[ts]);
+      if (++ts == ring.stages) {
+        ts = 0;
+        tp ^= 1;
+      }
+      const uint8_t* k_codes = k_ring + s * kTcTileBytes;
+      const uint8_t* v_codes = v_ring + s * kTcTileBytes;
+      // see the narrow kernel: a value row with NaN that some row must not see
+      bool nan_row = false;
+      if (!I8 && !tile.open) {
+        ok = ok && mbar_wait(&v_full[s], sp, &stop, p.status);
+        nan_row = valid && row_has_nan(reinterpret_cast<const uint4*>(v_codes + t * 128), lane);
+      }
+      TokenScale x = token_scale(valid ? scales.y : 0.0f);
+      if (nan_row) x.factor = x.inverse = NAN;
+      ok = ok && mbar_wait(&cols_empty[cb], (g >> 1 & 1) ^ 1, &stop, p.status);
+      Columns& c = cols[cb];
+      c.ks[t] = valid ? scales.x : 0.0f;
+      c.e[t] = valid ? x.e : -INFINITY;
+      c.f[t] = valid ? x.factor * kWideOne : 0.0f;
+      c.inverse[t] = valid ? x.inverse : 0.0f;
+      if (t == 0) {
+        c.place = tile.place;
+        c.open = tile.open;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&cols_full[cb]);
+      ok = ok && mbar_wait(&k_full[s], sp, &stop, p.status) && mbar_wait(&k16_empty, (g & 1) ^ 1, &stop, p.status);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      widen_row<I8>(k_codes, k16, t, !valid);
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&k_empty[s]);
+        mbar_arrive(&k16_full);
+      }
+      ok = ok && mbar_wait(&v_full[s], sp, &stop, p.status) && mbar_wait(&v16_empty, (g & 1) ^ 1, &stop, p.status);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      widen_row<I8>(v_codes, v16, t, !valid || nan_row);
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&v_empty[s]);
+        mbar_arrive(&v16_full);
+      }
+      if (++s == STAGES) {
+        s = 0;
+        sp ^= 1;
+      }
+    }
+  } else {
+    // ---- softmax: row = lane of the warp's quarter, half of the tile's columns
+    const int row = tid & 127, half = tid >> 7;
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const int d_half = (p.D / 2 + 15) / 16 * 16;   // output elements of the first half, in steps of 16
+    uint32_t g = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (uint32_t unit = 0; ok; ++unit) {
+      const int u = unit & 1;
+      ok = !wide_sync_or(!mbar_wait(&unit_full[u], unit >> 1 & 1, &stop, p.status));
+      if (!ok) break;
+      const UnitInfo x = units[u];
+      if (x.tiles < 0) break;
+      const int row0 = x.qt * kWideRows, gr = min(row0 + row, x.rows - 1);
+      const bool mine = row0 + row < x.rows;
+      const int qi = gr / p.by_group, q_head = head * p.G + gr % p.by_group;
+      const int pos = x.base_pos + qi;
+      float factor = 0.0f;
+      if (x.tiles > 0) {
+        // queries: half a row a thread, scaled by the row's power of two
+        const uint8_t* q = static_cast<const uint8_t*>(p.q);
+        const int elem = p.dtype == DSD_TYPE_F32 ? 4 : 2;
+        const bool aligned = reinterpret_cast<uintptr_t>(p.q) % (4 * elem) == 0 && p.qst[0] % 4 == 0 && p.qst[1] % 4 == 0;
+        q += (1ll * (x.q0 + qi) * p.qst[0] + 1ll * q_head * p.qst[1] + 64 * half) * elem;
+        const int n = mine ? min(max(p.D - 64 * half, 0), 64) : 0;
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; i += 4) {
+          const float4 y = widen_four(load_four(q + i * elem, elem, aligned), p.dtype);
+          top = max(top, max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
+                             max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w)))));
+        }
+        red[0][half][row] = __uint_as_float(top);
+        wide_sync_or(false);
+        top = max(__float_as_uint(red[0][0][row]), __float_as_uint(red[0][1][row]));
+        const int e = max(static_cast<int>(top >> 23) - 127, -100);
+        const float f = __uint_as_float(uint32_t(14 - e + 127) << 23);
+        factor = top >= 0x7f800000u ? NAN : p.scale_log2 * __uint_as_float(uint32_t(e - 14 + 127) << 23);
+#pragma unroll 2
+        for (int i = 0; i < 64; i += 8) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i + j < n) y = widen_four(load_four(q + (i + j) * elem, elem, aligned), p.dtype);
+            v[j] = y.x * f;
+            v[j + 1] = y.y * f;
+            v[j + 2] = y.z * f;
+            v[j + 3] = y.w * f;
+          }
+#pragma unroll
+          for (int piece = 0; piece < PIECES; ++piece) {
+            uint32_t out[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+              out[j] = *reinterpret_cast<const uint32_t*>(&h);
+              if (piece + 1 < PIECES) {
+                const float2 b = __half22float2(h);
+                v[2 * j] -= b.x;
+                v[2 * j + 1] -= b.y;
+              }
+            }
+            *reinterpret_cast<uint4*>(q16 + piece * Shape::kTile16 + half * kTcTileBytes + row * 128 +
+                                      (((i >> 3) ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+          }
+        }
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+        wide_sync_or(false);   // `red` is free again
+      }
+
+      float m = -INFINITY, l = 0.0f;   // the reference of the weights; the sum
+#pragma unroll 1
+      for (int i = 0; i < x.tiles && ok; ++i, ++g) {
+        const int buf = g & 1;
+        const Columns& c = cols[buf];
+        bool in = mbar_wait(&cols_full[buf], g >> 1 & 1, &stop, p.status);
+        in = mbar_wait(&s_full[buf], g >> 1 & 1, &stop, p.status) && in;
+        __syncwarp();
+        tc_fence_after();
+        const bool open = c.open != 0;
+        // columns lo .. hi are the row's to see
+        const int hi = open || !p.causal ? kTile : pos - c.place;
+        const int lo = open || !p.window ? 0 : max(max(pos - c.place, -1) - p.window + 1, 0);
+        const auto logits = [&](int at, float (&s)[16]) {
+          uint32_t raw[16];
+          tmem_load<16>(lanes + buf * kTile + at, raw);
+          float4 ks[4], es[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            ks[j] = *reinterpret_cast<const float4*>(&c.ks[at + 4 * j]);
+            es[j] = *reinterpret_cast<const float4*>(&c.e[at + 4 * j]);
+          }
+          tmem_load_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float k = j & 2 ? (j & 1 ? ks[j / 4].w : ks[j / 4].z) : (j & 1 ? ks[j / 4].y : ks[j / 4].x);
+            const float e = j & 2 ? (j & 1 ? es[j / 4].w : es[j / 4].z) : (j & 1 ? es[j / 4].y : es[j / 4].x);
+            s[j] = fmaf(__uint_as_float(raw[j]) * k, factor, e);
+          }
+          if (!open) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (at + j > hi || at + j < lo) s[j] = -INFINITY;
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int at = 64 * half; at < 64 * half + 64; at += 16) {
+          float s[16];
+          logits(at, s);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, s[j]);
+        }
+        red[buf][half][row] = top;
+        ok = !wide_sync_or(!in);
+        top = fmaxf(top, red[buf][half ^ 1][row]);
+        // P and O are the last tile's until its product is done
+        if (i > 0) {
+          if (!mbar_wait(&o_full, (g - 1) & 1, &stop, p.status)) stop = 1;
+          __syncwarp();
+          tc_fence_after();
+        }
+        const bool grows = top > m + kWideGrow || (m == -INFINITY && top > m);
+        if (__any_sync(~0u, grows)) {
+          const float now = grows ? top : m, m0 = now == -INFINITY ? 0.0f : now;
+          const float a = ex2(m - m0);   // 0 from -inf
+          l *= a;
+          m = now;
+          if (i > 0) {
+#pragma unroll 1
+            for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
+              uint32_t o[16];
+              tmem_load<16>(lanes + Shape::kO + at, o);
+              tmem_load_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
+              tmem_store16(lanes + Shape::kO + at, o);
+            }
+          }
+        }
+        const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+        for (int at = 64 * half; at < 64 * half + 64; at += 16) {
+          float s[16];
+          logits(at, s);
+          float4 fs[4], vs[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            fs[j] = *reinterpret_cast<const float4*>(&c.f[at + 4 * j]);
+            vs[j] = *reinterpret_cast<const float4*>(&c.inverse[at + 4 * j]);
+          }
+          uint32_t out[PIECES][8];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            float y[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int n = j + k;
+              const float f = n & 2 ? (n & 1 ? fs[n / 4].w : fs[n / 4].z) : (n & 1 ? fs[n / 4].y : fs[n / 4].x);
+              const float v = n & 2 ? (n & 1 ? vs[n / 4].w : vs[n / 4].z) : (n & 1 ? vs[n / 4].y : vs[n / 4].x);
+              const float wt = ex2(s[n] - m0);
+              y[k] = wt * f;
+              if (open) {
+                l = fmaf(wt, v, l);
+              } else if (s[n] == -INFINITY) {
+                y[k] = 0.0f;   // f may be NaN
+              } else {
+                l = fmaf(wt, v, l);
+              }
+            }
+#pragma unroll
+            for (int piece = 0; piece < PIECES; ++piece) {
+              const __half2 h = __floats2half2_rn(y[0], y[1]);
+              out[piece][j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+              if (piece + 1 < PIECES) {
+                const float2 b = __half22float2(h);
+                y[0] -= b.x;
+                y[1] -= b.y;
+              }
+            }
+          }
+#pragma unroll
+          for (int piece = 0; piece < PIECES; ++piece) tmem_store8(lanes + Shape::kP + piece * 64 + at / 2, out[piece]);
+        }
+        tmem_store_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s_empty[buf]);
+          mbar_arrive(&cols_empty[buf]);
+          mbar_arrive(&p_full);
+        }
+      }
+      if (x.tiles > 0 && ok) {
+        ok = mbar_wait(&o_full, (g - 1) & 1, &stop, p.status);
+        __syncwarp();
+        tc_fence_after();
+      }
+      // both halves' sums; the tile loop's last use of `red` lies behind a product of all warps
+      red[0][half][row] = l;
+      ok = !wide_sync_or(!ok);
+      if (!ok) break;
+      l = red[0][0][row] + red[0][1][row];
+      const bool whole = x.opens && x.ends;
+      const float one = whole ? (l == 0.0f ? 0.0f : 1.0f / l / kWideOne) : 1.0f / kWideOne;
+      const long long piece_at = (2ll * cta + x.opens) * p.R + row;
+      const long long out_at = 1ll * (x.q0 + qi) * p.ost[0] + 1ll * q_head * p.ost[1];
+#pragma unroll 1
+      for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
+        uint32_t o[16];
+        if (x.tiles > 0) {
+          tmem_load<16>(lanes + Shape::kO + at, o);
+          tmem_load_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0;
+        }
+        if (!mine) continue;
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) store_elem(p.out, out_at + at + j, p.dtype, l == 0.0f ? 0.0f : __uint_as_float(o[j]) * one);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<float4*>(&p.part_o[piece_at * p.D + at + j]) =
+                make_float4(__uint_as_float(o[j]) * one, __uint_as_float(o[j + 1]) * one, __uint_as_float(o[j + 2]) * one,
+                            __uint_as_float(o[j + 3]) * one);
+        }
+      }
+      if (half == 0 && mine) {
+        if (!whole) {
+          p.part_ml[2 * piece_at] = m;
+          p.part_ml[2 * piece_at + 1] = l;
+        } else if (p.lse) {
+          p.lse[1ll * (x.q0 + qi) * p.H + q_head] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * kLn2;
+        }
+      }
+      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.qt, x.last_gang, 0);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_empty[u]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 13)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kColumns));
+}
+
+}  // namespace dsds

@@ -14,6 +14,7 @@
 #include "dsd_scaled_append.cuh"
 #include "dsd_scaled_attn.cuh"
 #include "dsd_scaled_attn_tc.cuh"
+#include "dsd_scaled_attn_wide.cuh"
 
 namespace {
 
@@ -227,17 +228,28 @@ void WithTc(bool i8, bool fp32, int R, F&& f) {
 }
 constexpr int kTcMaxRows = 8;
 
+template <typename F>
+void WithWide(bool i8, bool fp32, F&& f) {
+  if (i8 && fp32) f(dsds::attn_wide_kernel<true, 2>, Tag<dsds::WideShape<2>>{});
+  else if (i8) f(dsds::attn_wide_kernel<true, 1>, Tag<dsds::WideShape<1>>{});
+  else if (fp32) f(dsds::attn_wide_kernel<false, 2>, Tag<dsds::WideShape<2>>{});
+  else f(dsds::attn_wide_kernel<false, 1>, Tag<dsds::WideShape<1>>{});
+}
+
 void SetAttentionAttributes() {
   SetSimple<false, 1>(); SetSimple<false, 2>(); SetSimple<false, 4>(); SetSimple<false, 8>();
   SetSimple<true, 1>(); SetSimple<true, 2>(); SetSimple<true, 4>(); SetSimple<true, 8>();
   for (int i8 = 0; i8 < 2; ++i8)
     for (int fp32 = 0; fp32 < 2; ++fp32)
-      for (int R = 1; R <= kTcMaxRows; R *= 2)
-        WithTc(i8, fp32, R, [](auto kernel, auto tag) {
-          using Shape = typename decltype(tag)::type;
-          Check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape::kSmem)),
-                "shared memory attribute");
-        });
+    {
+      const auto set = [](auto kernel, auto tag) {
+        using Shape = typename decltype(tag)::type;
+        Check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape::kSmem)),
+              "shared memory attribute");
+      };
+      for (int R = 1; R <= kTcMaxRows; R *= 2) WithTc(i8, fp32, R, set);
+      WithWide(i8, fp32, set);
+    }
 }
 
 template <bool I8>
@@ -327,7 +339,7 @@ CUtensorMap MapOf(const dsd_scaled_cache* c, const void* codes, const CodeOrder&
 }
 
 struct AttnPlan {
-  bool tc = false;
+  bool tc = false, wide = false;
   TcMaps maps;
   int R = 1, ncta = 0, gangs = 0;
   int64_t ml_at = 0, o_at = 0, bytes = 0;   // workspace: meta, then ml, then O
@@ -341,10 +353,11 @@ AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_s
   // query rows of a request: exact for one query each, the average otherwise
   const int64_t queries = a->q_offsets ? (int64_t(a->total_queries) + a->batch - 1) / a->batch : 1;
   const int64_t rows = queries * group;
-  const int most = pl.tc ? kTcMaxRows : 8;
-  while (pl.R < most && pl.R < rows) pl.R *= 2;
-  int per_sm = 8;
-  if (pl.tc)
+  pl.wide = pl.tc && rows > kTcMaxRows;
+  if (pl.wide) pl.R = dsds::kWideRows;
+  while (pl.R < kTcMaxRows && pl.R < rows) pl.R *= 2;
+  int per_sm = pl.wide ? 1 : 8;
+  if (pl.tc && !pl.wide)
     WithTc(i8, fp32, pl.R, [&](auto, auto tag) { per_sm = decltype(tag)::type::kCtas; });
   pl.gangs = std::max(1, per_sm * dev.sms / c->num_kv_heads);
   pl.ncta = pl.gangs * c->num_kv_heads;
@@ -448,9 +461,13 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   const bool i8 = c->kv_format == DSD_KV_I8_SCALED;
   if (pl.tc) {
     const CUtensorMap k_map = MapOf(c, c->k_codes, pl.maps.k), v_map = MapOf(c, c->v_codes, pl.maps.v);
-    WithTc(i8, a->dtype == DSD_TYPE_F32, p.R, [&](auto kernel, auto tag) {
-      kernel<<<p.ncta, dsds::kTcThreads, decltype(tag)::type::kSmem, s>>>(p, k_map, v_map, pl.maps.k.head_first);
-    });
+    const bool fp32 = a->dtype == DSD_TYPE_F32;
+    const auto launch = [&](auto kernel, auto tag) {
+      kernel<<<p.ncta, pl.wide ? dsds::kWideThreads : dsds::kTcThreads, decltype(tag)::type::kSmem, s>>>(
+          p, k_map, v_map, pl.maps.k.head_first);
+    };
+    if (pl.wide) WithWide(i8, fp32, launch);
+    else WithTc(i8, fp32, p.R, launch);
   } else if (i8) {
     LaunchSimple<true>(p, s);
   } else {
@@ -461,7 +478,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   // the join may be scheduled while the last CTAs of the attention run; it waits
   // for them before it reads
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(p.ncta), unsigned(std::min(p.R, 4)));
+  cfg.gridDim = dim3(unsigned(p.ncta), unsigned(std::min(p.R, 32)));
   cfg.blockDim = dim3(unsigned(p.D <= 128 ? 128 : 256));
   cfg.stream = s;
   cudaLaunchAttribute attr{};

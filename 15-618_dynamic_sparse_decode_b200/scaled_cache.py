@@ -15,14 +15,19 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
-from . import (DSD_EINVAL, KV_FP8_SCALED, KV_I8_SCALED, InvalidArgument, OutOfRange, ScaledAppendArgs,
-               ScaledAttentionArgs, ScaledCacheDesc, _check, load_library)
+from . import (DSD_EINVAL, KV_FP8_SCALED, KV_I8_SCALED, InvalidArgument, OutOfRange, ScaledAttentionArgs,
+               ScaledCacheDesc, _check, load_library)
 
 _FORMATS = {torch.float8_e4m3fn: KV_FP8_SCALED, torch.int8: KV_I8_SCALED}
 _CODES = {v: k for k, v in _FORMATS.items()}
+# dsd_scaled_append_args and dsd_scaled_attention_args: one pack costs a tenth of setting the fields
+_APPEND_ARGS = struct.Struct("@4i2P4q3Pq3P4i2P4q2P")
+_ATTENTION_ARGS = struct.Struct("@4i3P4q3PqPifiiPqP")
+_raw_stream = torch._C._cuda_getCurrentRawStream   # the current stream's handle, without a Stream object
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _BAD = ((8, "a device-side wait exceeded its budget"),
         (1, "a page id is outside the pool or a page is beyond the page-table row"),
@@ -127,9 +132,11 @@ class ScaledKVCache:
         self._desc = ScaledCacheDesc(self.kv_format, pages, page_size, heads, dim, self.block_tokens,
                                      k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                                      (ctypes.c_int64 * 3)(*strides(k_codes)), (ctypes.c_int64 * 3)(*strides(v_codes)))
-        self._desc_ref = ctypes.byref(self._desc)
+        self._desc_at = ctypes.addressof(self._desc)
         self._workspace = {}
+        self._index = device.index
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self._status_at = self.status.data_ptr()
 
     # ---- checks
     def _ints(self, name, t, n=None):
@@ -157,9 +164,6 @@ class ScaledKVCache:
             _invalid(f"the page table must be int32 [{batch}, pages] on {self.device}, rows contiguous")
         return table.data_ptr(), table.stride(0) if batch > 1 else table.shape[1]
 
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
-
     def check(self) -> None:
         """Waits for the device and raises if a call since the last check met bad device data."""
         bits = int(self.status.item())
@@ -185,78 +189,85 @@ class ScaledKVCache:
         receives the tokens that the touched pages hold (what :meth:`attend_pages` reads).
         """
         batch = seq_lens.shape[0]
-        tokens, heads = k.shape[0], self.num_kv_heads
-        kp = self._rows("k", k, None, (tokens, heads, self.head_dim))
-        vp = self._rows("v", v, k.dtype, (tokens, heads, self.head_dim))
+        tokens, heads, dim = k.shape[0], self.num_kv_heads, self.head_dim
+        kp = self._rows("k", k, None, (tokens, heads, dim))
+        vp = self._rows("v", v, k.dtype, (tokens, heads, dim))
         table, stride = self._table(page_table, batch)
-        a = ScaledAppendArgs()
-        a.dtype, a.batch, a.total_tokens, a.max_pages_per_request = _TYPES[k.dtype], batch, tokens, page_table.shape[1]
-        a.k, a.v, a.k_stride[:], a.v_stride[:] = kp, vp, k.stride()[:2], v.stride()[:2]
-        if token_offsets is not None:
-            a.token_offsets = self._ints("token_offsets", token_offsets, batch + 1)
-        a.seq_lens = self._ints("seq_lens", seq_lens)
-        a.page_table, a.page_table_stride = table, stride
+        offsets = None if token_offsets is None else self._ints("token_offsets", token_offsets, batch + 1)
+        lens = self._ints("seq_lens", seq_lens)
+        cos = sin = None
+        places = turned = pairs = 0
         if rotary is not None:
             if rotary.cos.device != self.device:
                 _invalid(f"the rotation table must be on {self.device}")
-            a.cos, a.sin = rotary.cos.data_ptr(), rotary.sin.data_ptr()
-            a.rotary_positions, a.rotary_dim, a.interleaved = rotary.cos.shape[0], 2 * rotary.cos.shape[1], rotary.interleaved
-        if positions is not None:
-            a.positions = self._ints("positions", positions, tokens)
+            cos, sin, pairs = rotary.cos.data_ptr(), rotary.sin.data_ptr(), rotary.interleaved
+            places, half = rotary.cos.shape
+            turned = 2 * half
+        at = None if positions is None else self._ints("positions", positions, tokens)
+        qp = op = None
+        q_heads = 0
+        q_stride = out_stride = (0, 0, 1)
         if q is not None:
-            a.q = self._rows("q", q, k.dtype)
+            qp = self._rows("q", q, k.dtype)
             if q.shape[0] != tokens:
                 _invalid("q must have a row for each token")
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            a.q_out = self._rows("q_out", q_out, q.dtype, q.shape)
-            a.num_q_heads, a.q_stride[:], a.q_out_stride[:] = q.shape[1], q.stride()[:2], q_out.stride()[:2]
+                op = q_out.data_ptr()
+            else:
+                op = self._rows("q_out", q_out, q.dtype, q.shape)
+            q_heads, q_stride, out_stride = q.shape[1], q.stride(), q_out.stride()
         elif q_out is not None:
             _invalid("q_out needs q")
-        if token_counts is not None:
-            a.token_counts = self._ints("token_counts", token_counts, self.num_pages)
-        a.status = self.status.data_ptr()
-        _check(self.lib.dsd_scaled_append(self.device.index, self._desc_ref, ctypes.byref(a), self._stream()))
+        counts = None if token_counts is None else self._ints("token_counts", token_counts, self.num_pages)
+        k_stride, v_stride = k.stride(), v.stride()
+        args = _APPEND_ARGS.pack(
+            _TYPES[k.dtype], batch, tokens, page_table.shape[1], kp or 0, vp or 0, k_stride[0], k_stride[1], v_stride[0],
+            v_stride[1], offsets or 0, lens or 0, table or 0, stride, cos or 0, sin or 0, at or 0, places, turned, pairs,
+            q_heads, qp or 0, op or 0, q_stride[0], q_stride[1], out_stride[0], out_stride[1], counts or 0, self._status_at)
+        _check(self.lib.dsd_scaled_append(self._index, self._desc_at, args, _raw_stream(self._index)))
         return q_out
 
     def _attend(self, q, table, lens, q_offsets, counts, scale, causal, window, out, return_lse):
         batch = lens.shape[0]
-        rows = q.shape[0]
-        a = ScaledAttentionArgs()
-        a.q = self._rows("q", q)
+        rows, heads = q.shape[0], q.shape[1]
+        qp = self._rows("q", q)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        a.out = self._rows("out", out, q.dtype, q.shape)
-        a.dtype, a.batch, a.total_queries, a.num_q_heads = _TYPES[q.dtype], batch, rows, q.shape[1]
-        a.q_stride[:], a.out_stride[:] = q.stride()[:2], out.stride()[:2]
-        a.lens = self._ints("lens", lens)
-        a.page_table, a.page_table_stride = self._table(table, batch)
-        a.max_pages_per_request = table.shape[1]
-        if q_offsets is not None:
-            a.q_offsets = self._ints("q_offsets", q_offsets, batch + 1)
-        if counts is not None:
-            a.page_counts = self._ints("page_counts", counts, self.num_pages)
-        a.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
-        a.causal, a.window = causal, window
-        a.status = self.status.data_ptr()
-        lse = None
-        if return_lse:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-            a.lse = lse.data_ptr()
-        key = (batch, rows, q.shape[1], q_offsets is None, q.dtype)
+            op = out.data_ptr()
+        else:
+            op = self._rows("out", out, q.dtype, q.shape)
+        lens_at = self._ints("lens", lens)
+        table_at, stride = self._table(table, batch)
+        offsets = None if q_offsets is None else self._ints("q_offsets", q_offsets, batch + 1)
+        held = None if counts is None else self._ints("page_counts", counts, self.num_pages)
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim)
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        key = (batch, rows, heads, offsets is None, q.dtype)
         need = self._workspace.get(key)   # bytes, a function of the sizes alone
         if need is None:
-            if len(self._workspace) >= 1024:
-                self._workspace.clear()
-            n = ctypes.c_int64()
-            _check(self.lib.dsd_scaled_attention_workspace(self.device.index, self._desc_ref, ctypes.byref(a),
-                                                           ctypes.byref(n)))
-            need = self._workspace[key] = n.value
+            need = self._workspace_bytes(key)
         # a new block each call: torch orders its reuse by stream, and a captured graph keeps its own
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-        _check(self.lib.dsd_scaled_attention(self.device.index, self._desc_ref, ctypes.byref(a), self._stream()))
+        q_stride, out_stride = q.stride(), out.stride()
+        args = _ATTENTION_ARGS.pack(
+            _TYPES[q.dtype], batch, rows, heads, qp or 0, op or 0, lse.data_ptr() if return_lse else 0, q_stride[0], q_stride[1],
+            out_stride[0], out_stride[1], offsets or 0, lens_at or 0, table_at or 0, stride, held or 0, table.shape[1], scale,
+            causal, window, work.data_ptr() or 0, need, self._status_at)
+        _check(self.lib.dsd_scaled_attention(self._index, self._desc_at, args, _raw_stream(self._index)))
         return (out, lse) if return_lse else out
+
+    def _workspace_bytes(self, key):
+        if len(self._workspace) >= 1024:
+            self._workspace.clear()
+        batch, rows, heads, single, dtype = key
+        a = ScaledAttentionArgs(dtype=_TYPES[dtype], batch=batch, total_queries=rows, num_q_heads=heads,
+                                q_offsets=None if single else 4, scale=1.0)
+        n = ctypes.c_int64()
+        _check(self.lib.dsd_scaled_attention_workspace(self._index, self._desc_at, ctypes.byref(a), ctypes.byref(n)))
+        need = self._workspace[key] = n.value
+        return need
 
     def attend(self, q, page_table, seq_lens, q_offsets=None, scale: float | None = None, causal: bool = True,
                window: int = 0, out=None, return_lse: bool = False):

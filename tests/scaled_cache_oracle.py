@@ -99,6 +99,13 @@ class Pool:
     def values(self, name, page, slot, h):
         return decode(self.codes[name][page, slot, h], self.fmt) * np.float64(self.scales[name][page, h, slot // self.bt])
 
+    def rows(self, name, page_row, places, h):
+        """Values of a request's tokens at `places`, [len][D]."""
+        places = np.asarray(places, np.int64)
+        page, slot = np.asarray(page_row, np.int64)[places // self.P], places % self.P
+        with np.errstate(invalid="ignore"):
+            return decode(self.codes[name][page, slot, h], self.fmt) * self.scales[name][page, h, slot // self.bt].astype(np.float64)[:, None]
+
 
 def attend_rows(q, k, v, scale, seen):
     """q [G][D], k/v [L][D] in 64 bits, seen [L] bool -> out [G][D], lse [G]; nothing seen: zeros, -inf."""
@@ -117,8 +124,7 @@ def attend(pool, q, page_row, length, scale, causal=True, window=0):
     t = np.arange(length)
     out, lse = np.zeros(q.shape), np.full((n, H), -np.inf)
     for h in range(pool.Hk):
-        k = np.array([pool.values("k", page_row[i // pool.P], i % pool.P, h) for i in t]).reshape(length, pool.D)
-        v = np.array([pool.values("v", page_row[i // pool.P], i % pool.P, h) for i in t]).reshape(length, pool.D)
+        k, v = pool.rows("k", page_row, t, h), pool.rows("v", page_row, t, h)
         for j in range(n):
             pos = length - n + j
             seen = np.ones(length, bool)

@@ -142,5 +142,8 @@ def test_struct_sizes_match_the_header(tmp_path):
     got = list(map(int, subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()))
     mine = [dsd.ScaledCacheDesc, dsd.ScaledAppendArgs, dsd.ScaledAttentionArgs]
     assert got[:3] == [ctypes.sizeof(m) for m in mine]
+    from importlib import import_module
+    binding = import_module(dsd.__name__ + ".scaled_cache")
+    assert [binding._APPEND_ARGS.size, binding._ATTENTION_ARGS.size] == got[1:3]
     assert got[3:] == [dsd.ScaledCacheDesc.v_stride.offset, dsd.ScaledAppendArgs.status.offset,
                        dsd.ScaledAttentionArgs.status.offset]

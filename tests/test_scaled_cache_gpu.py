@@ -225,21 +225,19 @@ def tolerance(q, pool, ids, length, scale, out, lse, dtype, G, seen=None):
     half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
     piece, spot = (2.0 ** -23, 2.0 ** -28) if dtype == "f32" else (2.0 ** -11, 2.0 ** -18)
     for h in range(pool.Hk):
-        k = np.array([pool.values("k", ids[i // pool.P], i % pool.P, h) for i in range(length)]).reshape(length, D)
-        v = np.array([pool.values("v", ids[i // pool.P], i % pool.P, h) for i in range(length)]).reshape(length, D)
-        k, v = np.nan_to_num(k), np.nan_to_num(v)
-        for j in range(n):
-            for g in range(h * G, (h + 1) * G):
-                x = np.nan_to_num(q[j, g].astype(np.float64), posinf=0, neginf=0)
-                big = (np.abs(k) @ np.abs(x)).max() * abs(scale) if length else 0.0
-                z = k @ x * scale
-                # contributions are normalised by the largest weight * |v scale|
-                total = np.exp(z - z.max()).sum() if length else 1.0
-                zerr = 2 * (D + 8) * 2.0 ** -24 * big
-                vmax = np.abs(v).max() if length else 0.0
-                d = zerr + 2.0 ** -20 + piece + length * spot / max(1.0, total)
-                tol_o[j, g] = half * np.abs(out[j, g]) + d * vmax
-                tol_l[j, g] = zerr + 2.0 ** -20 * max(1.0, abs(lse[j, g])) if np.isfinite(lse[j, g]) else 0.0
+        k, v = (np.nan_to_num(pool.rows(x, ids, np.arange(length), h)) for x in "kv")
+        hs = slice(h * G, (h + 1) * G)
+        x = np.nan_to_num(q[:, hs].astype(np.float64), posinf=0, neginf=0)
+        if not length:
+            continue
+        big = (np.abs(x) @ np.abs(k).T).max(-1) * abs(scale)
+        z = x @ k.T * scale
+        total = np.exp(z - z.max(-1, keepdims=True)).sum(-1)
+        zerr = 2 * (D + 8) * 2.0 ** -24 * big
+        d = zerr + 2.0 ** -20 + piece + length * spot / np.maximum(1.0, total)
+        tol_o[:, hs] = half * np.abs(out[:, hs]) + (d * np.abs(v).max())[..., None]
+        seen = np.isfinite(lse[:, hs])
+        tol_l[:, hs] = np.where(seen, zerr + 2.0 ** -20 * np.maximum(1.0, np.abs(np.where(seen, lse[:, hs], 0))), 0.0)
     return tol_o, tol_l
 
 
@@ -272,6 +270,16 @@ ATTENDS = [
     ("int8", "bf16", 128, 6, 2, 16, 16, "token", [100, 60], [20, 5], False, 0),
     ("fp8", "bf16", 64, 4, 2, 16, 16, "token", [100, 60], [20, 5], False, 30),
     ("fp8", "f16", 96, 40, 1, 16, 16, "token", [140, 33], [4, 2], True, 0),
+    # many key heads leave few ranges: several tiles and units to a CTA
+    ("fp8", "bf16", 128, 64, 64, 16, 16, "token", [1900, 3, 700, 0, 1300], None, True, 0),
+    ("int8", "f32", 64, 128, 64, 32, 8, "head", [900, 1700, 400], None, True, 500),
+    ("fp8", "bf16", 128, 512, 64, 16, 16, "token", [1500, 640], None, True, 0),
+    ("int8", "f16", 64, 192, 96, 16, 4, "token", [800, 1000], [5, 3], True, 0),
+    ("fp8", "bf16", 64, 96, 48, 16, 16, "token", [1200, 500, 90], [70, 130, 90], True, 0),
+    ("int8", "bf16", 128, 64, 64, 32, 32, "head", [700, 1000], [150, 40], True, 333),
+    ("fp8", "f32", 128, 64, 64, 16, 1, "token", [600, 300], [40, 20], True, 0),
+    ("int8", "f16", 80, 144, 72, 16, 16, "token", [1300], [200], False, 0),
+    ("fp8", "bf16", 72, 64, 64, 6, 6, "token", [6000, 1000], [3, 20], True, 0),
 ]
 
 
@@ -424,8 +432,7 @@ def test_bad_pages_and_lengths_are_masked(torch, dsd):
         x = f32(q[1:2])
         keep = np.array([i // P not in (1, 2) for i in range(60)])
         for h in range(2):
-            k = np.array([s.pool.values("k", s.table[1, i // P], i % P, h) for i in range(60)])
-            v = np.array([s.pool.values("v", s.table[1, i // P], i % P, h) for i in range(60)])
+            k, v = (s.pool.rows(n, s.table[1], np.arange(60), h) for n in "kv")
             w, _ = o.attend_rows(x[0, 2 * h:2 * h + 2], k, v, D ** -0.5, keep)
             assert np.abs(f32(out[1, 2 * h:2 * h + 2]) - w).max() < 2.0 ** -11 * np.abs(w).max() + 2.0 ** -9 * np.abs(v).max()
         with pytest.raises(dsd.OutOfRange):
