@@ -69,10 +69,18 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, int parity) {
                : "=r"(ok) : "r"(smem_addr(b)), "r"(parity) : "memory");
   return ok != 0;
 }
+// The same, asleep for up to 20 us at a time: spinning warps took issue slots from
+// the softmax.
+__device__ __forceinline__ bool mbar_sleep(uint64_t* b, int parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_addr(b)), "r"(parity), "r"(20000) : "memory");
+  return ok != 0;
+}
 // Bounded: gives up after about a second, or once another role has.
 __device__ __noinline__ bool mbar_wait_slow(uint64_t* b, int parity, volatile int* stop, int* status) {
   const long long until = clock64() + (1ll << 31);
-  while (!mbar_try(b, parity)) {
+  while (!mbar_sleep(b, parity)) {
     if (*stop) return false;
     if (clock64() > until) {
       *stop = 1;
@@ -119,7 +127,7 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&x)[N]) {
-  static_assert(N == 1 || N == 2 || N == 4 || N == 8 || N == 16 || N == 32);
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8 || N % 16 == 0);
   if constexpr (N == 1)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(x[0]) : "r"(addr));
   else if constexpr (N == 2)

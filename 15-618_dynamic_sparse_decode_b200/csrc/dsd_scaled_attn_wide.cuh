@@ -8,9 +8,8 @@
 // in fp16, so four warps write each K and V tile as fp16 operands and one product
 // does what the narrow kernel needs three 8-bit pieces for.  Queries are scaled by
 // a power of two of their row into fp16's range (exact for fp16 and for bf16 within
-// 2^-29 of the row's largest; fp32 rows take two fp16 pieces, 22 bits, added by the
-// accumulator).  Weights go back to TMEM as fp16 (2^-12 of their value) and are the
-// A operand of the second product there.
+// 2^-29 of the row's largest).  Weights go back to TMEM as fp16 (2^-12 of their
+// value) and are the A operand of the second product there.
 //
 // A thread owns half a row of S: the running maximum and sum are its own, two
 // threads meet once a tile for the row's maximum.  O stays in TMEM and is rescaled
@@ -29,11 +28,15 @@ constexpr int kWideRows = 128;
 constexpr float kWideGrow = 8.0f;     // log2 of how far a maximum may run behind
 constexpr float kWideOne = 64.0f;     // fp16 value of weight 1: 2^6 2^8 f < 2^15
 
-template <int PIECES>
+// PP: fp16 pieces of a weight.  One for bf16, whose outputs are far coarser than a
+// weight's 2^-12; two for fp16, or the weights' rounding would add to the output's
+// own.  fp32 rows stay with the narrow kernel: the accumulator's adds truncate, and
+// sums over 60000 tokens in it came out 1.6e-5 off, against 3e-7 there.
+template <int PP>
 struct WideShape {
-  static constexpr int kStages = PIECES == 1 ? 3 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kTile16 = 2 * kTcTileBytes;   // a tile of 128 x 128 fp16
-  static constexpr size_t kSmem = 1024 + size_t(kStages) * 2 * kTcTileBytes + (2 + PIECES) * size_t(kTile16);
+  static constexpr size_t kSmem = 1024 + size_t(kStages) * 2 * kTcTileBytes + 4 * size_t(kTile16);
   // TMEM columns: S twice, O, P
   static constexpr int kO = 256, kP = 384, kColumns = 512;
 };
@@ -74,6 +77,46 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&x)[
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two fp32 values in a register pair (packed fp32 instructions).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+  return x;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+  uint64_t x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "r"(a), "r"(b));
+  return x;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t x;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+  return x;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  return pair(ex2(a), ex2(b));
+}
+// w * x, 0 where w is 0 whatever x is
+__device__ __forceinline__ uint64_t seen_product(uint64_t w, uint64_t x) {
+  float a, b, c, d;
+  unpair(w, a, b);
+  unpair(x, c, d);
+  return pair(a != 0.0f ? a * c : 0.0f, b != 0.0f ? b * d : 0.0f);
+}
+
 // 16 codes as fp16, exactly.
 template <bool I8>
 __device__ __forceinline__ void widen16(uint4 c, uint4& lo, uint4& hi) {
@@ -90,27 +133,28 @@ __device__ __forceinline__ void widen16(uint4 c, uint4& lo, uint4& hi) {
       out[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
       out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
     } else {
-      const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(in[i] & 0xffff), __NV_E4M3);
-      const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(in[i] >> 16), __NV_E4M3);
-      out[2 * i] = uint32_t(x.x) | uint32_t(x.y) << 16;
-      out[2 * i + 1] = uint32_t(y.x) | uint32_t(y.y) << 16;
+      asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+          : "=r"(out[2 * i]), "=r"(out[2 * i + 1]) : "r"(in[i]));
     }
   }
   lo = make_uint4(out[0], out[1], out[2], out[3]);
   hi = make_uint4(out[4], out[5], out[6], out[7]);
 }
 
-// Row `t` of a swizzled code tile into the fp16 tile.
+// Row `t` of a swizzled code tile into the fp16 tile; all loads before the first use.
 template <bool I8>
 __device__ __forceinline__ void widen_row(const uint8_t* codes, uint8_t* wide, int t, bool zero) {
+  uint4 raw[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) raw[j] = *reinterpret_cast<const uint4*>(codes + (t * 128 + (j << 4) ^ (t & 7) << 4));
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    if (!zero) widen16<I8>(*reinterpret_cast<const uint4*>(codes + t * 128 + ((j ^ (t & 7)) << 4)), lo, hi);
-    uint8_t* to = wide + (j >> 2) * kTcTileBytes + t * 128;
-    const int piece = 2 * (j & 3);
-    *reinterpret_cast<uint4*>(to + ((piece ^ (t & 7)) << 4)) = lo;
-    *reinterpret_cast<uint4*>(to + (((piece + 1) ^ (t & 7)) << 4)) = hi;
+    uint4 lo, hi;
+    if (zero) raw[j] = make_uint4(0, 0, 0, 0);   // code 0 is 0 in both formats
+    widen16<I8>(raw[j], lo, hi);
+    uint8_t* to = wide + (j >> 2) * kTcTileBytes;
+    *reinterpret_cast<uint4*>(to + (t * 128 + ((2 * j & 7) << 4) ^ (t & 7) << 4)) = lo;
+    *reinterpret_cast<uint4*>(to + (t * 128 + ((2 * j & 7) + 1 << 4) ^ (t & 7) << 4)) = hi;
   }
 }
 
@@ -120,11 +164,11 @@ struct __align__(16) Columns {   // its size too: float4 reads of the second one
   int place, open;
 };
 
-template <bool I8, int PIECES>
+template <bool I8, int PP>
 __global__ void __launch_bounds__(kWideThreads, 1)
 attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, int head_first) {
-  using Shape = WideShape<PIECES>;
+  using Shape = WideShape<PP>;
   constexpr int STAGES = Shape::kStages;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* base = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
@@ -132,9 +176,9 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
   uint8_t* v_ring = k_ring + STAGES * kTcTileBytes;
   uint8_t* k16 = v_ring + STAGES * kTcTileBytes;
   uint8_t* v16 = k16 + Shape::kTile16;
-  uint8_t* q16 = v16 + Shape::kTile16;   // PIECES of them
+  uint8_t* q16 = v16 + 2 * Shape::kTile16;
   __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-  __shared__ uint64_t k16_full, k16_empty, v16_full, v16_empty, s_full[2], s_empty[2], p_full, o_full, q_full;
+  __shared__ uint64_t k16_full, k16_empty, v16_full[2], v16_empty[2], s_full[2], s_empty[2], p_full, o_full, q_full;
   __shared__ uint64_t cols_full[2], cols_empty[2], unit_full[2], unit_empty[2];
   __shared__ uint64_t token_full[kTokenStages], token_empty[kTokenStages], drained;
   __shared__ TileInfo info[kTokenStages];
@@ -156,6 +200,8 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       mbar_init(&v_empty[i], 4);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&v16_full[i], 4);
+      mbar_init(&v16_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 8);
       mbar_init(&cols_full[i], 4);
@@ -165,8 +211,6 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
     }
     mbar_init(&k16_full, 4);
     mbar_init(&k16_empty, 1);
-    mbar_init(&v16_full, 4);
-    mbar_init(&v16_empty, 1);
     mbar_init(&p_full, 8);
     mbar_init(&o_full, 1);
     mbar_init(&q_full, 8);
@@ -240,16 +284,17 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
     const auto weigh = [&]() {   // O of tile g - 1
       const int t = g - 1;
       owed = false;
-      ok = ok && all(&p_full, t & 1) && all(&v16_full, t & 1);
+      ok = ok && all(&p_full, t & 1) && all(&v16_full[t & 1], t >> 1 & 1);
       if (!ok) return;
       tc_fence_after();
       if (leader) {
+        const uint64_t v = v_d + (t & 1) * (Shape::kTile16 >> 4);
 #pragma unroll
-        for (int piece = 0; piece < PIECES; ++piece)
+        for (int piece = 0; piece < PP; ++piece)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            mma_f16_tmem(tmem + Shape::kO, tmem + Shape::kP + piece * 64 + 8 * k, v_d + 128 * k, o_desc, !owed_first || k > 0 || piece > 0);
-        mma_commit(&v16_empty);
+            mma_f16_tmem(tmem + Shape::kO, tmem + Shape::kP + piece * 64 + 8 * k, v + 128 * k, o_desc, !owed_first || k > 0 || piece > 0);
+        mma_commit(&v16_empty[t & 1]);
         mma_commit(&o_full);
       }
       __syncwarp();
@@ -285,11 +330,10 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         if (leader) {
           const int steps = p.D / 16;
 #pragma unroll
-          for (int piece = 0; piece < PIECES; ++piece)
-#pragma unroll 1
-            for (int k = 0; k < steps; ++k) {
-              const uint64_t at = (k >> 2) * (kTcTileBytes >> 4) + 2 * (k & 3);
-              mma_f16(tmem + buf * kTile, q_d + piece * (Shape::kTile16 >> 4) + at, k_d + at, s_desc, k > 0 || piece > 0);
+          for (int k = 0; k < 8; ++k)
+            if (k < steps) {
+              const int at = (k >> 2) * (kTcTileBytes >> 4) + 2 * (k & 3);
+              mma_f16(tmem + buf * kTile, q_d + at, k_d + at, s_desc, k > 0);
             }
           mma_commit(&k16_empty);
           mma_commit(&s_full[buf]);
@@ -349,6 +393,16 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       }
       const uint8_t* k_codes = k_ring + s * kTcTileBytes;
       const uint8_t* v_codes = v_ring + s * kTcTileBytes;
+      ok = ok && mbar_wait(&k_full[s], sp, &stop, p.status) && mbar_wait(&k16_empty, (g & 1) ^ 1, &stop, p.status);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      widen_row<I8>(k_codes, k16, t, !valid);
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&k16_full);
+        mbar_arrive(&k_empty[s]);
+      }
       // see the narrow kernel: a value row with NaN that some row must not see
       bool nan_row = false;
       if (!I8 && !tile.open) {
@@ -369,25 +423,15 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&cols_full[cb]);
-      ok = ok && mbar_wait(&k_full[s], sp, &stop, p.status) && mbar_wait(&k16_empty, (g & 1) ^ 1, &stop, p.status);
+      ok = ok && mbar_wait(&v_full[s], sp, &stop, p.status) && mbar_wait(&v16_empty[cb], (g >> 1 & 1) ^ 1, &stop, p.status);
       ok = __all_sync(~0u, ok);
       if (!ok) break;
-      widen_row<I8>(k_codes, k16, t, !valid);
+      widen_row<I8>(v_codes, v16 + cb * Shape::kTile16, t, !valid || nan_row);
       proxy_fence();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&k_empty[s]);
-        mbar_arrive(&k16_full);
-      }
-      ok = ok && mbar_wait(&v_full[s], sp, &stop, p.status) && mbar_wait(&v16_empty, (g & 1) ^ 1, &stop, p.status);
-      ok = __all_sync(~0u, ok);
-      if (!ok) break;
-      widen_row<I8>(v_codes, v16, t, !valid || nan_row);
-      proxy_fence();
-      __syncwarp();
-      if (lane == 0) {
+        mbar_arrive(&v16_full[cb]);
         mbar_arrive(&v_empty[s]);
-        mbar_arrive(&v16_full);
       }
       if (++s == STAGES) {
         s = 0;
@@ -416,7 +460,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       if (x.tiles > 0) {
         // queries: half a row a thread, scaled by the row's power of two
         const uint8_t* q = static_cast<const uint8_t*>(p.q);
-        const int elem = p.dtype == DSD_TYPE_F32 ? 4 : 2;
+        constexpr int elem = 2;   // fp32 rows take the narrow kernel
         const bool aligned = reinterpret_cast<uintptr_t>(p.q) % (4 * elem) == 0 && p.qst[0] % 4 == 0 && p.qst[1] % 4 == 0;
         q += (1ll * (x.q0 + qi) * p.qst[0] + 1ll * q_head * p.qst[1] + 64 * half) * elem;
         const int n = mine ? min(max(p.D - 64 * half, 0), 64) : 0;
@@ -445,22 +489,14 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
             v[j + 2] = y.z * f;
             v[j + 3] = y.w * f;
           }
+          uint32_t out[4];
 #pragma unroll
-          for (int piece = 0; piece < PIECES; ++piece) {
-            uint32_t out[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-              out[j] = *reinterpret_cast<const uint32_t*>(&h);
-              if (piece + 1 < PIECES) {
-                const float2 b = __half22float2(h);
-                v[2 * j] -= b.x;
-                v[2 * j + 1] -= b.y;
-              }
-            }
-            *reinterpret_cast<uint4*>(q16 + piece * Shape::kTile16 + half * kTcTileBytes + row * 128 +
-                                      (((i >> 3) ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+          for (int j = 0; j < 4; ++j) {
+            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            out[j] = *reinterpret_cast<const uint32_t*>(&h);
           }
+          *reinterpret_cast<uint4*>(q16 + half * kTcTileBytes + row * 128 + (((i >> 3) ^ (row & 7)) << 4)) =
+              make_uint4(out[0], out[1], out[2], out[3]);
         }
         proxy_fence();
         __syncwarp();
@@ -478,115 +514,125 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         __syncwarp();
         tc_fence_after();
         const bool open = c.open != 0;
-        // columns lo .. hi are the row's to see
-        const int hi = open || !p.causal ? kTile : pos - c.place;
-        const int lo = open || !p.window ? 0 : max(max(pos - c.place, -1) - p.window + 1, 0);
-        const auto logits = [&](int at, float (&s)[16]) {
-          uint32_t raw[16];
-          tmem_load<16>(lanes + buf * kTile + at, raw);
-          float4 ks[4], es[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            ks[j] = *reinterpret_cast<const float4*>(&c.ks[at + 4 * j]);
-            es[j] = *reinterpret_cast<const float4*>(&c.e[at + 4 * j]);
-          }
+        // two columns a register pair: one instruction for both
+        uint64_t s[32];
+        {
+          uint32_t raw[64];
+          tmem_load<64>(lanes + buf * kTile + 64 * half, raw);
           tmem_load_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float k = j & 2 ? (j & 1 ? ks[j / 4].w : ks[j / 4].z) : (j & 1 ? ks[j / 4].y : ks[j / 4].x);
-            const float e = j & 2 ? (j & 1 ? es[j / 4].w : es[j / 4].z) : (j & 1 ? es[j / 4].y : es[j / 4].x);
-            s[j] = fmaf(__uint_as_float(raw[j]) * k, factor, e);
-          }
-          if (!open) {
+          for (int j = 0; j < 32; ++j) s[j] = pair(raw[2 * j], raw[2 * j + 1]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[buf]);
+        const uint64_t factor2 = pair(factor, factor);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (at + j > hi || at + j < lo) s[j] = -INFINITY;
-          }
-        };
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int at = 64 * half; at < 64 * half + 64; at += 16) {
-          float s[16];
-          logits(at, s);
+        for (int j = 0; j < 32; j += 2) {
+          const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&c.ks[64 * half + 2 * j]);
+          const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&c.e[64 * half + 2 * j]);
+          s[j] = fma2(mul2(s[j], k.x), factor2, e.x);
+          s[j + 1] = fma2(mul2(s[j + 1], k.y), factor2, e.y);
+        }
+        if (!open) {
+          // columns lo .. hi are the row's to see
+          const int hi = (p.causal ? pos - c.place : kTile) - 64 * half;
+          const int lo = (p.window ? max(max(pos - c.place, -1) - p.window + 1, 0) : 0) - 64 * half;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) top = fmaxf(top, s[j]);
+          for (int j = 0; j < 32; ++j) {
+            float a, b;
+            unpair(s[j], a, b);
+            s[j] = pair(2 * j > hi || 2 * j < lo ? -INFINITY : a, 2 * j + 1 > hi || 2 * j + 1 < lo ? -INFINITY : b);
+          }
+        }
+        float top;
+        {
+          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float a, b;
+            unpair(s[j], a, b);
+            t[j & 3] = fmaxf(t[j & 3], fmaxf(a, b));
+          }
+          top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         }
         red[buf][half][row] = top;
         ok = !wide_sync_or(!in);
         top = fmaxf(top, red[buf][half ^ 1][row]);
+        const bool grows = top > m + kWideGrow || (m == -INFINITY && top > m);
+        const bool any = __any_sync(~0u, grows);
+        float a = 1.0f;
+        if (grows) {
+          a = ex2(m - top);   // 0 from -inf
+          l *= a;
+          m = top;
+        }
+        const float m0 = m == -INFINITY ? 0.0f : -m;
+        const uint64_t m2 = pair(m0, m0);
+        uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&c.inverse[64 * half + 2 * j]);
+          const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&c.f[64 * half + 2 * j]);
+          uint64_t w0 = ex2_pair(add2(s[j], m2)), w1 = ex2_pair(add2(s[j + 1], m2));
+          if (open) {
+            sum0 = fma2(w0, v.x, sum0);
+            sum1 = fma2(w1, v.y, sum1);
+            s[j] = mul2(w0, f.x);
+            s[j + 1] = mul2(w1, f.y);
+          } else {
+            // f and inverse of a masked place may be NaN: a weight of zero stays one
+            sum0 = add2(sum0, seen_product(w0, v.x));
+            sum1 = add2(sum1, seen_product(w1, v.y));
+            s[j] = seen_product(w0, f.x);
+            s[j + 1] = seen_product(w1, f.y);
+          }
+        }
+        {
+          float x0, x1;
+          unpair(add2(sum0, sum1), x0, x1);
+          l += x0 + x1;
+        }
         // P and O are the last tile's until its product is done
         if (i > 0) {
           if (!mbar_wait(&o_full, (g - 1) & 1, &stop, p.status)) stop = 1;
           __syncwarp();
           tc_fence_after();
         }
-        const bool grows = top > m + kWideGrow || (m == -INFINITY && top > m);
-        if (__any_sync(~0u, grows)) {
-          const float now = grows ? top : m, m0 = now == -INFINITY ? 0.0f : now;
-          const float a = ex2(m - m0);   // 0 from -inf
-          l *= a;
-          m = now;
-          if (i > 0) {
-#pragma unroll 1
-            for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
-              uint32_t o[16];
-              tmem_load<16>(lanes + Shape::kO + at, o);
-              tmem_load_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
-              tmem_store16(lanes + Shape::kO + at, o);
+        for (int at = 0; at < 32; at += 16) {
+#pragma unroll
+          for (int piece = 0; piece < PP; ++piece) {
+            uint32_t out[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float x0, x1;
+              unpair(s[at + j], x0, x1);
+              const __half2 h = __floats2half2_rn(x0, x1);
+              out[j] = *reinterpret_cast<const uint32_t*>(&h);
+              if (piece + 1 < PP) {
+                const float2 b = __half22float2(h);
+                s[at + j] = pair(x0 - b.x, x1 - b.y);
+              }
             }
+            tmem_store16(lanes + Shape::kP + piece * 64 + 32 * half + at, out);
           }
         }
-        const float m0 = m == -INFINITY ? 0.0f : m;
+        if (i > 0 && any) {
 #pragma unroll 1
-        for (int at = 64 * half; at < 64 * half + 64; at += 16) {
-          float s[16];
-          logits(at, s);
-          float4 fs[4], vs[4];
+          for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
+            uint32_t o[16];
+            tmem_load<16>(lanes + Shape::kO + at, o);
+            tmem_load_wait();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            fs[j] = *reinterpret_cast<const float4*>(&c.f[at + 4 * j]);
-            vs[j] = *reinterpret_cast<const float4*>(&c.inverse[at + 4 * j]);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
+            tmem_store16(lanes + Shape::kO + at, o);
           }
-          uint32_t out[PIECES][8];
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            float y[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int n = j + k;
-              const float f = n & 2 ? (n & 1 ? fs[n / 4].w : fs[n / 4].z) : (n & 1 ? fs[n / 4].y : fs[n / 4].x);
-              const float v = n & 2 ? (n & 1 ? vs[n / 4].w : vs[n / 4].z) : (n & 1 ? vs[n / 4].y : vs[n / 4].x);
-              const float wt = ex2(s[n] - m0);
-              y[k] = wt * f;
-              if (open) {
-                l = fmaf(wt, v, l);
-              } else if (s[n] == -INFINITY) {
-                y[k] = 0.0f;   // f may be NaN
-              } else {
-                l = fmaf(wt, v, l);
-              }
-            }
-#pragma unroll
-            for (int piece = 0; piece < PIECES; ++piece) {
-              const __half2 h = __floats2half2_rn(y[0], y[1]);
-              out[piece][j / 2] = *reinterpret_cast<const uint32_t*>(&h);
-              if (piece + 1 < PIECES) {
-                const float2 b = __half22float2(h);
-                y[0] -= b.x;
-                y[1] -= b.y;
-              }
-            }
-          }
-#pragma unroll
-          for (int piece = 0; piece < PIECES; ++piece) tmem_store8(lanes + Shape::kP + piece * 64 + at / 2, out[piece]);
         }
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&s_empty[buf]);
           mbar_arrive(&cols_empty[buf]);
           mbar_arrive(&p_full);
         }

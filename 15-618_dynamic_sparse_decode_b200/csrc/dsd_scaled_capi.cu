@@ -229,10 +229,11 @@ void WithTc(bool i8, bool fp32, int R, F&& f) {
 constexpr int kTcMaxRows = 8;
 
 template <typename F>
-void WithWide(bool i8, bool fp32, F&& f) {
-  if (i8 && fp32) f(dsds::attn_wide_kernel<true, 2>, Tag<dsds::WideShape<2>>{});
+void WithWide(bool i8, int dtype, F&& f) {
+  const bool two = dtype == DSD_TYPE_F16;
+  if (i8 && two) f(dsds::attn_wide_kernel<true, 2>, Tag<dsds::WideShape<2>>{});
   else if (i8) f(dsds::attn_wide_kernel<true, 1>, Tag<dsds::WideShape<1>>{});
-  else if (fp32) f(dsds::attn_wide_kernel<false, 2>, Tag<dsds::WideShape<2>>{});
+  else if (two) f(dsds::attn_wide_kernel<false, 2>, Tag<dsds::WideShape<2>>{});
   else f(dsds::attn_wide_kernel<false, 1>, Tag<dsds::WideShape<1>>{});
 }
 
@@ -248,7 +249,7 @@ void SetAttentionAttributes() {
               "shared memory attribute");
       };
       for (int R = 1; R <= kTcMaxRows; R *= 2) WithTc(i8, fp32, R, set);
-      WithWide(i8, fp32, set);
+      WithWide(i8, fp32 ? DSD_TYPE_F16 : DSD_TYPE_BF16, set);
     }
 }
 
@@ -353,7 +354,7 @@ AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_s
   // query rows of a request: exact for one query each, the average otherwise
   const int64_t queries = a->q_offsets ? (int64_t(a->total_queries) + a->batch - 1) / a->batch : 1;
   const int64_t rows = queries * group;
-  pl.wide = pl.tc && rows > kTcMaxRows;
+  pl.wide = pl.tc && !fp32 && rows > kTcMaxRows;
   if (pl.wide) pl.R = dsds::kWideRows;
   while (pl.R < kTcMaxRows && pl.R < rows) pl.R *= 2;
   int per_sm = pl.wide ? 1 : 8;
@@ -466,7 +467,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
       kernel<<<p.ncta, pl.wide ? dsds::kWideThreads : dsds::kTcThreads, decltype(tag)::type::kSmem, s>>>(
           p, k_map, v_map, pl.maps.k.head_first);
     };
-    if (pl.wide) WithWide(i8, fp32, launch);
+    if (pl.wide) WithWide(i8, a->dtype, launch);
     else WithTc(i8, fp32, p.R, launch);
   } else if (i8) {
     LaunchSimple<true>(p, s);
