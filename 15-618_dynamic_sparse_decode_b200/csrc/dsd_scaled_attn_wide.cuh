@@ -514,47 +514,51 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         __syncwarp();
         tc_fence_after();
         const bool open = c.open != 0;
-        // two columns a register pair: one instruction for both
-        uint64_t s[32];
-        {
-          uint32_t raw[64];
-          tmem_load<64>(lanes + buf * kTile + 64 * half, raw);
+        // columns lo .. hi of the half are the row's to see
+        const int hi = (open || !p.causal ? kTile : pos - c.place) - 64 * half;
+        const int lo = (open || !p.window ? 0 : max(max(pos - c.place, -1) - p.window + 1, 0)) - 64 * half;
+        const uint64_t factor2 = pair(factor, factor);
+        // 32 columns' logits, two to a register pair: one instruction for both.  They
+        // are made twice, for the maximum and for the weights: 64 kept values left the
+        // scheduler no registers to load ahead (weights 4000 cycles a tile).
+        const auto logits = [&](int at, uint64_t (&s)[16]) {
+          uint32_t raw[32];
+          tmem_load<32>(lanes + buf * kTile + 64 * half + at, raw);
+          ulonglong2 k[8], e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            k[j] = *reinterpret_cast<const ulonglong2*>(&c.ks[64 * half + at + 4 * j]);
+            e[j] = *reinterpret_cast<const ulonglong2*>(&c.e[64 * half + at + 4 * j]);
+          }
           tmem_load_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = pair(raw[2 * j], raw[2 * j + 1]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[buf]);
-        const uint64_t factor2 = pair(factor, factor);
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&c.ks[64 * half + 2 * j]);
-          const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&c.e[64 * half + 2 * j]);
-          s[j] = fma2(mul2(s[j], k.x), factor2, e.x);
-          s[j + 1] = fma2(mul2(s[j + 1], k.y), factor2, e.y);
-        }
-        if (!open) {
-          // columns lo .. hi are the row's to see
-          const int hi = (p.causal ? pos - c.place : kTile) - 64 * half;
-          const int lo = (p.window ? max(max(pos - c.place, -1) - p.window + 1, 0) : 0) - 64 * half;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float a, b;
-            unpair(s[j], a, b);
-            s[j] = pair(2 * j > hi || 2 * j < lo ? -INFINITY : a, 2 * j + 1 > hi || 2 * j + 1 < lo ? -INFINITY : b);
+          for (int j = 0; j < 8; ++j) {
+            s[2 * j] = fma2(mul2(pair(raw[4 * j], raw[4 * j + 1]), k[j].x), factor2, e[j].x);
+            s[2 * j + 1] = fma2(mul2(pair(raw[4 * j + 2], raw[4 * j + 3]), k[j].y), factor2, e[j].y);
           }
-        }
-        float top;
-        {
+          if (!open) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float a, b;
+              unpair(s[j], a, b);
+              s[j] = pair(at + 2 * j > hi || at + 2 * j < lo ? -INFINITY : a,
+                          at + 2 * j + 1 > hi || at + 2 * j + 1 < lo ? -INFINITY : b);
+            }
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int at = 0; at < 64; at += 32) {
+          uint64_t s[16];
+          logits(at, s);
           float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < 16; ++j) {
             float a, b;
             unpair(s[j], a, b);
             t[j & 3] = fmaxf(t[j & 3], fmaxf(a, b));
           }
-          top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
         }
         red[buf][half][row] = top;
         ok = !wide_sync_or(!in);
@@ -569,55 +573,65 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         }
         const float m0 = m == -INFINITY ? 0.0f : -m;
         const uint64_t m2 = pair(m0, m0);
-        uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&c.inverse[64 * half + 2 * j]);
-          const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&c.f[64 * half + 2 * j]);
-          uint64_t w0 = ex2_pair(add2(s[j], m2)), w1 = ex2_pair(add2(s[j + 1], m2));
-          if (open) {
-            sum0 = fma2(w0, v.x, sum0);
-            sum1 = fma2(w1, v.y, sum1);
-            s[j] = mul2(w0, f.x);
-            s[j + 1] = mul2(w1, f.y);
-          } else {
-            // f and inverse of a masked place may be NaN: a weight of zero stays one
-            sum0 = add2(sum0, seen_product(w0, v.x));
-            sum1 = add2(sum1, seen_product(w1, v.y));
-            s[j] = seen_product(w0, f.x);
-            s[j + 1] = seen_product(w1, f.y);
-          }
-        }
-        {
-          float x0, x1;
-          unpair(add2(sum0, sum1), x0, x1);
-          l += x0 + x1;
-        }
         // P and O are the last tile's until its product is done
         if (i > 0) {
           if (!mbar_wait(&o_full, (g - 1) & 1, &stop, p.status)) stop = 1;
           __syncwarp();
           tc_fence_after();
         }
+#pragma unroll 1
+        for (int at = 0; at < 64; at += 32) {
+          uint64_t s[16];
+          logits(at, s);
+          uint64_t sum0 = 0, sum1 = 0;
+          if (open) {
+            ulonglong2 v[8], f[8];
 #pragma unroll
-        for (int at = 0; at < 32; at += 16) {
+            for (int j = 0; j < 8; ++j) {
+              v[j] = *reinterpret_cast<const ulonglong2*>(&c.inverse[64 * half + at + 4 * j]);
+              f[j] = *reinterpret_cast<const ulonglong2*>(&c.f[64 * half + at + 4 * j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint64_t w0 = ex2_pair(add2(s[2 * j], m2)), w1 = ex2_pair(add2(s[2 * j + 1], m2));
+              sum0 = fma2(w0, v[j].x, sum0);
+              sum1 = fma2(w1, v[j].y, sum1);
+              s[2 * j] = mul2(w0, f[j].x);
+              s[2 * j + 1] = mul2(w1, f[j].y);
+            }
+          } else {
+            // f and inverse of a masked place may be NaN: a weight of zero stays one
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const uint64_t v = *reinterpret_cast<const uint64_t*>(&c.inverse[64 * half + at + 2 * j]);
+              const uint64_t f = *reinterpret_cast<const uint64_t*>(&c.f[64 * half + at + 2 * j]);
+              const uint64_t w0 = ex2_pair(add2(s[j], m2));
+              sum0 = add2(sum0, seen_product(w0, v));
+              s[j] = seen_product(w0, f);
+            }
+          }
+          float x0, x1;
+          unpair(add2(sum0, sum1), x0, x1);
+          l += x0 + x1;
 #pragma unroll
           for (int piece = 0; piece < PP; ++piece) {
             uint32_t out[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              float x0, x1;
-              unpair(s[at + j], x0, x1);
+              unpair(s[j], x0, x1);
               const __half2 h = __floats2half2_rn(x0, x1);
               out[j] = *reinterpret_cast<const uint32_t*>(&h);
               if (piece + 1 < PP) {
                 const float2 b = __half22float2(h);
-                s[at + j] = pair(x0 - b.x, x1 - b.y);
+                s[j] = pair(x0 - b.x, x1 - b.y);
               }
             }
-            tmem_store16(lanes + Shape::kP + piece * 64 + 32 * half + at, out);
+            tmem_store16(lanes + Shape::kP + piece * 64 + 32 * half + at / 2, out);
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[buf]);
         if (i > 0 && any) {
 #pragma unroll 1
           for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
