@@ -443,6 +443,9 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
     const int row = tid & 127, half = tid >> 7;
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
     const int d_half = (p.D / 2 + 15) / 16 * 16;   // output elements of the first half, in steps of 16
+    // 16-byte accesses where every row starts on their boundary
+    const bool q_aligned = reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && p.qst[0] % 8 == 0 && p.qst[1] % 8 == 0;
+    const bool out_aligned = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ost[0] % 8 == 0 && p.ost[1] % 8 == 0;
     uint32_t g = 0;
     bool ok = true;
 #pragma unroll 1
@@ -459,15 +462,29 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       float factor = 0.0f;
       if (x.tiles > 0) {
         // queries: half a row a thread, scaled by the row's power of two
-        const uint8_t* q = static_cast<const uint8_t*>(p.q);
-        constexpr int elem = 2;   // fp32 rows take the narrow kernel
-        const bool aligned = reinterpret_cast<uintptr_t>(p.q) % (4 * elem) == 0 && p.qst[0] % 4 == 0 && p.qst[1] % 4 == 0;
-        q += (1ll * (x.q0 + qi) * p.qst[0] + 1ll * q_head * p.qst[1] + 64 * half) * elem;
-        const int n = mine ? min(max(p.D - 64 * half, 0), 64) : 0;
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + 1ll * (x.q0 + qi) * p.qst[0] + 1ll * q_head * p.qst[1] + 64 * half;
+        const int n = mine ? min(max(p.D - 64 * half, 0), 64) : 0;   // a multiple of 16
+        uint4 raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+        if (q_aligned) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (8 * i < n) raw[i] = __ldg(reinterpret_cast<const uint4*>(q) + i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (8 * i < n)
+              raw[i] = make_uint4(q[8 * i] | q[8 * i + 1] << 16, q[8 * i + 2] | q[8 * i + 3] << 16,
+                                  q[8 * i + 4] | q[8 * i + 5] << 16, q[8 * i + 6] | q[8 * i + 7] << 16);
+        }
+        const auto values = [&](int i, int j) {   // elements 8 i + 4 j to + 3
+          return widen_four(make_uint4(j ? raw[i].z : raw[i].x, j ? raw[i].w : raw[i].y, 0, 0), p.dtype);
+        };
         uint32_t top = 0;
-#pragma unroll 4
-        for (int i = 0; i < n; i += 4) {
-          const float4 y = widen_four(load_four(q + i * elem, elem, aligned), p.dtype);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float4 y = values(i / 2, i & 1);
           top = max(top, max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
                              max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w)))));
         }
@@ -477,25 +494,17 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         const int e = max(static_cast<int>(top >> 23) - 127, -100);
         const float f = __uint_as_float(uint32_t(14 - e + 127) << 23);
         factor = top >= 0x7f800000u ? NAN : p.scale_log2 * __uint_as_float(uint32_t(e - 14 + 127) << 23);
-#pragma unroll 2
-        for (int i = 0; i < 64; i += 8) {
-          float v[8];
 #pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i + j < n) y = widen_four(load_four(q + (i + j) * elem, elem, aligned), p.dtype);
-            v[j] = y.x * f;
-            v[j + 1] = y.y * f;
-            v[j + 2] = y.z * f;
-            v[j + 3] = y.w * f;
-          }
+        for (int i = 0; i < 8; ++i) {
           uint32_t out[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            out[j] = *reinterpret_cast<const uint32_t*>(&h);
+          for (int j = 0; j < 2; ++j) {
+            const float4 y = values(i, j);
+            const __half2 a = __floats2half2_rn(y.x * f, y.y * f), b = __floats2half2_rn(y.z * f, y.w * f);
+            out[2 * j] = *reinterpret_cast<const uint32_t*>(&a);
+            out[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&b);
           }
-          *reinterpret_cast<uint4*>(q16 + half * kTcTileBytes + row * 128 + (((i >> 3) ^ (row & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(q16 + half * kTcTileBytes + row * 128 + ((i ^ (row & 7)) << 4)) =
               make_uint4(out[0], out[1], out[2], out[3]);
         }
         proxy_fence();
@@ -677,8 +686,27 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         }
         if (!mine) continue;
         if (whole) {
+          uint32_t packed[8];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) store_elem(p.out, out_at + at + j, p.dtype, l == 0.0f ? 0.0f : __uint_as_float(o[j]) * one);
+          for (int j = 0; j < 8; ++j) {
+            const float y0 = l == 0.0f ? 0.0f : __uint_as_float(o[2 * j]) * one;
+            const float y1 = l == 0.0f ? 0.0f : __uint_as_float(o[2 * j + 1]) * one;
+            if (p.dtype == DSD_TYPE_BF16) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
+              packed[j] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+              const __half2 h = __floats2half2_rn(y0, y1);
+              packed[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+          uint16_t* to = static_cast<uint16_t*>(p.out) + out_at + at;
+          if (out_aligned) {
+            reinterpret_cast<uint4*>(to)[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            reinterpret_cast<uint4*>(to)[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) to[j] = static_cast<uint16_t>(packed[j / 2] >> (j & 1 ? 16 : 0));
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 16; j += 4)
