@@ -11,9 +11,12 @@
 // 2^-29 of the row's largest).  Weights go back to TMEM as fp16 (2^-12 of their
 // value) and are the A operand of the second product there.
 //
-// A thread owns half a row of S: the running maximum and sum are its own, two
-// threads meet once a tile for the row's maximum.  O stays in TMEM and is rescaled
-// only when a row's maximum has grown by more than 2^8, which fp16 weights bear.
+// A thread owns half a row of S: the running sum is its own, the reference that the
+// weights are taken from is the row's.  It stays while no maximum has grown past it
+// by more than 2^8, which fp16 weights bear, so that a tile is one pass over its
+// logits; when one has, the eight warps vote, O is rescaled in TMEM and the weights
+// are made again (with a pass for the maximum every tile: 544 us against the chunk
+// case's present figure in the design notes).
 //
 // Roles: warps 0-7 softmax, 8-11 widen the codes, 12 TMA, 13 MMA issue, 14 token
 // data, 15 units.
@@ -108,6 +111,11 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
   float a, b;
   unpair(x, a, b);
   return pair(ex2(a), ex2(b));
+}
+__device__ __forceinline__ float max_pair(float m, uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  return fmaxf(m, fmaxf(a, b));
 }
 // w * x, 0 where w is 0 whatever x is
 __device__ __forceinline__ uint64_t seen_product(uint64_t w, uint64_t x) {
@@ -555,103 +563,108 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
             }
           }
         };
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int at = 0; at < 64; at += 32) {
-          uint64_t s[16];
-          logits(at, s);
-          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float a, b;
-            unpair(s[j], a, b);
-            t[j & 3] = fmaxf(t[j & 3], fmaxf(a, b));
-          }
-          top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-        }
-        red[buf][half][row] = top;
-        ok = !wide_sync_or(!in);
-        top = fmaxf(top, red[buf][half ^ 1][row]);
-        const bool grows = top > m + kWideGrow || (m == -INFINITY && top > m);
-        const bool any = __any_sync(~0u, grows);
-        float a = 1.0f;
-        if (grows) {
-          a = ex2(m - top);   // 0 from -inf
-          l *= a;
-          m = top;
-        }
-        const float m0 = m == -INFINITY ? 0.0f : -m;
-        const uint64_t m2 = pair(m0, m0);
         // P and O are the last tile's until its product is done
         if (i > 0) {
-          if (!mbar_wait(&o_full, (g - 1) & 1, &stop, p.status)) stop = 1;
+          in = mbar_wait(&o_full, (g - 1) & 1, &stop, p.status) && in;
           __syncwarp();
           tc_fence_after();
         }
+        // The half's weights under the reference m0, into P; their sum and the largest logit.
+        const auto weigh = [&](float m0, float& top) {
+          const uint64_t m2 = pair(-m0, -m0);
+          float sum = 0.0f;
 #pragma unroll 1
-        for (int at = 0; at < 64; at += 32) {
-          uint64_t s[16];
-          logits(at, s);
-          uint64_t sum0 = 0, sum1 = 0;
-          if (open) {
-            ulonglong2 v[8], f[8];
+          for (int at = 0; at < 64; at += 32) {
+            uint64_t s[16];
+            logits(at, s);
+            float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            uint64_t sum0 = 0, sum1 = 0;
+            if (open) {
+              ulonglong2 v[8], f[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              v[j] = *reinterpret_cast<const ulonglong2*>(&c.inverse[64 * half + at + 4 * j]);
-              f[j] = *reinterpret_cast<const ulonglong2*>(&c.f[64 * half + at + 4 * j]);
-            }
+              for (int j = 0; j < 8; ++j) {
+                v[j] = *reinterpret_cast<const ulonglong2*>(&c.inverse[64 * half + at + 4 * j]);
+                f[j] = *reinterpret_cast<const ulonglong2*>(&c.f[64 * half + at + 4 * j]);
+              }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint64_t w0 = ex2_pair(add2(s[2 * j], m2)), w1 = ex2_pair(add2(s[2 * j + 1], m2));
-              sum0 = fma2(w0, v[j].x, sum0);
-              sum1 = fma2(w1, v[j].y, sum1);
-              s[2 * j] = mul2(w0, f[j].x);
-              s[2 * j + 1] = mul2(w1, f[j].y);
-            }
-          } else {
-            // f and inverse of a masked place may be NaN: a weight of zero stays one
+              for (int j = 0; j < 8; ++j) {
+                t[2 * j & 3] = max_pair(t[2 * j & 3], s[2 * j]);
+                t[(2 * j + 1) & 3] = max_pair(t[(2 * j + 1) & 3], s[2 * j + 1]);
+                const uint64_t w0 = ex2_pair(add2(s[2 * j], m2)), w1 = ex2_pair(add2(s[2 * j + 1], m2));
+                sum0 = fma2(w0, v[j].x, sum0);
+                sum1 = fma2(w1, v[j].y, sum1);
+                s[2 * j] = mul2(w0, f[j].x);
+                s[2 * j + 1] = mul2(w1, f[j].y);
+              }
+            } else {
+              // f and inverse of a masked place may be NaN: a weight of zero stays one
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const uint64_t v = *reinterpret_cast<const uint64_t*>(&c.inverse[64 * half + at + 2 * j]);
-              const uint64_t f = *reinterpret_cast<const uint64_t*>(&c.f[64 * half + at + 2 * j]);
-              const uint64_t w0 = ex2_pair(add2(s[j], m2));
-              sum0 = add2(sum0, seen_product(w0, v));
-              s[j] = seen_product(w0, f);
-            }
-          }
-          float x0, x1;
-          unpair(add2(sum0, sum1), x0, x1);
-          l += x0 + x1;
-#pragma unroll
-          for (int piece = 0; piece < PP; ++piece) {
-            uint32_t out[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              unpair(s[j], x0, x1);
-              const __half2 h = __floats2half2_rn(x0, x1);
-              out[j] = *reinterpret_cast<const uint32_t*>(&h);
-              if (piece + 1 < PP) {
-                const float2 b = __half22float2(h);
-                s[j] = pair(x0 - b.x, x1 - b.y);
+              for (int j = 0; j < 16; ++j) {
+                const uint64_t v = *reinterpret_cast<const uint64_t*>(&c.inverse[64 * half + at + 2 * j]);
+                const uint64_t f = *reinterpret_cast<const uint64_t*>(&c.f[64 * half + at + 2 * j]);
+                t[j & 3] = max_pair(t[j & 3], s[j]);
+                const uint64_t w0 = ex2_pair(add2(s[j], m2));
+                sum0 = add2(sum0, seen_product(w0, v));
+                s[j] = seen_product(w0, f);
               }
             }
-            tmem_store16(lanes + Shape::kP + piece * 64 + 32 * half + at / 2, out);
+            top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+            float x0, x1;
+            unpair(add2(sum0, sum1), x0, x1);
+            sum += x0 + x1;
+#pragma unroll
+            for (int piece = 0; piece < PP; ++piece) {
+              uint32_t out[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                unpair(s[j], x0, x1);
+                const __half2 h = __floats2half2_rn(x0, x1);
+                out[j] = *reinterpret_cast<const uint32_t*>(&h);
+                if (piece + 1 < PP) {
+                  const float2 b = __half22float2(h);
+                  s[j] = pair(x0 - b.x, x1 - b.y);
+                }
+              }
+              tmem_store16(lanes + Shape::kP + piece * 64 + 32 * half + at / 2, out);
+            }
+          }
+          return sum;
+        };
+        // One pass on the reference of the tiles so far; where a row's maximum has grown
+        // past what fp16 bears (seldom after the first tile), all eight warps agree on
+        // new references and make the weights again.
+        float top = -INFINITY;
+        float sum = weigh(m == -INFINITY ? 0.0f : m, top);
+        const auto grown = [&](float t) { return t > m + kWideGrow || (m == -INFINITY && t > m); };
+        if (wide_sync_or(grown(top) || !in)) {
+          ok = !wide_sync_or(!in);
+          if (!ok) break;
+          red[buf][half][row] = top;
+          wide_sync_or(false);
+          top = fmaxf(top, red[buf][half ^ 1][row]);
+          float a = 1.0f;
+          if (grown(top)) {
+            a = ex2(m - top);   // 0 from -inf
+            l *= a;
+            m = top;
+          }
+          sum = weigh(m == -INFINITY ? 0.0f : m, top);
+          if (i > 0) {
+#pragma unroll 1
+            for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
+              uint32_t o[16];
+              tmem_load<16>(lanes + Shape::kO + at, o);
+              tmem_load_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
+              tmem_store16(lanes + Shape::kO + at, o);
+            }
           }
         }
+        l += sum;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_empty[buf]);
-        if (i > 0 && any) {
-#pragma unroll 1
-          for (int at = half ? d_half : 0; at < (half ? p.D : d_half); at += 16) {
-            uint32_t o[16];
-            tmem_load<16>(lanes + Shape::kO + at, o);
-            tmem_load_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
-            tmem_store16(lanes + Shape::kO + at, o);
-          }
-        }
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
