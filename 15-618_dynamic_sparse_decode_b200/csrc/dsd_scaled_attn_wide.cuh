@@ -9,7 +9,12 @@
 // does what the narrow kernel needs three 8-bit pieces for.  Queries are scaled by
 // a power of two of their row into fp16's range (exact for fp16 and for bf16 within
 // 2^-29 of the row's largest).  Weights go back to TMEM as fp16 (2^-12 of their
-// value) and are the A operand of the second product there.
+// value) and are the A operand of the second product there.  A weight carries its
+// value scale: P = 2^(s - r) vs with the row's reference r taken from the largest
+// logit and the largest value scale, so that O / sum is the output as it stands and a
+// column has two constants, its scales (with the exponent of vs in the logits, as in
+// the narrow kernel, it had four, and their loads were a quarter of the pass).  A
+// token's weight keeps its bits down to 2^-20 of that largest product.
 //
 // A thread owns half a row of S: the running sum is its own, the reference that the
 // weights are taken from is the row's.  It stays while no maximum has grown past it
@@ -29,7 +34,7 @@ namespace dsds {
 constexpr int kWideThreads = 512;
 constexpr int kWideRows = 128;
 constexpr float kWideGrow = 8.0f;     // log2 of how far a maximum may run behind
-constexpr float kWideOne = 64.0f;     // fp16 value of weight 1: 2^6 2^8 f < 2^15
+constexpr float kWideOne = 6.0f;      // log2 of the largest weight on a fresh reference
 
 // PP: fp16 pieces of a weight.  One for bf16, whose outputs are far coarser than a
 // weight's 2^-12; two for fp16, or the weights' rounding would add to the output's
@@ -168,8 +173,10 @@ __device__ __forceinline__ void widen_row(const uint8_t* codes, uint8_t* wide, i
 
 // A tile's tokens as the softmax reads them, four at a time.
 struct __align__(16) Columns {   // its size too: float4 reads of the second one
-  float ks[kTile], e[kTile], f[kTile], inverse[kTile];
-  int place, open;
+  float ks[kTile], vs[kTile];
+  uint32_t valid[4];   // a bit per token
+  uint32_t largest[4]; // value scale of each 32 tokens, as bits
+  int place, open;     // open: every row sees every token that is there
 };
 
 template <bool I8, int PP>
@@ -417,14 +424,17 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         ok = ok && mbar_wait(&v_full[s], sp, &stop, p.status);
         nan_row = valid && row_has_nan(reinterpret_cast<const uint4*>(v_codes + t * 128), lane);
       }
-      TokenScale x = token_scale(valid ? scales.y : 0.0f);
-      if (nan_row) x.factor = x.inverse = NAN;
+      const float vs = !valid ? 0.0f : nan_row ? NAN : scales.y;
+      const uint32_t present = __ballot_sync(~0u, valid);
+      const uint32_t largest = __reduce_max_sync(~0u, vs < INFINITY ? __float_as_uint(vs) : 0u);
       ok = ok && mbar_wait(&cols_empty[cb], (g >> 1 & 1) ^ 1, &stop, p.status);
       Columns& c = cols[cb];
       c.ks[t] = valid ? scales.x : 0.0f;
-      c.e[t] = valid ? x.e : -INFINITY;
-      c.f[t] = valid ? x.factor * kWideOne : 0.0f;
-      c.inverse[t] = valid ? x.inverse : 0.0f;
+      c.vs[t] = vs;
+      if (lane == 0) {
+        c.valid[t >> 5] = present;
+        c.largest[t >> 5] = largest;
+      }
       if (t == 0) {
         c.place = tile.place;
         c.open = tile.open;
@@ -500,8 +510,9 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         wide_sync_or(false);
         top = max(__float_as_uint(red[0][0][row]), __float_as_uint(red[0][1][row]));
         const int e = max(static_cast<int>(top >> 23) - 127, -100);
-        const float f = __uint_as_float(uint32_t(14 - e + 127) << 23);
-        factor = top >= 0x7f800000u ? NAN : p.scale_log2 * __uint_as_float(uint32_t(e - 14 + 127) << 23);
+        // a negative scale turns the query: the largest product is the largest logit then
+        const float f = copysignf(__uint_as_float(uint32_t(14 - e + 127) << 23), p.scale_log2);
+        factor = top >= 0x7f800000u ? NAN : fabsf(p.scale_log2) * __uint_as_float(uint32_t(e - 14 + 127) << 23);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           uint32_t out[4];
@@ -530,87 +541,64 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         in = mbar_wait(&s_full[buf], g >> 1 & 1, &stop, p.status) && in;
         __syncwarp();
         tc_fence_after();
-        const bool open = c.open != 0;
-        // columns lo .. hi of the half are the row's to see
-        const int hi = (open || !p.causal ? kTile : pos - c.place) - 64 * half;
-        const int lo = (open || !p.window ? 0 : max(max(pos - c.place, -1) - p.window + 1, 0)) - 64 * half;
-        const uint64_t factor2 = pair(factor, factor);
-        // 32 columns' logits, two to a register pair: one instruction for both.  They
-        // are made twice, for the maximum and for the weights: 64 kept values left the
-        // scheduler no registers to load ahead (weights 4000 cycles a tile).
-        const auto logits = [&](int at, uint64_t (&s)[16]) {
-          uint32_t raw[32];
-          tmem_load<32>(lanes + buf * kTile + 64 * half + at, raw);
-          ulonglong2 k[8], e[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            k[j] = *reinterpret_cast<const ulonglong2*>(&c.ks[64 * half + at + 4 * j]);
-            e[j] = *reinterpret_cast<const ulonglong2*>(&c.e[64 * half + at + 4 * j]);
-          }
-          tmem_load_wait();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            s[2 * j] = fma2(mul2(pair(raw[4 * j], raw[4 * j + 1]), k[j].x), factor2, e[j].x);
-            s[2 * j + 1] = fma2(mul2(pair(raw[4 * j + 2], raw[4 * j + 3]), k[j].y), factor2, e[j].y);
-          }
-          if (!open) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float a, b;
-              unpair(s[j], a, b);
-              s[j] = pair(at + 2 * j > hi || at + 2 * j < lo ? -INFINITY : a,
-                          at + 2 * j + 1 > hi || at + 2 * j + 1 < lo ? -INFINITY : b);
-            }
-          }
-        };
+        const uint4 valid = *reinterpret_cast<const uint4*>(c.valid), largest = *reinterpret_cast<const uint4*>(c.largest);
+        const bool open = c.open != 0 && (valid.x & valid.y & valid.z & valid.w) == ~0u;
+        // 2^scale_up bounds the tile's value scales from above
+        const int top_bits = static_cast<int>(max(max(largest.x, largest.y), max(largest.z, largest.w)) >> 23) - 126;
+        const float scale_up = static_cast<float>(min(max(top_bits, -64), 100));
         // P and O are the last tile's until its product is done
         if (i > 0) {
           in = mbar_wait(&o_full, (g - 1) & 1, &stop, p.status) && in;
           __syncwarp();
           tc_fence_after();
         }
-        // The half's weights under the reference m0, into P; their sum and the largest logit.
-        const auto weigh = [&](float m0, float& top) {
-          const uint64_t m2 = pair(-m0, -m0);
+        // The half's weights under the reference r, into P; their sum and the largest
+        // product S ks.  Values lie two to a register pair: one instruction for both.
+        const auto weigh = [&](float r, float& top) {
+          const uint64_t factor2 = pair(factor, factor), r2 = pair(-r, -r);
           float sum = 0.0f;
 #pragma unroll 1
-          for (int at = 0; at < 64; at += 32) {
-            uint64_t s[16];
-            logits(at, s);
+          for (int at = 64 * half; at < 64 * half + 64; at += 32) {
+            uint32_t raw[32];
+            tmem_load<32>(lanes + buf * kTile + at, raw);
+            ulonglong2 k[8], v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const ulonglong2*>(&c.ks[at + 4 * j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const ulonglong2*>(&c.vs[at + 4 * j]);
+            tmem_load_wait();
             float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            uint64_t sum0 = 0, sum1 = 0;
+            uint64_t sums[2] = {0, 0}, s[16];
             if (open) {
-              ulonglong2 v[8], f[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                v[j] = *reinterpret_cast<const ulonglong2*>(&c.inverse[64 * half + at + 4 * j]);
-                f[j] = *reinterpret_cast<const ulonglong2*>(&c.f[64 * half + at + 4 * j]);
-              }
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                t[2 * j & 3] = max_pair(t[2 * j & 3], s[2 * j]);
-                t[(2 * j + 1) & 3] = max_pair(t[(2 * j + 1) & 3], s[2 * j + 1]);
-                const uint64_t w0 = ex2_pair(add2(s[2 * j], m2)), w1 = ex2_pair(add2(s[2 * j + 1], m2));
-                sum0 = fma2(w0, v[j].x, sum0);
-                sum1 = fma2(w1, v[j].y, sum1);
-                s[2 * j] = mul2(w0, f[j].x);
-                s[2 * j + 1] = mul2(w1, f[j].y);
-              }
-            } else {
-              // f and inverse of a masked place may be NaN: a weight of zero stays one
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                const uint64_t v = *reinterpret_cast<const uint64_t*>(&c.inverse[64 * half + at + 2 * j]);
-                const uint64_t f = *reinterpret_cast<const uint64_t*>(&c.f[64 * half + at + 2 * j]);
-                t[j & 3] = max_pair(t[j & 3], s[j]);
-                const uint64_t w0 = ex2_pair(add2(s[j], m2));
-                sum0 = add2(sum0, seen_product(w0, v));
-                s[j] = seen_product(w0, f);
+                const uint64_t x = mul2(pair(raw[2 * j], raw[2 * j + 1]), j & 1 ? k[j / 2].y : k[j / 2].x);
+                t[j & 3] = max_pair(t[j & 3], x);
+                const uint64_t w = ex2_pair(fma2(x, factor2, r2));
+                sums[j & 1] = add2(sums[j & 1], w);
+                s[j] = mul2(w, j & 1 ? v[j / 2].y : v[j / 2].x);
+              }
+            } else {
+              // columns lo .. hi are the row's to see
+              const int hi = (p.causal ? pos - c.place : kTile) - at;
+              const int lo = (p.window ? max(max(pos - c.place, -1) - p.window + 1, 0) : 0) - at;
+              const uint32_t there = c.valid[at / 32];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float a, b;
+                unpair(mul2(pair(raw[2 * j], raw[2 * j + 1]), j & 1 ? k[j / 2].y : k[j / 2].x), a, b);
+                const bool see_a = (there >> (2 * j) & 1) && 2 * j <= hi && 2 * j >= lo;
+                const bool see_b = (there >> (2 * j + 1) & 1) && 2 * j + 1 <= hi && 2 * j + 1 >= lo;
+                t[j & 3] = fmaxf(t[j & 3], fmaxf(see_a ? a : -INFINITY, see_b ? b : -INFINITY));
+                const uint64_t w = pair(see_a ? ex2(fmaf(a, factor, -r)) : 0.0f, see_b ? ex2(fmaf(b, factor, -r)) : 0.0f);
+                sums[j & 1] = add2(sums[j & 1], w);
+                // the scale of a place that the row does not see may be NaN
+                s[j] = seen_product(w, j & 1 ? v[j / 2].y : v[j / 2].x);
               }
             }
             top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
             float x0, x1;
-            unpair(add2(sum0, sum1), x0, x1);
+            unpair(add2(sums[0], sums[1]), x0, x1);
             sum += x0 + x1;
 #pragma unroll
             for (int piece = 0; piece < PP; ++piece) {
@@ -625,28 +613,30 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
                   s[j] = pair(x0 - b.x, x1 - b.y);
                 }
               }
-              tmem_store16(lanes + Shape::kP + piece * 64 + 32 * half + at / 2, out);
+              tmem_store16(lanes + Shape::kP + piece * 64 + at / 2, out);
             }
           }
           return sum;
         };
-        // One pass on the reference of the tiles so far; where a row's maximum has grown
-        // past what fp16 bears (seldom after the first tile), all eight warps agree on
-        // new references and make the weights again.
+        // One pass on the reference of the tiles so far; where a row's largest product
+        // has grown past what fp16 bears (seldom after the first tile), all eight warps
+        // agree on new references and make the weights again.
         float top = -INFINITY;
         float sum = weigh(m == -INFINITY ? 0.0f : m, top);
-        const auto grown = [&](float t) { return t > m + kWideGrow || (m == -INFINITY && t > m); };
-        if (wide_sync_or(grown(top) || !in)) {
+        // the reference that this tile alone would take (-inf: the row sees nothing of it)
+        const auto fresh = [&](float t) { return t == -INFINITY ? -INFINITY : t * factor + scale_up - kWideOne; };
+        const auto grown = [&](float f) { return f > m + kWideGrow || (m == -INFINITY && f > m); };
+        if (wide_sync_or(grown(fresh(top)) || !in)) {
           ok = !wide_sync_or(!in);
           if (!ok) break;
           red[buf][half][row] = top;
           wide_sync_or(false);
-          top = fmaxf(top, red[buf][half ^ 1][row]);
+          const float now = fresh(fmaxf(top, red[buf][half ^ 1][row]));
           float a = 1.0f;
-          if (grown(top)) {
-            a = ex2(m - top);   // 0 from -inf
+          if (grown(now)) {
+            a = ex2(m - now);   // 0 from -inf
             l *= a;
-            m = top;
+            m = now;
           }
           sum = weigh(m == -INFINITY ? 0.0f : m, top);
           if (i > 0) {
@@ -684,7 +674,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       if (!ok) break;
       l = red[0][0][row] + red[0][1][row];
       const bool whole = x.opens && x.ends;
-      const float one = whole ? (l == 0.0f ? 0.0f : 1.0f / l / kWideOne) : 1.0f / kWideOne;
+      const float one = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
       const long long piece_at = (2ll * cta + x.opens) * p.R + row;
       const long long out_at = 1ll * (x.q0 + qi) * p.ost[0] + 1ll * q_head * p.ost[1];
 #pragma unroll 1
