@@ -20,7 +20,8 @@
 namespace dsds {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendKeep = 4;   // slots (of 2*VE values) a lane keeps in registers
+constexpr int kAppendKeep = 2;   // slots (of 2*VE values) a lane keeps in registers
+constexpr int kAppendHeads = 4;  // query heads a lane has in flight
 
 struct AppendParams {
   uint8_t* k;
@@ -47,6 +48,7 @@ struct AppendParams {
   int* status;
   int slots;   // slots of a row
   int team;    // warps per (block, head)
+  int y_kv;    // blockIdx.y below: keys and values; from there on: queries
 };
 
 template <bool I8>
@@ -155,18 +157,23 @@ __device__ __forceinline__ Slot<VE> slot_of(const AppendParams& p, int s) {
 }
 
 template <typename T, int VE>
-__device__ __forceinline__ void load_slot(const AppendParams& p, const T* row, const Slot<VE>& s, int pos,
-                                          bool turn, float (&x)[2 * VE]) {
+__device__ __forceinline__ void load_pair(const T* row, const Slot<VE>& s, float (&x)[2 * VE]) {
   load_vec<T, VE>(row + s.e0, x);
   if (s.two) load_vec<T, VE>(row + s.e1, x + VE);
   else
 #pragma unroll
     for (int i = 0; i < VE; ++i) x[VE + i] = 0.0f;
-  if (!turn || !s.turned) return;
-  float c[VE], n[VE];
+}
+
+template <int VE>
+__device__ __forceinline__ void load_angles(const AppendParams& p, const Slot<VE>& s, int pos, float (&c)[VE], float (&n)[VE]) {
   const long long at = 1ll * pos * (p.rd / 2) + s.angle;
   load_table<VE>(p.cos + at, c);
   load_table<VE>(p.sin + at, n);
+}
+
+template <int VE>
+__device__ __forceinline__ void turn_slot(const AppendParams& p, const float (&c)[VE], const float (&n)[VE], float (&x)[2 * VE]) {
   // unfused: the same bits as a product, a product and their sum in fp32
   const auto turn_pair = [](float& a, float& b, float c, float n) {
     const float y = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, n));
@@ -182,6 +189,16 @@ __device__ __forceinline__ void load_slot(const AppendParams& p, const T* row, c
   }
 }
 
+template <typename T, int VE>
+__device__ __forceinline__ void load_slot(const AppendParams& p, const T* row, const Slot<VE>& s, int pos,
+                                          bool turn, float (&x)[2 * VE]) {
+  load_pair<T, VE>(row, s, x);
+  if (!turn || !s.turned) return;
+  float c[VE], n[VE];
+  load_angles<VE>(p, s, pos, c, n);
+  turn_slot<VE>(p, c, n, x);
+}
+
 template <int VE>
 __device__ __forceinline__ float finite_max(const float (&x)[2 * VE], float m) {
 #pragma unroll
@@ -193,8 +210,8 @@ __device__ __forceinline__ float finite_max(const float (&x)[2 * VE], float m) {
 }
 
 template <typename T, bool I8, int VE>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ float team_max[kAppendThreads / 32];
+__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ float team_max[2][kAppendThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int u = blockIdx.x;
   int b = u, row0 = u, n = 1, i = 0;
@@ -238,23 +255,58 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
   const int teams = kAppendThreads / 32 / p.team;
   const int team = warp / p.team, rank = warp % p.team * 32 + lane, width = p.team * 32;
-  const int items = 2 * p.Hk + p.Hq;
+  const int items = 2 * p.Hk;
   const int work = ntok * p.slots;
   const auto position = [&](int t) {
     return p.positions ? p.positions[row + t] : static_cast<int>(from) + t;
   };
   const auto in_table = [&](int pos) { return !p.cos || (pos >= 0 && pos < p.rot_positions); };
-  for (int base = blockIdx.y * teams; base < items; base += gridDim.y * teams) {
+  if (blockIdx.y >= p.y_kv) {
+    // ---- queries: a lane keeps its slot's angles and takes the heads in turn
+    const int groups = max(1, kAppendThreads / work);   // lanes that share a slot
+    const int q_parts = gridDim.y - p.y_kv, q_part = blockIdx.y - p.y_kv;
+    const int stride = groups * q_parts;
+    for (int at = threadIdx.x; at < work * groups; at += kAppendThreads) {
+      const int slot = at % work, t = slot / p.slots, pos = position(t);
+      if (!in_table(pos)) {
+        if (p.status) atomicOr(p.status, DSD_SCALED_BAD_POSITION);
+        continue;
+      }
+      const Slot<VE> s = slot_of<VE>(p, slot % p.slots);
+      const bool turn = p.cos && s.turned;
+      float c[VE], n[VE];
+      if (turn) load_angles<VE>(p, s, pos, c, n);
+      const T* in = static_cast<const T*>(p.qin) + (row + t) * p.qin_st[0];
+      T* out = static_cast<T*>(p.qout) + (row + t) * p.qout_st[0];
+      for (int h0 = at / work * q_parts + q_part; h0 < p.Hq; h0 += kAppendHeads * stride) {
+        float x[kAppendHeads][2 * VE];
+#pragma unroll
+        for (int j = 0; j < kAppendHeads; ++j)
+          if (h0 + j * stride < p.Hq) load_pair<T, VE>(in + (h0 + j * stride) * p.qin_st[1], s, x[j]);
+#pragma unroll
+        for (int j = 0; j < kAppendHeads; ++j)
+          if (h0 + j * stride < p.Hq) {
+            if (turn) turn_slot<VE>(p, c, n, x[j]);
+            T* o = out + (h0 + j * stride) * p.qout_st[1];
+            store_vec<T, VE>(o + s.e0, x[j]);
+            if (s.two) store_vec<T, VE>(o + s.e1, x[j] + VE);
+          }
+      }
+    }
+    return;
+  }
+  int flip = 0;
+  for (int base = blockIdx.y * teams; base < items; base += p.y_kv * teams) {
     const int item = base + team;
-    const bool is_q = item >= 2 * p.Hk, is_v = !is_q && item >= p.Hk;
-    const int head = is_q ? item - 2 * p.Hk : is_v ? item - p.Hk : item;
+    const bool is_v = item >= p.Hk;
+    const int head = is_v ? item - p.Hk : item;
     const bool turn = p.cos && !is_v;
-    const bool on = item < items && (is_q || good);
-    const long long* in_st = is_q ? p.qin_st : is_v ? p.vin_st : p.kin_st;
-    const T* in = static_cast<const T*>(is_q ? p.qin : is_v ? p.vin : p.kin) + row * in_st[0] + head * in_st[1];
+    const bool on = item < items && good;
+    const long long* in_st = is_v ? p.vin_st : p.kin_st;
+    const T* in = static_cast<const T*>(is_v ? p.vin : p.kin) + row * in_st[0] + head * in_st[1];
     const long long si = (1ll * page * p.Hk + head) * p.nblk + first / p.bt;
     float* scales = is_v ? p.vs : p.ks;
-    const float old = on && !is_q && held ? scales[si] : 0.0f;
+    const float old = on && held ? scales[si] : 0.0f;
 
     float keep[kAppendKeep][2 * VE];
     bool live[kAppendKeep];
@@ -274,7 +326,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         }
       }
     }
-    if (on && !is_q)
+    if (on)
       for (int at = kAppendKeep * width + rank; at < work; at += width) {
         const int t = at / p.slots, pos = position(t);
         if (!in_table(pos)) {
@@ -288,33 +340,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     // non-negative floats order like their bits
     m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(m)));
     if (p.team > 1) {
-      __syncthreads();   // the last round's maxima have been read
-      if (lane == 0) team_max[warp] = m;
+      // two arrays in turn: one is read while the next round's is written
+      if (lane == 0) team_max[flip][warp] = m;
       __syncthreads();
-      for (int j = 0; j < p.team; ++j) m = fmaxf(m, team_max[team * p.team + j]);
+      for (int j = 0; j < p.team; ++j) m = fmaxf(m, team_max[flip][team * p.team + j]);
+      flip ^= 1;
     }
     if (!on) continue;
-
-    if (is_q) {
-      T* out = static_cast<T*>(p.qout) + row * p.qout_st[0] + head * p.qout_st[1];
-      const auto put = [&](int at, const float (&x)[2 * VE]) {
-        const Slot<VE> s = slot_of<VE>(p, at % p.slots);
-        T* o = out + at / p.slots * p.qout_st[0];
-        store_vec<T, VE>(o + s.e0, x);
-        if (s.two) store_vec<T, VE>(o + s.e1, x + VE);
-      };
-#pragma unroll
-      for (int j = 0; j < kAppendKeep; ++j)
-        if (live[j]) put(j * width + rank, keep[j]);
-      for (int at = kAppendKeep * width + rank; at < work; at += width) {
-        const int t = at / p.slots, pos = position(t);
-        if (!in_table(pos)) continue;
-        float x[2 * VE];
-        load_slot<T, VE>(p, in + t * in_st[0], slot_of<VE>(p, at % p.slots), pos, turn, x);
-        put(at, x);
-      }
-      continue;
-    }
 
     constexpr float kQmax = I8 ? 127.0f : 448.0f;
     const float fresh = m < 7.888609052210118e-31f ? 0.0f : m * (1.0f / kQmax);   // 2^-100

@@ -183,11 +183,17 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   const int block_slots = (p.off ? std::min(p.bt, p.total) : 1) * p.slots;
   p.team = 1;
   while (p.team < 8 && p.team * 32 * dsds::kAppendKeep < block_slots) p.team *= 2;
+  // blockIdx.y: CTAs of one block of tokens, keys and values first, then queries;
+  // as many as fill the GPU eight times over when there are few blocks, and no more
+  // than four rounds (of heads) to a CTA when there are many
   const int teams = dsds::kAppendThreads / 32 / p.team;
-  const int items = 2 * p.Hk + p.Hq, rounds = (items + teams - 1) / teams;
-  const int64_t want = 8ll * dev.sms;
-  const int y = int(std::min<int64_t>(std::min(rounds, 65535), std::max<int64_t>(1, (want + units - 1) / units)));
-  const dim3 grid{static_cast<unsigned>(units), static_cast<unsigned>(y), 1};
+  const auto parts = [&](int rounds) {
+    const int64_t want = (8ll * dev.sms + units - 1) / units;
+    return int(std::min<int64_t>(rounds, std::max<int64_t>(want, (rounds + 3) / 4)));
+  };
+  p.y_kv = parts((2 * p.Hk + teams - 1) / teams);
+  const int y_q = p.Hq ? parts((p.Hq + 4 * dsds::kAppendHeads - 1) / (4 * dsds::kAppendHeads)) : 0;
+  const dim3 grid{static_cast<unsigned>(units), static_cast<unsigned>(p.y_kv + y_q), 1};
   const bool i8 = c->kv_format == DSD_KV_I8_SCALED;
   if (a->dtype == DSD_TYPE_F32) LaunchAppend<float>(p, i8, ve, grid, s);
   else if (a->dtype == DSD_TYPE_BF16) LaunchAppend<__nv_bfloat16>(p, i8, ve, grid, s);
