@@ -165,6 +165,31 @@ __device__ __forceinline__ void load_pair(const T* row, const Slot<VE>& s, float
     for (int i = 0; i < VE; ++i) x[VE + i] = 0.0f;
 }
 
+// A slot as it lies in memory.
+template <typename T, int VE>
+struct RawSlot {
+  __align__(16) T v[2 * VE];
+
+  __device__ __forceinline__ void load(const T* row, const Slot<VE>& s) {
+    if constexpr (VE == 1) {
+      v[0] = row[s.e0];
+      v[1] = s.two ? row[s.e1] : T(0.0f);
+    } else {
+      constexpr int kVecs = VE * sizeof(T) / 16;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row + s.e0) + i);
+        reinterpret_cast<uint4*>(v)[kVecs + i] =
+            s.two ? __ldg(reinterpret_cast<const uint4*>(row + s.e1) + i) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void widen(float (&x)[2 * VE]) const {
+#pragma unroll
+    for (int i = 0; i < 2 * VE; ++i) x[i] = to_float(v[i]);
+  }
+};
+
 template <int VE>
 __device__ __forceinline__ void load_angles(const AppendParams& p, const Slot<VE>& s, int pos, float (&c)[VE], float (&n)[VE]) {
   const long long at = 1ll * pos * (p.rd / 2) + s.angle;
@@ -263,6 +288,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_
   const auto in_table = [&](int pos) { return !p.cos || (pos >= 0 && pos < p.rot_positions); };
   if (blockIdx.y >= p.y_kv) {
     // ---- queries: a lane keeps its slot's angles and takes the heads in turn
+    constexpr int kHeads = sizeof(T) == 4 ? 2 : kAppendHeads;
     const int groups = max(1, kAppendThreads / work);   // lanes that share a slot
     const int q_parts = gridDim.y - p.y_kv, q_part = blockIdx.y - p.y_kv;
     const int stride = groups * q_parts;
@@ -278,18 +304,20 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_
       if (turn) load_angles<VE>(p, s, pos, c, n);
       const T* in = static_cast<const T*>(p.qin) + (row + t) * p.qin_st[0];
       T* out = static_cast<T*>(p.qout) + (row + t) * p.qout_st[0];
-      for (int h0 = at / work * q_parts + q_part; h0 < p.Hq; h0 += kAppendHeads * stride) {
-        float x[kAppendHeads][2 * VE];
+      for (int h0 = at / work * q_parts + q_part; h0 < p.Hq; h0 += kHeads * stride) {
+        RawSlot<T, VE> raw[kHeads];   // as they lie: half the registers of 16-bit rows
 #pragma unroll
-        for (int j = 0; j < kAppendHeads; ++j)
-          if (h0 + j * stride < p.Hq) load_pair<T, VE>(in + (h0 + j * stride) * p.qin_st[1], s, x[j]);
+        for (int j = 0; j < kHeads; ++j)
+          if (h0 + j * stride < p.Hq) raw[j].load(in + (h0 + j * stride) * p.qin_st[1], s);
 #pragma unroll
-        for (int j = 0; j < kAppendHeads; ++j)
+        for (int j = 0; j < kHeads; ++j)
           if (h0 + j * stride < p.Hq) {
-            if (turn) turn_slot<VE>(p, c, n, x[j]);
+            float x[2 * VE];
+            raw[j].widen(x);
+            if (turn) turn_slot<VE>(p, c, n, x);
             T* o = out + (h0 + j * stride) * p.qout_st[1];
-            store_vec<T, VE>(o + s.e0, x[j]);
-            if (s.two) store_vec<T, VE>(o + s.e1, x[j] + VE);
+            store_vec<T, VE>(o + s.e0, x);
+            if (s.two) store_vec<T, VE>(o + s.e1, x + VE);
           }
       }
     }
