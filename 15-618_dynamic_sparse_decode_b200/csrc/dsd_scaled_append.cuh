@@ -224,6 +224,32 @@ __device__ __forceinline__ void load_slot(const AppendParams& p, const T* row, c
   turn_slot<VE>(p, c, n, x);
 }
 
+// Older codes of a block under its new scale.
+template <bool I8, int VE>
+__device__ __noinline__ void requantise(const AppendParams& p, uint8_t* codes, long long token_stride, int held, int rank,
+                                        int width, float ratio) {
+  const int vecs = p.D / VE;
+  for (int at = rank; at < held * vecs; at += width) {
+    uint8_t* c = codes + at / vecs * token_stride + at % vecs * VE;
+    float x[VE];
+    if constexpr (VE == 1) {
+      x[0] = code_value<I8>(*c);
+    } else {
+      const uint2 raw = *reinterpret_cast<const uint2*>(c);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) x[j] = code_value<I8>(reinterpret_cast<const uint8_t*>(&raw)[j]);
+    }
+    store_codes<I8, VE>(c, x, ratio);
+  }
+}
+
+// Largest magnitude, NaN aside; may be infinite.
+template <int VE>
+__device__ __forceinline__ float largest(const float (&x)[2 * VE], float m) {
+#pragma unroll
+  for (int i = 0; i < 2 * VE; ++i) m = fmaxf(m, fabsf(x[i]));
+  return m;
+}
 template <int VE>
 __device__ __forceinline__ float finite_max(const float (&x)[2 * VE], float m) {
 #pragma unroll
@@ -234,9 +260,13 @@ __device__ __forceinline__ float finite_max(const float (&x)[2 * VE], float m) {
   return m;
 }
 
-template <typename T, bool I8, int VE>
-__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ float team_max[2][kAppendThreads / 32];
+// J > 0: a team's lanes hold the block whole, J slots each, and take a head's keys and
+// values in one round: all loads in flight, one barrier for both maxima, the slots'
+// places and (J <= 2, 16-bit rows) angles kept from head to head.  J = 0: any block,
+// its rows read again for the rounding.
+template <typename T, bool I8, int VE, int J>
+__global__ void __launch_bounds__(kAppendThreads, J ? 2 : 3) append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ float team_max[2][2][kAppendThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int u = blockIdx.x;
   int b = u, row0 = u, n = 1, i = 0;
@@ -324,6 +354,115 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_
     return;
   }
   int flip = 0;
+  if constexpr (J > 0) {
+    constexpr bool kKeepAngles = J <= 2 && sizeof(T) == 2;
+    constexpr float kQmax = I8 ? 127.0f : 448.0f;
+    bool live[J];
+    int t[J], pos[J];
+    Slot<VE> slot[J];
+    float c[kKeepAngles ? J : 1][VE], n[kKeepAngles ? J : 1][VE];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int at = j * width + rank;
+      t[j] = at < work ? at / p.slots : 0;
+      slot[j] = slot_of<VE>(p, at - t[j] * p.slots);
+      pos[j] = position(t[j]);
+      live[j] = good && at < work;
+      if (live[j] && !in_table(pos[j])) {
+        live[j] = false;
+        if (p.status) atomicOr(p.status, DSD_SCALED_BAD_POSITION);
+      }
+      if constexpr (kKeepAngles)
+        if (live[j] && p.cos && slot[j].turned) load_angles<VE>(p, slot[j], pos[j], c[j], n[j]);
+    }
+    const auto key = [&](int j, const RawSlot<T, VE>& raw, float (&x)[2 * VE]) {
+      raw.widen(x);
+      if (!p.cos || !slot[j].turned) return;
+      if constexpr (kKeepAngles) {
+        turn_slot<VE>(p, c[j], n[j], x);
+      } else {
+        load_angles<VE>(p, slot[j], pos[j], c[0], n[0]);
+        turn_slot<VE>(p, c[0], n[0], x);
+      }
+    };
+    for (int base = blockIdx.y * teams; base < p.Hk; base += p.y_kv * teams) {
+      const int head = base + team;
+      const bool on = head < p.Hk && good;
+      const long long si = (1ll * page * p.Hk + head) * p.nblk + first / p.bt;
+      const float old_k = on && held ? p.ks[si] : 0.0f, old_v = on && held ? p.vs[si] : 0.0f;
+      const T* kin = static_cast<const T*>(p.kin) + row * p.kin_st[0] + head * p.kin_st[1];
+      const T* vin = static_cast<const T*>(p.vin) + row * p.vin_st[0] + head * p.vin_st[1];
+      RawSlot<T, VE> k[J], v[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (on && live[j]) {
+          k[j].load(kin + t[j] * p.kin_st[0], slot[j]);
+          v[j].load(vin + t[j] * p.vin_st[0], slot[j]);
+        }
+      float mk = 0.0f, mv = 0.0f;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (on && live[j]) {
+          float x[2 * VE];
+          key(j, k[j], x);
+          mk = largest<VE>(x, mk);
+          v[j].widen(x);
+          mv = largest<VE>(x, mv);
+        }
+      if (mk == INFINITY || mv == INFINITY) {   // seldom: infinities stay out of the scale
+        mk = mv = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (on && live[j]) {
+            float x[2 * VE];
+            key(j, k[j], x);
+            mk = finite_max<VE>(x, mk);
+            v[j].widen(x);
+            mv = finite_max<VE>(x, mv);
+          }
+      }
+      // non-negative floats order like their bits
+      mk = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mk)));
+      mv = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mv)));
+      if (p.team > 1) {
+        // two arrays in turn: one is read while the next round's is written
+        if (lane == 0) {
+          team_max[flip][0][warp] = mk;
+          team_max[flip][1][warp] = mv;
+        }
+        __syncthreads();
+        for (int j = 0; j < p.team; ++j) {
+          mk = fmaxf(mk, team_max[flip][0][team * p.team + j]);
+          mv = fmaxf(mv, team_max[flip][1][team * p.team + j]);
+        }
+        flip ^= 1;
+      }
+      if (!on) continue;
+      const auto finish = [&](bool is_v, float m, float old) {
+        const float fresh = m < 7.888609052210118e-31f ? 0.0f : m * (1.0f / kQmax);   // 2^-100
+        const float scale = held ? fmaxf(old, fresh) : fresh;
+        const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+        const long long* st = is_v ? p.vst : p.kst;
+        uint8_t* codes = (is_v ? p.v : p.k) + page * st[0] + first * st[1] + head * st[2];
+        if (held && scale > old) requantise<I8, VE>(p, codes, st[1], held, rank, width, old * inv);
+        // every lane of the team has read `old` before the maximum's exchange
+        if (rank == 0) (is_v ? p.vs : p.ks)[si] = scale;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (live[j]) {
+            float x[2 * VE];
+            if (is_v) v[j].widen(x);
+            else key(j, k[j], x);
+            uint8_t* to = codes + (held + t[j]) * st[1];
+            store_codes<I8, VE>(to + slot[j].e0, x, inv);
+            if (slot[j].two) store_codes<I8, VE>(to + slot[j].e1, x + VE, inv);
+          }
+      };
+      finish(false, mk, old_k);
+      finish(true, mv, old_v);
+    }
+    return;
+  }
   for (int base = blockIdx.y * teams; base < items; base += p.y_kv * teams) {
     const int item = base + team;
     const bool is_v = item >= p.Hk;
@@ -369,9 +508,9 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_
     m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(m)));
     if (p.team > 1) {
       // two arrays in turn: one is read while the next round's is written
-      if (lane == 0) team_max[flip][warp] = m;
+      if (lane == 0) team_max[flip][0][warp] = m;
       __syncthreads();
-      for (int j = 0; j < p.team; ++j) m = fmaxf(m, team_max[flip][team * p.team + j]);
+      for (int j = 0; j < p.team; ++j) m = fmaxf(m, team_max[flip][0][team * p.team + j]);
       flip ^= 1;
     }
     if (!on) continue;
@@ -382,22 +521,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const __grid_
     const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
     const long long* st = is_v ? p.vst : p.kst;
     uint8_t* codes = (is_v ? p.v : p.k) + page * st[0] + first * st[1] + head * st[2];
-    if (held && scale > old) {
-      const float ratio = old * inv;
-      const int vecs = p.D / VE;
-      for (int at = rank; at < held * vecs; at += width) {
-        uint8_t* c = codes + at / vecs * st[1] + at % vecs * VE;
-        float x[VE];
-        if constexpr (VE == 1) {
-          x[0] = code_value<I8>(*c);
-        } else {
-          const uint2 raw = *reinterpret_cast<const uint2*>(c);
-#pragma unroll
-          for (int j = 0; j < VE; ++j) x[j] = code_value<I8>(reinterpret_cast<const uint8_t*>(&raw)[j]);
-        }
-        store_codes<I8, VE>(c, x, ratio);
-      }
-    }
+    if (held && scale > old) requantise<I8, VE>(p, codes, st[1], held, rank, width, old * inv);
     // every lane of the team has read `old` before the maximum's exchange
     if (rank == 0) scales[si] = scale;
     const auto put = [&](int at, const float (&x)[2 * VE]) {

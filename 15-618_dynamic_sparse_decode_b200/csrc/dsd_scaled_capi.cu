@@ -80,15 +80,19 @@ void CheckType(int dtype) {
 // ------------------------------------------------------------------ append
 
 template <typename T, bool I8>
-void LaunchAppendAs(const AppendParams& p, int ve, dim3 grid, cudaStream_t s) {
-  if (ve == 8) dsds::append_kernel<T, I8, 8><<<grid, dsds::kAppendThreads, 0, s>>>(p);
-  else dsds::append_kernel<T, I8, 1><<<grid, dsds::kAppendThreads, 0, s>>>(p);
+void LaunchAppendAs(const AppendParams& p, int ve, int j, dim3 grid, cudaStream_t s) {
+  using namespace dsds;
+  if (ve == 1) append_kernel<T, I8, 1, 0><<<grid, kAppendThreads, 0, s>>>(p);
+  else if (j == 1) append_kernel<T, I8, 8, 1><<<grid, kAppendThreads, 0, s>>>(p);
+  else if (j == 2) append_kernel<T, I8, 8, 2><<<grid, kAppendThreads, 0, s>>>(p);
+  else if (j == 4) append_kernel<T, I8, 8, 4><<<grid, kAppendThreads, 0, s>>>(p);
+  else append_kernel<T, I8, 8, 0><<<grid, kAppendThreads, 0, s>>>(p);
 }
 
 template <typename T>
-void LaunchAppend(const AppendParams& p, bool i8, int ve, dim3 grid, cudaStream_t s) {
-  if (i8) LaunchAppendAs<T, true>(p, ve, grid, s);
-  else LaunchAppendAs<T, false>(p, ve, grid, s);
+void LaunchAppend(const AppendParams& p, bool i8, int ve, int j, dim3 grid, cudaStream_t s) {
+  if (i8) LaunchAppendAs<T, true>(p, ve, j, grid, s);
+  else LaunchAppendAs<T, false>(p, ve, j, grid, s);
 }
 
 void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args* a, cudaStream_t s) {
@@ -179,10 +183,13 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   p.slots = (p.D + 2 * ve - 1) / (2 * ve);
   const int64_t units = p.off ? int64_t(p.total) / p.bt + 2 * int64_t(p.batch) : p.batch;
   if (units > INT32_MAX) Fail(DSD_EINVAL, "too many tokens for one call");
-  // a team's lanes keep the whole block in registers where 8 warps can
+  // A team of warps holds a head's block whole, one slot a lane where a warp can (a
+  // decode step), else two, four in the largest teams; blocks beyond that are read twice.
   const int block_slots = (p.off ? std::min(p.bt, p.total) : 1) * p.slots;
+  const int largest = dsds::kAppendThreads * 4;
+  const int j = ve == 1 || block_slots > largest ? 0 : block_slots <= 32 ? 1 : block_slots <= largest / 2 ? 2 : 4;
   p.team = 1;
-  while (p.team < 8 && p.team * 32 * dsds::kAppendKeep < block_slots) p.team *= 2;
+  while (p.team < 8 && p.team * 32 * (j ? j : dsds::kAppendKeep) < block_slots) p.team *= 2;
   // blockIdx.y: CTAs of one block of tokens, keys and values first, then queries;
   // as many as fill the GPU eight times over when there are few blocks, and no more
   // than four rounds (of heads) to a CTA when there are many
@@ -191,13 +198,13 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
     const int64_t want = (8ll * dev.sms + units - 1) / units;
     return int(std::min<int64_t>(rounds, std::max<int64_t>(want, (rounds + 3) / 4)));
   };
-  p.y_kv = parts((2 * p.Hk + teams - 1) / teams);
+  p.y_kv = parts(((j ? 1 : 2) * p.Hk + teams - 1) / teams);
   const int y_q = p.Hq ? parts((p.Hq + 4 * dsds::kAppendHeads - 1) / (4 * dsds::kAppendHeads)) : 0;
   const dim3 grid{static_cast<unsigned>(units), static_cast<unsigned>(p.y_kv + y_q), 1};
   const bool i8 = c->kv_format == DSD_KV_I8_SCALED;
-  if (a->dtype == DSD_TYPE_F32) LaunchAppend<float>(p, i8, ve, grid, s);
-  else if (a->dtype == DSD_TYPE_BF16) LaunchAppend<__nv_bfloat16>(p, i8, ve, grid, s);
-  else LaunchAppend<__half>(p, i8, ve, grid, s);
+  if (a->dtype == DSD_TYPE_F32) LaunchAppend<float>(p, i8, ve, j, grid, s);
+  else if (a->dtype == DSD_TYPE_BF16) LaunchAppend<__nv_bfloat16>(p, i8, ve, j, grid, s);
+  else LaunchAppend<__half>(p, i8, ve, j, grid, s);
   Check(cudaGetLastError(), "append launch");
 }
 
