@@ -269,6 +269,8 @@ __global__ void __launch_bounds__(kAppendThreads, J ? 2 : 3) append_kernel(const
   __shared__ float team_max[2][2][kAppendThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int u = blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
   int b = u, row0 = u, n = 1, i = 0;
   if (p.off) {
     // the last request whose first unit is not behind u

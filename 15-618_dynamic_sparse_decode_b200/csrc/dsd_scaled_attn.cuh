@@ -37,6 +37,8 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
   const int cta = blockIdx.x;
 
   const int head = cta % p.Hk;
+  pdl_wait();
+  pdl_trigger();
   plan_walk<kSimpleThreads>(p, cta / p.Hk, wb, &walk_s);
   Walk w = walk_s;
   if (tid == 0) p.meta[cta] = make_int4(0, 0, -1, 0);

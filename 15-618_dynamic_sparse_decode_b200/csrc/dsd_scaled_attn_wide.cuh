@@ -236,8 +236,14 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
     mbar_init(&drained, 1);
     stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    p.meta[cta] = make_int4(0, 0, -1, 0);
   }
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (tid == 0) p.meta[cta] = make_int4(0, 0, -1, 0);
   plan_walk<kWideThreads>(p, cta / p.Hk, reinterpret_cast<int*>(k_ring), &walk_s);
   Walk w = walk_s;
   if (w.left == 0) return;

@@ -77,16 +77,34 @@ void CheckType(int dtype) {
     Fail(DSD_EINVAL, "dtype must be DSD_TYPE_F32, DSD_TYPE_BF16 or DSD_TYPE_F16");
 }
 
+// Launches a kernel that may be placed before its predecessor in the stream has
+// ended (it waits on the device before it touches memory): the launch's latency
+// disappears behind the predecessor's last blocks.
+template <typename... P, typename... A>
+void Launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  Check(cudaLaunchKernelEx(&cfg, kernel, args...), "kernel launch");
+}
+
 // ------------------------------------------------------------------ append
 
 template <typename T, bool I8>
 void LaunchAppendAs(const AppendParams& p, int ve, int j, dim3 grid, cudaStream_t s) {
   using namespace dsds;
-  if (ve == 1) append_kernel<T, I8, 1, 0><<<grid, kAppendThreads, 0, s>>>(p);
-  else if (j == 1) append_kernel<T, I8, 8, 1><<<grid, kAppendThreads, 0, s>>>(p);
-  else if (j == 2) append_kernel<T, I8, 8, 2><<<grid, kAppendThreads, 0, s>>>(p);
-  else if (j == 4) append_kernel<T, I8, 8, 4><<<grid, kAppendThreads, 0, s>>>(p);
-  else append_kernel<T, I8, 8, 0><<<grid, kAppendThreads, 0, s>>>(p);
+  if (ve == 1) Launch(append_kernel<T, I8, 1, 0>, grid, kAppendThreads, 0, s, p);
+  else if (j == 1) Launch(append_kernel<T, I8, 8, 1>, grid, kAppendThreads, 0, s, p);
+  else if (j == 2) Launch(append_kernel<T, I8, 8, 2>, grid, kAppendThreads, 0, s, p);
+  else if (j == 4) Launch(append_kernel<T, I8, 8, 4>, grid, kAppendThreads, 0, s, p);
+  else Launch(append_kernel<T, I8, 8, 0>, grid, kAppendThreads, 0, s, p);
 }
 
 template <typename T>
@@ -205,7 +223,6 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   if (a->dtype == DSD_TYPE_F32) LaunchAppend<float>(p, i8, ve, j, grid, s);
   else if (a->dtype == DSD_TYPE_BF16) LaunchAppend<__nv_bfloat16>(p, i8, ve, j, grid, s);
   else LaunchAppend<__half>(p, i8, ve, j, grid, s);
-  Check(cudaGetLastError(), "append launch");
 }
 
 // --------------------------------------------------------------- attention
@@ -270,10 +287,10 @@ template <bool I8>
 void LaunchSimple(const AttnParams& p, cudaStream_t s) {
   const size_t smem = dsds::simple_smem(p.R, p.D, p.batch);
   switch (p.R) {
-    case 1: dsds::attn_simple_kernel<I8, 1><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
-    case 2: dsds::attn_simple_kernel<I8, 2><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
-    case 4: dsds::attn_simple_kernel<I8, 4><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
-    default: dsds::attn_simple_kernel<I8, 8><<<p.ncta, dsds::kSimpleThreads, smem, s>>>(p); break;
+    case 1: Launch(dsds::attn_simple_kernel<I8, 1>, dim3(p.ncta), dsds::kSimpleThreads, smem, s, p); break;
+    case 2: Launch(dsds::attn_simple_kernel<I8, 2>, dim3(p.ncta), dsds::kSimpleThreads, smem, s, p); break;
+    case 4: Launch(dsds::attn_simple_kernel<I8, 4>, dim3(p.ncta), dsds::kSimpleThreads, smem, s, p); break;
+    default: Launch(dsds::attn_simple_kernel<I8, 8>, dim3(p.ncta), dsds::kSimpleThreads, smem, s, p); break;
   }
 }
 
@@ -477,8 +494,8 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
     const CUtensorMap k_map = MapOf(c, c->k_codes, pl.maps.k), v_map = MapOf(c, c->v_codes, pl.maps.v);
     const bool fp32 = a->dtype == DSD_TYPE_F32;
     const auto launch = [&](auto kernel, auto tag) {
-      kernel<<<p.ncta, pl.wide ? dsds::kWideThreads : dsds::kTcThreads, decltype(tag)::type::kSmem, s>>>(
-          p, k_map, v_map, pl.maps.k.head_first);
+      Launch(kernel, dim3(p.ncta), pl.wide ? dsds::kWideThreads : dsds::kTcThreads, decltype(tag)::type::kSmem, s, p,
+             k_map, v_map, int(pl.maps.k.head_first));
     };
     if (pl.wide) WithWide(i8, a->dtype, launch);
     else WithTc(i8, fp32, p.R, launch);
@@ -487,20 +504,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   } else {
     LaunchSimple<false>(p, s);
   }
-  Check(cudaGetLastError(), "attention launch");
-
-  // the join may be scheduled while the last CTAs of the attention run; it waits
-  // for them before it reads
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(p.ncta), unsigned(std::min(p.R, 32)));
-  cfg.blockDim = dim3(unsigned(p.D <= 128 ? 128 : 256));
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  Check(cudaLaunchKernelEx(&cfg, dsds::combine_kernel, p), "combine launch");
+  Launch(dsds::combine_kernel, dim3(unsigned(p.ncta), unsigned(std::min(p.R, 32))), p.D <= 128 ? 128 : 256, 0, s, p);
 }
 
 }  // namespace

@@ -50,6 +50,12 @@ __device__ __forceinline__ int operator/(int n, const Divisor& v) {
 }
 __device__ __forceinline__ int operator%(int n, const Divisor& v) { return n - n / v * v.d; }
 
+// Every kernel here is launched before its predecessor in the stream has ended: it
+// touches memory after pdl_wait(), which waits for that end.  pdl_trigger() lets the
+// successor's blocks be placed once all blocks of this grid have started.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 struct AttnParams {
   const uint8_t* k;
   const uint8_t* v;
@@ -385,7 +391,8 @@ __device__ __forceinline__ void write_row_lse(const AttnParams& p, const Request
 // the rest, added in that order, so the result does not depend on timing.
 // head_dim <= 256 threads.
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  pdl_wait();
+  pdl_trigger();
   const int c = blockIdx.x, d = threadIdx.x;
   const int4 u = p.meta[c];
   if (u.z < 0) return;
