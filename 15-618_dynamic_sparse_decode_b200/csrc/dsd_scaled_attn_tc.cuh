@@ -231,7 +231,7 @@ struct UnitInfo {
   int rows;           // query rows from the unit's first on (wide: the request's)
   int q0, base_pos;   // wide: first query row, place of the first query
   int opens, ends;    // the segment has the unit's first / last slot
-  int last_gang;
+  int last_slot;      // of the unit, on the axis
 };
 
 // Token data of a tile, from warp 6.  A scale covers a block of bt tokens, so a
@@ -393,35 +393,6 @@ __device__ __forceinline__ void walk_tokens(const AttnParams& p, Walk w, int hea
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Row `row` of a unit's queries, a lane four elements, as pieces in the operand;
-// returns the row's factor.
-template <bool I8, int R, int PIECES>
-__device__ __noinline__ float cut_row(float4 x, int row, uint8_t* op, float scale_log2) {
-  const int lane = threadIdx.x & 31;
-  uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
-                     max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
-  top = __reduce_max_sync(~0u, top);
-  // the row's power of two: 2^e <= largest < 2^(e+1)
-  const int e = max(static_cast<int>(top >> 23) - 127, -100);
-  uint16_t lo[PIECES], hi[PIECES];
-  const float f = __uint_as_float(uint32_t((I8 ? 7 * PIECES - 2 : 7) - e + 127) << 23);
-  if constexpr (I8) {
-    cut_int<PIECES>(__float2int_rn(x.x * f), __float2int_rn(x.y * f), lo);
-    cut_int<PIECES>(__float2int_rn(x.z * f), __float2int_rn(x.w * f), hi);
-  } else {
-    cut_e4m3<PIECES>(x.x * f, x.y * f, lo);
-    cut_e4m3<PIECES>(x.z * f, x.w * f, hi);
-  }
-#pragma unroll
-  for (int j = 0; j < PIECES; ++j) {
-    const int n = j * R + row;
-    *reinterpret_cast<uint32_t*>(op + n * 128 + (4 * lane ^ (n & 7) << 4)) = uint32_t(lo[j]) | uint32_t(hi[j]) << 16;
-  }
-  // the first piece's unit: e4m3 2^(e - 7), int8 2^(e - 5); a row that is not finite is NaN
-  const float unit = __uint_as_float(uint32_t(e - (I8 ? 5 : 7) + 127) << 23);
-  return top >= 0x7f800000u ? NAN : scale_log2 * unit;
-}
-
 // Four elements of a row as they lie; aligned: one access.
 __device__ __forceinline__ uint4 load_four(const uint8_t* at, int elem, bool aligned) {
   uint4 y{0, 0, 0, 0};
@@ -449,6 +420,52 @@ __device__ __forceinline__ float4 widen_four(uint4 y, int dtype) {
                        __uint_as_float(y.y & 0xffff0000u));
   const float2 a = __half22float2(*reinterpret_cast<__half2*>(&y.x)), b = __half22float2(*reinterpret_cast<__half2*>(&y.y));
   return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// A unit's queries in pieces.  A row is shared by as many lanes as four rows leave
+// each (eight, of 16 elements), so that a group's rows are cut side by side.
+template <int R>
+struct QueryLanes {
+  static constexpr int kRows = R < 4 ? R : 4;          // rows at a time
+  static constexpr int kLanes = 32 / kRows;            // lanes of a row
+  static constexpr int kQuads = 32 / kLanes;           // runs of four elements a lane
+};
+
+template <bool I8, int R, int PIECES>
+__device__ __forceinline__ void cut_rows(const float4 (&x)[QueryLanes<R>::kQuads], int row, uint8_t* op, float scale_log2,
+                                         float* factor) {
+  constexpr int kLanes = QueryLanes<R>::kLanes, kQuads = QueryLanes<R>::kQuads;
+  const int part = threadIdx.x & (kLanes - 1);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i)
+    top = max(top, max(max(__float_as_uint(fabsf(x[i].x)), __float_as_uint(fabsf(x[i].y))),
+                       max(__float_as_uint(fabsf(x[i].z)), __float_as_uint(fabsf(x[i].w)))));
+#pragma unroll
+  for (int o = kLanes / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+  // the row's power of two: 2^e <= largest < 2^(e+1)
+  const int e = max(static_cast<int>(top >> 23) - 127, -100);
+  const float f = __uint_as_float(uint32_t((I8 ? 7 * PIECES - 2 : 7) - e + 127) << 23);
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i) {
+    uint16_t lo[PIECES], hi[PIECES];
+    if constexpr (I8) {
+      cut_int<PIECES>(__float2int_rn(x[i].x * f), __float2int_rn(x[i].y * f), lo);
+      cut_int<PIECES>(__float2int_rn(x[i].z * f), __float2int_rn(x[i].w * f), hi);
+    } else {
+      cut_e4m3<PIECES>(x[i].x * f, x[i].y * f, lo);
+      cut_e4m3<PIECES>(x[i].z * f, x[i].w * f, hi);
+    }
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int n = j * R + row;
+      *reinterpret_cast<uint32_t*>(op + n * 128 + (4 * (part * kQuads + i) ^ (n & 7) << 4)) =
+          uint32_t(lo[j]) | uint32_t(hi[j]) << 16;
+    }
+  }
+  // the first piece's unit: e4m3 2^(e - 7), int8 2^(e - 5); a row that is not finite is NaN
+  const float unit = __uint_as_float(uint32_t(e - (I8 ? 5 : 7) + 127) << 23);
+  if (part == 0) *factor = top >= 0x7f800000u ? NAN : scale_log2 * unit;
 }
 
 template <bool I8, int R, int PIECES>
@@ -618,46 +635,54 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
   } else if (warp == 6) {
     walk_tokens(p, w, head, TokenRing(token_smem, p), info, token_full, token_empty, &stop);
   } else if (warp == 7) {
-    // ---- queries, cut into pieces; a lane takes four elements of every row
+    // ---- queries, cut into pieces
+    using Lanes = QueryLanes<R>;
+    constexpr int kGroups = R / Lanes::kRows, kQuads = Lanes::kQuads;
     const int elem = p.dtype == DSD_TYPE_F32 ? 4 : 2;
     const bool aligned = reinterpret_cast<uintptr_t>(p.q) % (4 * elem) == 0 && p.qst[0] % 4 == 0 && p.qst[1] % 4 == 0;
+    const int my_row = lane / Lanes::kLanes, my_elem = lane % Lanes::kLanes * 4 * kQuads;
     bool ok = true;
 #pragma unroll 1
     for (uint32_t unit = 0; ok; ++unit) {
       const int u = unit & 1;
       const bool end = w.left <= 0;
       const Request r = w.r;
+      const int row0 = w.qt * R;
+      uint4 raw[kGroups][kQuads];
+      if (!end) {
+        // every address is a valid one: the loads are in flight together
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+          const int gr = min(row0 + i * Lanes::kRows + my_row, r.rows - 1);
+          const long long at = 1ll * (r.q0 + gr / p.by_group) * p.qst[0] + 1ll * (head * p.G + gr % p.by_group) * p.qst[1];
+#pragma unroll
+          for (int j = 0; j < kQuads; ++j)
+            raw[i][j] = load_four(static_cast<const uint8_t*>(p.q) + (at + (my_elem + 4 * j < p.D ? my_elem + 4 * j : 0)) * elem,
+                                  elem, aligned);
+        }
+      }
       Span span{0, 0};
       if (!end) span = span_of(p, r, w.qt);
       const int slots = slots_of(span);
       const Segment seg = segment_of(w, slots);
-      const int row0 = w.qt * R, base_pos = r.len - r.nq;
-      // lane = row: where it lies and what it sees
-      const int gr = min(row0 + lane, r.rows - 1);
-      const int qi = gr / p.by_group, q_head = head * p.G + gr % p.by_group;
-      const long long at = 1ll * (r.q0 + qi) * p.qst[0] + 1ll * q_head * p.qst[1];
-      const bool in_row = 4 * lane < p.D;   // head_dim is a multiple of 16 here
-      uint4 raw[R];
-      if (!end) {
-        // every address is a valid one: the loads are in flight together
-#pragma unroll
-        for (int row = 0; row < R; ++row)
-          raw[row] = load_four(static_cast<const uint8_t*>(p.q) + (__shfl_sync(~0u, at, row) + (in_row ? 4 * lane : 0)) * elem,
-                               elem, aligned);
-      }
       ok = mbar_wait(&unit_empty[u], (unit >> 1 & 1) ^ 1, &stop, p.status);
       ok = __all_sync(~0u, ok);
       if (!ok) break;
       if (!end) {
 #pragma unroll
-        for (int row = 0; row < R; ++row) {
-          float4 x = widen_four(raw[row], p.dtype);
-          if (!in_row || row0 + row >= r.rows) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          const float factor = cut_row<I8, R, PIECES>(x, row, q_op + u * Shape::kOperand, p.scale_log2);
-          if (lane == 0) row_factor[u][row] = factor;
+        for (int i = 0; i < kGroups; ++i) {
+          const int row = i * Lanes::kRows + my_row;
+          float4 x[kQuads];
+#pragma unroll
+          for (int j = 0; j < kQuads; ++j) {
+            x[j] = widen_four(raw[i][j], p.dtype);
+            if (my_elem + 4 * j >= p.D || row0 + row >= r.rows) x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+          cut_rows<I8, R, PIECES>(x, row, q_op + u * Shape::kOperand, p.scale_log2, &row_factor[u][row]);
         }
         if (lane < R) {
-          row_pos[u][lane] = base_pos + qi;
+          const int gr = min(row0 + lane, r.rows - 1), qi = gr / p.by_group, q_head = head * p.G + gr % p.by_group;
+          row_pos[u][lane] = r.len - r.nq + qi;
           row_out[u][lane] = 1ll * (r.q0 + qi) * p.ost[0] + 1ll * q_head * p.ost[1];
           row_lse[u][lane] = (r.q0 + qi) * p.H + q_head;
         }
@@ -670,7 +695,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
         x.rows = r.rows - row0;
         x.opens = seg.opens;
         x.ends = seg.ends;
-        x.last_gang = end ? 0 : gang_of(p, w.at - w.slot + slots - 1, w.total);
+        x.last_slot = w.at - w.slot + slots - 1;
       }
       proxy_fence();
       __syncwarp();
@@ -869,7 +894,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
           }
         }
       }
-      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.qt, x.last_gang, 0);
+      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.qt, gang_of(p, x.last_slot, w.total), 0);
       // `red` is written again behind the barrier at the next unit's start
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[u]);

@@ -286,7 +286,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         x.base_pos = r.len - r.nq;
         x.opens = seg.opens;
         x.ends = seg.ends;
-        x.last_gang = end ? 0 : gang_of(p, w.at - w.slot + slots - 1, w.total);
+        x.last_slot = w.at - w.slot + slots - 1;
         mbar_arrive(&unit_full[u]);
       }
       __syncwarp();
@@ -732,7 +732,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
           p.lse[1ll * (x.q0 + qi) * p.H + q_head] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * kLn2;
         }
       }
-      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.qt, x.last_gang, 0);
+      if (x.opens && !x.ends && tid == 0) p.meta[cta] = make_int4(x.b, x.qt, gang_of(p, x.last_slot, w.total), 0);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[u]);
