@@ -463,84 +463,84 @@ __global__ void __launch_bounds__(kAppendThreads, J ? 2 : 3) append_kernel(const
       finish(false, mk, old_k);
       finish(true, mv, old_v);
     }
-    return;
-  }
-  for (int base = blockIdx.y * teams; base < items; base += p.y_kv * teams) {
-    const int item = base + team;
-    const bool is_v = item >= p.Hk;
-    const int head = is_v ? item - p.Hk : item;
-    const bool turn = p.cos && !is_v;
-    const bool on = item < items && good;
-    const long long* in_st = is_v ? p.vin_st : p.kin_st;
-    const T* in = static_cast<const T*>(is_v ? p.vin : p.kin) + row * in_st[0] + head * in_st[1];
-    const long long si = (1ll * page * p.Hk + head) * p.nblk + first / p.bt;
-    float* scales = is_v ? p.vs : p.ks;
-    const float old = on && held ? scales[si] : 0.0f;
+  } else {
+    for (int base = blockIdx.y * teams; base < items; base += p.y_kv * teams) {
+      const int item = base + team;
+      const bool is_v = item >= p.Hk;
+      const int head = is_v ? item - p.Hk : item;
+      const bool turn = p.cos && !is_v;
+      const bool on = item < items && good;
+      const long long* in_st = is_v ? p.vin_st : p.kin_st;
+      const T* in = static_cast<const T*>(is_v ? p.vin : p.kin) + row * in_st[0] + head * in_st[1];
+      const long long si = (1ll * page * p.Hk + head) * p.nblk + first / p.bt;
+      float* scales = is_v ? p.vs : p.ks;
+      const float old = on && held ? scales[si] : 0.0f;
 
-    float keep[kAppendKeep][2 * VE];
-    bool live[kAppendKeep];
-    float m = 0.0f;
+      float keep[kAppendKeep][2 * VE];
+      bool live[kAppendKeep];
+      float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kAppendKeep; ++j) {
-      const int at = j * width + rank;
-      live[j] = on && at < work;
-      if (live[j]) {
-        const int t = at / p.slots, pos = position(t);
-        live[j] = in_table(pos);
+      for (int j = 0; j < kAppendKeep; ++j) {
+        const int at = j * width + rank;
+        live[j] = on && at < work;
         if (live[j]) {
-          load_slot<T, VE>(p, in + t * in_st[0], slot_of<VE>(p, at % p.slots), pos, turn, keep[j]);
-          m = finite_max<VE>(keep[j], m);
-        } else if (p.status) {
-          atomicOr(p.status, DSD_SCALED_BAD_POSITION);
+          const int t = at / p.slots, pos = position(t);
+          live[j] = in_table(pos);
+          if (live[j]) {
+            load_slot<T, VE>(p, in + t * in_st[0], slot_of<VE>(p, at % p.slots), pos, turn, keep[j]);
+            m = finite_max<VE>(keep[j], m);
+          } else if (p.status) {
+            atomicOr(p.status, DSD_SCALED_BAD_POSITION);
+          }
         }
       }
-    }
-    if (on)
+      if (on)
+        for (int at = kAppendKeep * width + rank; at < work; at += width) {
+          const int t = at / p.slots, pos = position(t);
+          if (!in_table(pos)) {
+            if (p.status) atomicOr(p.status, DSD_SCALED_BAD_POSITION);
+            continue;
+          }
+          float x[2 * VE];
+          load_slot<T, VE>(p, in + t * in_st[0], slot_of<VE>(p, at % p.slots), pos, turn, x);
+          m = finite_max<VE>(x, m);
+        }
+      // non-negative floats order like their bits
+      m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(m)));
+      if (p.team > 1) {
+        // two arrays in turn: one is read while the next round's is written
+        if (lane == 0) team_max[flip][0][warp] = m;
+        __syncthreads();
+        for (int j = 0; j < p.team; ++j) m = fmaxf(m, team_max[flip][0][team * p.team + j]);
+        flip ^= 1;
+      }
+      if (!on) continue;
+
+      constexpr float kQmax = I8 ? 127.0f : 448.0f;
+      const float fresh = m < 7.888609052210118e-31f ? 0.0f : m * (1.0f / kQmax);   // 2^-100
+      const float scale = held ? fmaxf(old, fresh) : fresh;
+      const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+      const long long* st = is_v ? p.vst : p.kst;
+      uint8_t* codes = (is_v ? p.v : p.k) + page * st[0] + first * st[1] + head * st[2];
+      if (held && scale > old) requantise<I8, VE>(p, codes, st[1], held, rank, width, old * inv);
+      // every lane of the team has read `old` before the maximum's exchange
+      if (rank == 0) scales[si] = scale;
+      const auto put = [&](int at, const float (&x)[2 * VE]) {
+        const Slot<VE> s = slot_of<VE>(p, at % p.slots);
+        uint8_t* c = codes + (held + at / p.slots) * st[1];
+        store_codes<I8, VE>(c + s.e0, x, inv);
+        if (s.two) store_codes<I8, VE>(c + s.e1, x + VE, inv);
+      };
+#pragma unroll
+      for (int j = 0; j < kAppendKeep; ++j)
+        if (live[j]) put(j * width + rank, keep[j]);
       for (int at = kAppendKeep * width + rank; at < work; at += width) {
         const int t = at / p.slots, pos = position(t);
-        if (!in_table(pos)) {
-          if (p.status) atomicOr(p.status, DSD_SCALED_BAD_POSITION);
-          continue;
-        }
+        if (!in_table(pos)) continue;
         float x[2 * VE];
         load_slot<T, VE>(p, in + t * in_st[0], slot_of<VE>(p, at % p.slots), pos, turn, x);
-        m = finite_max<VE>(x, m);
+        put(at, x);
       }
-    // non-negative floats order like their bits
-    m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(m)));
-    if (p.team > 1) {
-      // two arrays in turn: one is read while the next round's is written
-      if (lane == 0) team_max[flip][0][warp] = m;
-      __syncthreads();
-      for (int j = 0; j < p.team; ++j) m = fmaxf(m, team_max[flip][0][team * p.team + j]);
-      flip ^= 1;
-    }
-    if (!on) continue;
-
-    constexpr float kQmax = I8 ? 127.0f : 448.0f;
-    const float fresh = m < 7.888609052210118e-31f ? 0.0f : m * (1.0f / kQmax);   // 2^-100
-    const float scale = held ? fmaxf(old, fresh) : fresh;
-    const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-    const long long* st = is_v ? p.vst : p.kst;
-    uint8_t* codes = (is_v ? p.v : p.k) + page * st[0] + first * st[1] + head * st[2];
-    if (held && scale > old) requantise<I8, VE>(p, codes, st[1], held, rank, width, old * inv);
-    // every lane of the team has read `old` before the maximum's exchange
-    if (rank == 0) scales[si] = scale;
-    const auto put = [&](int at, const float (&x)[2 * VE]) {
-      const Slot<VE> s = slot_of<VE>(p, at % p.slots);
-      uint8_t* c = codes + (held + at / p.slots) * st[1];
-      store_codes<I8, VE>(c + s.e0, x, inv);
-      if (s.two) store_codes<I8, VE>(c + s.e1, x + VE, inv);
-    };
-#pragma unroll
-    for (int j = 0; j < kAppendKeep; ++j)
-      if (live[j]) put(j * width + rank, keep[j]);
-    for (int at = kAppendKeep * width + rank; at < work; at += width) {
-      const int t = at / p.slots, pos = position(t);
-      if (!in_table(pos)) continue;
-      float x[2 * VE];
-      load_slot<T, VE>(p, in + t * in_st[0], slot_of<VE>(p, at % p.slots), pos, turn, x);
-      put(at, x);
     }
   }
 }

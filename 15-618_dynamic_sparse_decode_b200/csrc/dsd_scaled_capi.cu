@@ -392,6 +392,7 @@ AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_s
     WithTc(i8, fp32, pl.R, [&](auto, auto tag) { per_sm = decltype(tag)::type::kCtas; });
   pl.gangs = std::max(1, per_sm * dev.sms / c->num_kv_heads);
   pl.ncta = pl.gangs * c->num_kv_heads;
+  if (pl.gangs > dsds::kMaxPieces) Fail(DSD_EUNAVAILABLE, "more SMs than the join is laid out for");
   pl.ml_at = (int64_t(pl.ncta) * 16 + 255) / 256 * 256;
   pl.o_at = pl.ml_at + (int64_t(pl.ncta) * 2 * pl.R * 8 + 255) / 256 * 256;
   pl.bytes = pl.o_at + int64_t(pl.ncta) * 2 * pl.R * c->head_dim * 4;
