@@ -9,8 +9,12 @@
 // begin at offsets[b] / block_tokens + 2 b, which leaves room for the partly filled
 // blocks at both ends, and a warp-wide search finds b again.
 //
-// Bound: HBM bytes (read both rows once, write a byte an element); every value
-// stays in registers between the maximum and the rounding.
+// Bound: HBM bytes (read both rows once, write a byte an element); a row stays in
+// registers, as it lies, between the maximum and the rounding.  56000 tokens of
+// fp16, 32 + 2 x 8 heads of 128, half of each rotated, e4m3 in blocks of 64: 0.27 ms,
+// 5.0 TB/s of the measured 6.56 (queries alone 5.7, keys and values alone 3.5, where
+// the rounding's instructions still show).  With keys, values and queries as rounds
+// of one loop it took 0.61 ms.
 #pragma once
 
 #include <type_traits>

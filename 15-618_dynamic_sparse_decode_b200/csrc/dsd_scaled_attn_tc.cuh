@@ -16,6 +16,13 @@
 // The pieces cost columns of a product that a decode step leaves idle anyway:
 // with 8 query rows per key head, S and O have 24 of their up to 256 columns.
 //
+// Bound: HBM.  64 requests of 16-32k tokens, 32 heads over 8, token-major pages of
+// 32: 0.505 ms, 6.4 TB/s (0.98 of the measured copy rate; head-major 6.58 TB/s);
+// about 20 us of every call are its start, the tail of its ranges and the join, so
+// smaller calls reach less.  Two CTAs per SM with three stages each; three CTAs with
+// two stages measured the same for 1 or 2 rows and a fifth slower for 4 (80
+// registers).
+//
 // Roles: warps 0-3 softmax (thread = token for S^T, = element d for O^T), warp 4
 // TMA, warp 5 MMA issue, warp 6 token data (page, scales, masks of a tile), warp 7
 // the next unit's queries.  Warps 4, 6 and 7 walk the CTA's range ahead of the
@@ -238,7 +245,7 @@ struct UnitInfo {
 // tile has at most 128 / bt + 1 entries: the two scales and how many of the
 // block's tokens are there.  As many tiles ahead as the ring has room for: the
 // scales come from far apart in memory, and one tile ahead left the softmax
-// waiting for them (64 requests x 16-32k: 1.01 ms, with eight ahead see DESIGN).
+// waiting for them (64 requests x 16-32k: 1.01 ms, with eight ahead 0.62 ms).
 struct TokenRing {
   float2* scales;    // [stages][entries]
   int* limit;        // [stages][entries]
@@ -378,7 +385,7 @@ __device__ __forceinline__ void walk_tokens(const AttnParams& p, Walk w, int hea
         ring.limit[s * ring.entries + e] = limit;
       }
       if (lane == 0) {
-        const int place = p.tpp ? first * p.P + off : tile * p.ppt * p.P;
+        const int place = p.counts ? 0 : p.tpp ? first * p.P + off : tile * p.ppt * p.P;
         info[s] = {place, lead, p.counts || (place >= all_from && place <= all_to - (kTile - 1))};
       }
       mbar_arrive_after_copies(&token_full[s]);

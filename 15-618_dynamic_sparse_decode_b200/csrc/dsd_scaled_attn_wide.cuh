@@ -8,20 +8,25 @@
 // in fp16, so four warps write each K and V tile as fp16 operands and one product
 // does what the narrow kernel needs three 8-bit pieces for.  Queries are scaled by
 // a power of two of their row into fp16's range (exact for fp16 and for bf16 within
-// 2^-29 of the row's largest).  Weights go back to TMEM as fp16 (2^-12 of their
-// value) and are the A operand of the second product there.  A weight carries its
-// value scale: P = 2^(s - r) vs with the row's reference r taken from the largest
-// logit and the largest value scale, so that O / sum is the output as it stands and a
-// column has two constants, its scales (with the exponent of vs in the logits, as in
-// the narrow kernel, it had four, and their loads were a quarter of the pass).  A
-// token's weight keeps its bits down to 2^-20 of that largest product.
+// 2^-29 of the row's largest).
 //
-// A thread owns half a row of S: the running sum is its own, the reference that the
-// weights are taken from is the row's.  It stays while no maximum has grown past it
-// by more than 2^8, which fp16 weights bear, so that a tile is one pass over its
-// logits; when one has, the eight warps vote, O is rescaled in TMEM and the weights
-// are made again (with a pass for the maximum every tile: 544 us against the chunk
-// case's present figure in the design notes).
+// A weight carries its value scale: P = 2^(s - r) vs, fp16, back in TMEM as the A
+// operand of the second product.  The row's reference r comes from its largest
+// logit and the tile's largest value scale, so that O / sum is the output as it
+// stands and a column has two constants, its scales (with the exponent of vs in the
+// logits, as in the narrow kernel, it had four: chunks 522 us, with two 489 us).  A
+// weight keeps its bits down to 2^-20 of the row's largest.
+//
+// The reference stays while nothing has grown past it by more than 2^8, which fp16
+// weights bear, so a tile is one pass over its logits; else the eight warps vote, O
+// is rescaled in TMEM and the weights are made again (a pass for the maximum every
+// tile: 544 us).  A thread owns half a row of S, 32 columns at a time: 64 values
+// kept in registers left none to load ahead with (759 us), and sixteen warps with a
+// quarter each came out at 766 us.
+//
+// Bound: the softmax warps' latency (the tensor cores are 20% busy, ex2 21%); three
+// requests of 300-700 queries over 5000-9000 tokens, 32 heads over 8: 0.49 ms, 484
+// TFLOP/s of the 1679 a bf16 product reaches.
 //
 // Roles: warps 0-7 softmax, 8-11 widen the codes, 12 TMA, 13 MMA issue, 14 token
 // data, 15 units.

@@ -133,7 +133,8 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   }
   if (a->batch == 0 || a->total_tokens == 0) return;
   CheckCachePointers(c);
-  if (!a->k || !a->v || !a->seq_lens || !a->page_table) Fail(DSD_EINVAL, "null device array");
+  if (!a->k || !a->v || !a->seq_lens || (!a->page_table && a->max_pages_per_request > 0))
+    Fail(DSD_EINVAL, "null device array");
   if (a->num_q_heads && (!a->q || !a->q_out)) Fail(DSD_EINVAL, "num_q_heads > 0 needs q and q_out");
   const int eb = ElemBytes(a->dtype);
   const void* rows[] = {a->k, a->v, a->num_q_heads ? a->q : a->k, a->num_q_heads ? a->q_out : a->k};
@@ -423,7 +424,8 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   CheckAttention(c, a);
   if (a->batch == 0 || a->total_queries == 0) return;
   CheckCachePointers(c);
-  if (!a->q || !a->out || !a->lens || !a->page_table) Fail(DSD_EINVAL, "null device array");
+  if (!a->q || !a->out || !a->lens || (!a->page_table && a->max_pages_per_request > 0))
+    Fail(DSD_EINVAL, "null device array");
   const int eb = ElemBytes(a->dtype);
   if (!Aligned(a->q, eb) || !Aligned(a->out, eb) || !Aligned(a->lse, 4))
     Fail(DSD_EINVAL, "q, out and lse must be aligned to their type");

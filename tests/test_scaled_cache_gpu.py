@@ -306,6 +306,155 @@ def test_attend(torch, dsd, fmt, dtype, D, H, Hk, P, bt, layout, lens, new, caus
         at += n
 
 
+@pytest.mark.parametrize("arrangement", ["kv in one page", "padded rows", "padded pages", "odd base", "rows of tokens"])
+@pytest.mark.parametrize("new", [None, [40, 7]])
+def test_attend_and_append_other_arrangements(torch, dsd, arrangement, new):
+    """Pools whose K and V share pages or whose strides TMA does or does not take give the plain pool's bits."""
+    s = Setup(torch, dsd, "fp8", [150, 60], 64, 2, 16, seed=31)
+    pages, P, Hk, D = s.pool.codes["k"].shape
+    raw = torch.zeros(pages * P * Hk * D * 6 + 4096, dtype=torch.int8, device="cuda")
+
+    def views():
+        if arrangement == "kv in one page":
+            both = raw[:2 * pages * P * Hk * D].view(pages, 2, P, Hk, D)
+            return both[:, 0], both[:, 1]
+        if arrangement == "padded rows":          # 72 bytes a row
+            both = raw[:2 * pages * P * Hk * 72].view(2, pages, P, Hk, 72)
+            return both[0, ..., 4:68], both[1, ..., :64]
+        if arrangement == "padded pages":         # a page stride that is no multiple of a token's
+            both = raw[:2 * pages * (P * Hk * D + 48)].view(2, pages, -1)
+            return tuple(both[i, :, :P * Hk * D].unflatten(1, (P, Hk, D)) for i in range(2))
+        if arrangement == "odd base":
+            both = raw[8:8 + 2 * pages * P * Hk * D].view(2, pages, P, Hk, D)
+            return both[0], both[1]
+        both = raw[:2 * pages * P * Hk * D].view(2, P, pages, Hk, D).transpose(1, 2)   # slot-major pool
+        return both[0], both[1]
+
+    k, v = views()
+    k.copy_(s.cache.k_codes.view(torch.int8))
+    v.copy_(s.cache.v_codes.view(torch.int8))
+    other = dsd.ScaledKVCache.from_tensors(k.view(torch.float8_e4m3fn),
+                                           v.view(torch.float8_e4m3fn), s.cache.k_scales.clone(), s.cache.v_scales.clone())
+    counts = new or [1, 1]
+    T = sum(counts)
+    offs = offsets_of(torch, counts) if new else None
+    rot = dsd.RotaryTable.from_base(200, 64)
+    x = [torch.randn(T, h, 64, device="cuda").bfloat16() * 2 for h in (2, 2, 8)]
+    before = raw.clone()
+    outs = []
+    for c in (s.cache, other):
+        q = c.append(x[0], x[1], s.d_table, s.d_lens, offs, rotary=rot, q=x[2])
+        outs.append((q, *c.attend(q, s.d_table, s.d_lens, offs, return_lse=True)))
+        c.check()
+    assert torch.equal(outs[0][0], outs[1][0])
+    for c in "kv":
+        assert torch.equal(getattr(s.cache, c + "_codes").view(torch.int8), {"k": k, "v": v}[c])
+        assert torch.equal(getattr(s.cache, c + "_scales"), getattr(other, c + "_scales"))
+    # nothing outside the views was written
+    mine = torch.zeros_like(raw, dtype=torch.bool)
+    for y in (k, v):
+        mine.as_strided(y.shape, y.stride(), y.storage_offset()).fill_(True)
+    assert torch.equal(raw[~mine], before[~mine])
+    # the paths differ in rounding only: both within the bound of the exact result
+    at = 0
+    s.pool.codes = {n: getattr(s.cache, n + "_codes").view(torch.int8).cpu().numpy().view(np.uint8) for n in "kv"}
+    s.pool.scales = {n: getattr(s.cache, n + "_scales").cpu().numpy() for n in "kv"}
+    for b, n in enumerate(counts):
+        y = f32(outs[0][0][at:at + n])
+        want, wl = o.attend(s.pool, y, s.table[b], s.lens[b], 0.125)
+        to, tl = tolerance(y, s.pool, s.table[b], s.lens[b], 0.125, want, wl, "bf16", 4)
+        for _, out, lse in outs:
+            close(f32(out[at:at + n]).astype(np.float64), want, to)
+            close(f32(lse[at:at + n]).astype(np.float64), wl, tl)
+        at += n
+
+
+def test_empty_tables_and_batches(torch, dsd):
+    """A page table without columns, a batch without requests, a call without queries."""
+    cache = dsd.ScaledKVCache(4, 16, 2, 64)
+    none = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    out, lse = cache.attend(q, none, lens, return_lse=True)
+    assert not out.any() and bool((lse == -float("inf")).all())
+    out = cache.attend_pages(q, none, lens, torch.zeros(4, dtype=torch.int32, device="cuda"))
+    assert not out.any()
+    assert cache.attend(q[:0], none[:0], lens[:0]).shape == (0, 4, 64)
+    assert cache.append(q[:0, :2], q[:0, :2], none[:0], lens[:0]) is None
+    cache.check()
+    cache.append(q[:, :2], q[:, :2], none, lens + 1)      # a token but no page
+    assert not cache.k_codes.view(torch.int8).any()
+    with pytest.raises(dsd.OutOfRange):
+        cache.check()
+
+
+def test_large_batches_take_the_general_plan(torch, dsd):
+    """More than 128 requests, and ragged queries with empty requests between."""
+    rng = np.random.default_rng(5)
+    for B, ragged in ((300, False), (200, True)):
+        lens = rng.integers(0, 90, B).tolist()
+        s = Setup(torch, dsd, "int8", lens, 64, 2, 16, seed=B)
+        new = rng.integers(0, 4, B).tolist() if ragged else [1] * B
+        q = torch.randn(sum(new), 4, 64, device="cuda").half()
+        out = s.cache.attend(q, s.d_table, s.d_lens, offsets_of(torch, new) if ragged else None)
+        s.cache.check()
+        at = 0
+        for b, n in enumerate(new):
+            x = f32(q[at:at + n])
+            if n:
+                want, wl = o.attend(s.pool, x, s.table[b], lens[b], 0.125)
+                to, _ = tolerance(x, s.pool, s.table[b], lens[b], 0.125, want, wl, "f16", 2)
+                close(f32(out[at:at + n]).astype(np.float64), want, to)
+            at += n
+
+
+def test_negative_and_zero_logit_scale(torch, dsd):
+    s = Setup(torch, dsd, "fp8", [300, 40], 128, 2, 16, seed=41)
+    for n in ([1, 1], [30, 20]):
+        q = torch.randn(sum(n), 8, 128, device="cuda").bfloat16()
+        for scale in (-0.1, 0.0, 0.5):
+            out, lse = s.cache.attend(q, s.d_table, s.d_lens, offsets_of(torch, n), scale=scale, return_lse=True)
+            at = 0
+            for b, m in enumerate(n):
+                x = f32(q[at:at + m])
+                want, wl = o.attend(s.pool, x, s.table[b], s.lens[b], scale)
+                to, tl = tolerance(x, s.pool, s.table[b], s.lens[b], scale, want, wl, "bf16", 4)
+                close(f32(out[at:at + m]).astype(np.float64), want, to)
+                close(f32(lse[at:at + m]).astype(np.float64), wl, tl)
+                at += m
+
+
+def test_first_call_inside_a_capture(dsd, tmp_path):
+    """A process whose first append and attend are captured, then replayed."""
+    import subprocess
+    import sys
+    from conftest import PKG_NAME, ROOT
+    code = f"""
+import importlib, sys
+sys.path.insert(0, {ROOT!r})
+import torch
+dsd = importlib.import_module({PKG_NAME!r})
+cache = dsd.ScaledKVCache(8, 16, 2, 64)
+table = torch.arange(8, dtype=torch.int32, device="cuda").reshape(2, 4)
+lens = torch.tensor([40, 20], dtype=torch.int32, device="cuda")
+x = torch.randn(2, 2, 64, device="cuda").bfloat16()
+q = torch.randn(2, 8, 64, device="cuda").bfloat16()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    cache.append(x, x, table, lens)
+    out = cache.attend(q, table, lens)
+g.replay()
+torch.cuda.synchronize()
+want = cache.attend(q, table, lens)
+assert torch.equal(out, want) and out.isfinite().all()
+cache.check()
+print("ok")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("fmt,dtype,D,H,Hk,P", [("fp8", "bf16", 128, 8, 2, 16), ("int8", "f32", 64, 2, 2, 32),
                                                 ("fp8", "f16", 96, 4, 1, 256), ("int8", "bf16", 72, 4, 2, 6)])
 def test_attend_pages(torch, dsd, fmt, dtype, D, H, Hk, P):
