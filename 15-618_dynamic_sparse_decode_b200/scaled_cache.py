@@ -212,7 +212,7 @@ class ScaledKVCache:
             if q.shape[0] != tokens:
                 _invalid("q must have a row for each token")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = torch.empty_like(q)
                 op = q_out.data_ptr()
             else:
                 op = self._rows("q_out", q_out, q.dtype, q.shape)
@@ -233,7 +233,7 @@ class ScaledKVCache:
         rows, heads = q.shape[0], q.shape[1]
         qp = self._rows("q", q)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q)
             op = out.data_ptr()
         else:
             op = self._rows("out", out, q.dtype, q.shape)
@@ -243,13 +243,13 @@ class ScaledKVCache:
         held = None if counts is None else self._ints("page_counts", counts, self.num_pages)
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        lse = self.k_scales.new_empty((rows, heads)) if return_lse else None
         key = (batch, rows, heads, offsets is None, q.dtype)
         need = self._workspace.get(key)   # bytes, a function of the sizes alone
         if need is None:
             need = self._workspace_bytes(key)
         # a new block each call: torch orders its reuse by stream, and a captured graph keeps its own
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        work = self.status.new_empty((need + 3) // 4)
         q_stride, out_stride = q.stride(), out.stride()
         args = _ATTENTION_ARGS.pack(
             _TYPES[q.dtype], batch, rows, heads, qp or 0, op or 0, lse.data_ptr() if return_lse else 0, q_stride[0], q_stride[1],
