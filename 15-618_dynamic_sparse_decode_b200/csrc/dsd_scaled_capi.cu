@@ -410,12 +410,15 @@ void CheckAttention(const dsd_scaled_cache* c, const dsd_scaled_attention_args* 
     Fail(DSD_EINVAL, "without q_offsets every request has one query: total_queries must equal batch");
   if (a->num_q_heads < 1 || a->num_q_heads > 4096 || a->num_q_heads % c->num_kv_heads)
     Fail(DSD_EINVAL, "num_q_heads must be a multiple of num_kv_heads, at most 4096");
-  if (int64_t(a->total_queries) * a->num_q_heads > INT32_MAX) Fail(DSD_EINVAL, "too many query rows for one call");
+  if (int64_t(a->total_queries) * a->num_q_heads > INT32_MAX - 4096)
+    Fail(DSD_EINVAL, "too many query rows for one call");
   if (a->max_pages_per_request < 0 || a->page_table_stride < 0)
     Fail(DSD_EINVAL, "page-table sizes must not be negative");
   if (a->window < 0) Fail(DSD_EINVAL, "window must not be negative");
   if (a->page_counts && (a->causal || a->window))
     Fail(DSD_EINVAL, "a page list has no order: causal and window must be 0 with page_counts");
+  if (a->page_counts && int64_t(a->max_pages_per_request) * (c->page_size / dsds::kTile + 1) > INT32_MAX)
+    Fail(DSD_EINVAL, "the page lists are too long for one call");
   if (!std::isfinite(a->scale)) Fail(DSD_EINVAL, "scale must be finite");
 }
 
@@ -478,6 +481,10 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   p.ppt = p.P <= dsds::kTile ? dsds::kTile / p.P : 0;
   p.tpp = p.P <= dsds::kTile ? 0 : (p.P + dsds::kTile - 1) / dsds::kTile;
   p.R = pl.R;
+  // one query each, at most 128 requests, and no sum of tiles beyond an int
+  const int64_t tiles = p.counts ? int64_t(p.max_pages) * std::max(1, p.tpp)
+                                 : (int64_t(p.max_pages) * p.P + 7) / 8 + p.max_pages;
+  p.few = !p.q_off && p.batch <= 128 && tiles * ((p.G + p.R - 1) / p.R) * p.batch < INT32_MAX;
   p.by_page = dsds::divisor_of(p.P);
   p.by_group = dsds::divisor_of(p.G);
   p.by_block = dsds::divisor_of(p.bt);

@@ -79,6 +79,7 @@ struct AttnParams {
   int ppt;            // pages per tile (page_size <= 128), else 0
   int tpp;            // tiles per page (page_size > 128), else 0
   int R;              // query rows of a unit
+  int few;            // plan_few will do: its sums fit
   Divisor by_page, by_group, by_block, by_tpp, by_tile;   // P, G, bt, tpp, ppt * P (1 where 0)
   int token_entries, token_stages;   // of TokenRing
   int ncta, gangs;    // ncta = gangs * Hk; CTA = gang * Hk + head
@@ -246,7 +247,7 @@ __device__ __forceinline__ void plan_few(const AttnParams& p, int gang, Walk* w)
 template <int THREADS>
 __device__ void plan_walk(const AttnParams& p, int gang, int* wb, Walk* w) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (!p.q_off && p.batch <= 128) {
+  if (p.few) {
     if (warp == 0) plan_few(p, gang, w);
     __syncthreads();
     return;
@@ -258,7 +259,7 @@ __device__ void plan_walk(const AttnParams& p, int gang, int* wb, Walk* w) {
     if (blockIdx.x == 0 && p.status && (p.q_off == nullptr || lane == 0)) bad |= bad_request(p, b, r);
     const int qts = (r.rows + p.R - 1) / p.R;
     // one query: every row tile sees the same tokens; several: the lanes share the row tiles
-    int sum = 0;
+    long long sum = 0;
 #pragma unroll 1
     for (int qt = p.q_off ? lane : 0; qt < qts; qt += 32) {
       sum += slots_of(span_of(p, r, qt));
@@ -267,8 +268,11 @@ __device__ void plan_walk(const AttnParams& p, int gang, int* wb, Walk* w) {
         break;
       }
     }
-    if (p.q_off) sum = __reduce_add_sync(~0u, sum);
-    if (!p.q_off || lane == 0) wb[b] = sum;
+    if (p.q_off) {
+#pragma unroll 1
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    }
+    if (!p.q_off || lane == 0) wb[b] = static_cast<int>(min(sum, static_cast<long long>(INT_MAX)));
   }
   __syncthreads();
   if (warp == 0) {
@@ -277,7 +281,7 @@ __device__ void plan_walk(const AttnParams& p, int gang, int* wb, Walk* w) {
     for (int b = lane; b < p.batch; b += 32) all += wb[b];
 #pragma unroll 1
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
-    if (all > INT_MAX) {   // more than hours of work: refused
+    if (all >= INT_MAX) {   // more than hours of work: refused
       bad |= DSD_SCALED_BAD_LENGTH;
       all = 0;
     }

@@ -5,9 +5,10 @@ The binding of ``dsd_scaled_append`` / ``dsd_scaled_attention``
 stored key or value is ``code * scale``: an e4m3 or int8 code under one fp32
 scale for each page, key head and run of ``block_tokens`` tokens of a page.
 
-Every call runs on the current torch stream of the cache's device, allocates
-only what it returns plus the attention's workspace (from torch's allocator),
-never synchronises, and can be captured into a CUDA graph.  What only the device
+For serving: results carry no gradient.  Every call runs on the current torch
+stream of the cache's device, allocates only what it returns plus the
+attention's workspace (from torch's allocator), never synchronises, and can be
+captured into a CUDA graph.  What only the device
 can see (page ids, lengths, positions) is checked there: see
 :meth:`ScaledKVCache.check`.
 """
@@ -254,7 +255,7 @@ class ScaledKVCache:
         args = _ATTENTION_ARGS.pack(
             _TYPES[q.dtype], batch, rows, heads, qp or 0, op or 0, lse.data_ptr() if return_lse else 0, q_stride[0], q_stride[1],
             out_stride[0], out_stride[1], offsets or 0, lens_at or 0, table_at or 0, stride, held or 0, table.shape[1], scale,
-            causal, window, work.data_ptr() or 0, need, self._status_at)
+            causal, min(window, 0x7fffffff), work.data_ptr() or 0, need, self._status_at)
         _check(self.lib.dsd_scaled_attention(self._index, self._desc_at, args, _raw_stream(self._index)))
         return (out, lse) if return_lse else out
 
