@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kSimpleThreads) attn_simple_kernel(const __gri
   if (w.left == 0) return;
   while (w.left > 0) {
     const Request r = w.r;
-    const Span span = span_of(p, r, w.qt);
+    const Span span = w.span;
     const int slots = slots_of(span);
     const Segment seg = segment_of(w, slots);
     const int row0 = w.qt * R;

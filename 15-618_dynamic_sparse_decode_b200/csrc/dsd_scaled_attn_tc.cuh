@@ -289,7 +289,7 @@ __device__ __forceinline__ void walk_boxes(const AttnParams& p, Walk w, int head
 #pragma unroll 1
   while (w.left > 0 && ok) {
     const Request r = w.r;
-    const Span span = span_of(p, r, w.qt);
+    const Span span = w.span;
     const Segment seg = segment_of(w, slots_of(span));
     const int tiles = span.n == 0 ? 0 : seg.n;
     int next = -1;
@@ -340,7 +340,7 @@ __device__ __forceinline__ void walk_tokens(const AttnParams& p, Walk w, int hea
 #pragma unroll 1
   while (w.left > 0 && ok) {
     const Request r = w.r;
-    const Span span = span_of(p, r, w.qt);
+    const Span span = w.span;
     const Segment seg = segment_of(w, slots_of(span));
     const int tiles = span.n == 0 ? 0 : seg.n;
     const int* table = p.table + 1ll * w.b * p.table_stride;
@@ -668,8 +668,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUt
                                   elem, aligned);
         }
       }
-      Span span{0, 0};
-      if (!end) span = span_of(p, r, w.qt);
+      const Span span = w.span;
       const int slots = slots_of(span);
       const Segment seg = segment_of(w, slots);
       ok = mbar_wait(&unit_empty[u], (unit >> 1 & 1) ^ 1, &stop, p.status);

@@ -275,8 +275,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       const int u = unit & 1;
       const bool end = w.left <= 0;
       const Request r = w.r;
-      Span span{0, 0};
-      if (!end) span = span_of(p, r, w.qt);
+      const Span span = w.span;
       const int slots = slots_of(span);
       const Segment seg = segment_of(w, slots);
       ok = __all_sync(~0u, mbar_wait(&unit_empty[u], (unit >> 1 & 1) ^ 1, &stop, p.status));
@@ -393,7 +392,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
     int tiles_left = 0;
 #pragma unroll 1
     while (w.left > 0) {
-      const Span span = span_of(p, w.r, w.qt);
+      const Span span = w.span;
       const Segment seg = segment_of(w, slots_of(span));
       tiles_left += span.n == 0 ? 0 : seg.n;
       next_unit(p, seg, w);

@@ -165,6 +165,7 @@ struct Walk {
   int at, left;   // slot of the axis, slots left
   int total;
   Request r;      // of b
+  Span span;      // of (b, qt)
 };
 
 // The axis in p.gangs parts that differ by one slot at most (fewer where there are
@@ -196,19 +197,27 @@ __device__ __forceinline__ unsigned bad_request(const AttnParams& p, int b, cons
 __device__ __forceinline__ void plan_few(const AttnParams& p, int gang, Walk* w) {
   const int lane = threadIdx.x & 31;
   const int per = (p.batch + 31) / 32, first = lane * per;
+  int lens[4];   // all loads before the first use
+#pragma unroll
+  for (int j = 0; j < 4; ++j) lens[j] = j < per && first + j < p.batch ? p.lens[first + j] : 0;
   Request r[4];
+  Span span[4];
   int slots[4], mine = 0;
   unsigned bad = 0;
   const int row_tiles = (p.G + p.R - 1) / p.R;
+  const long long most = p.counts ? p.max_pages : 1ll * p.max_pages * p.P;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     slots[j] = 0;
     if (j >= per || first + j >= p.batch) continue;
-    r[j] = request_of(p, first + j);
-    if (blockIdx.x == 0 && p.status) bad |= bad_request(p, first + j, r[j]);
-    slots[j] = r[j].rows ? row_tiles * slots_of(span_of(p, r[j], 0)) : 0;
+    r[j] = {first + j, 1, p.G, static_cast<int>(min(max(static_cast<long long>(lens[j]), 0ll), most))};
+    if (lens[j] < 0) bad |= DSD_SCALED_BAD_LENGTH;
+    if (lens[j] > most) bad |= DSD_SCALED_BAD_PAGE;
+    span[j] = span_of(p, r[j], 0);
+    slots[j] = row_tiles * slots_of(span[j]);
     mine += slots[j];
   }
+  if (blockIdx.x || !p.status) bad = 0;
   if (bad) atomicOr(p.status, static_cast<int>(bad));
   int upto = mine;
 #pragma unroll
@@ -233,6 +242,7 @@ __device__ __forceinline__ void plan_few(const AttnParams& p, int gang, Walk* w)
         const int each = slots[j] / row_tiles;
         x.b = first + j;
         x.r = r[j];
+        x.span = span[j];   // the same for every row tile of one query
         x.qt = rest / each;
         x.slot = rest - x.qt * each;
         rest = -1;
@@ -340,6 +350,7 @@ __device__ void plan_walk(const AttnParams& p, int gang, int* wb, Walk* w) {
         }
       }
     }
+    if (x.left > 0) x.span = span_of(p, x.r, x.qt);
     if (lane == 0) *w = x;
   }
   if (bad && blockIdx.x == 0 && p.status) atomicOr(p.status, static_cast<int>(bad));
@@ -368,13 +379,15 @@ __device__ __noinline__ void next_unit(const AttnParams& p, const Segment& seg, 
   w.left -= seg.n;
   if (w.left <= 0) return;
   w.slot = 0;
-  if (++w.qt < (w.r.rows + p.R - 1) / p.R) return;
-  w.qt = 0;
-  do {
-    ++w.b;
-    if (w.b >= p.batch) return;
-    w.r = request_of(p, w.b);
-  } while (w.r.rows == 0);
+  if (++w.qt >= (w.r.rows + p.R - 1) / p.R) {
+    w.qt = 0;
+    do {
+      ++w.b;
+      if (w.b >= p.batch) return;
+      w.r = request_of(p, w.b);
+    } while (w.r.rows == 0);
+  }
+  w.span = span_of(p, w.r, w.qt);
 }
 
 // Token i (0..127) of a unit's tile: its page (-1: none), slot in the page, place in the request.

@@ -20,8 +20,8 @@ import struct
 
 import torch
 
-from . import (DSD_EINVAL, KV_FP8_SCALED, KV_I8_SCALED, InvalidArgument, OutOfRange, ScaledAttentionArgs,
-               ScaledCacheDesc, _check, load_library)
+from . import (DSD_EINVAL, DSD_ERANGE, DSD_ETIMEOUT, KV_FP8_SCALED, KV_I8_SCALED, DsdError, InvalidArgument, OutOfRange,
+               ScaledAttentionArgs, ScaledCacheDesc, _check, load_library)
 
 _FORMATS = {torch.float8_e4m3fn: KV_FP8_SCALED, torch.int8: KV_I8_SCALED}
 _CODES = {v: k for k, v in _FORMATS.items()}
@@ -173,8 +173,8 @@ class ScaledKVCache:
             for bit, message in _BAD:
                 if bits & bit:
                     if bit == 8:
-                        raise RuntimeError(message)
-                    raise OutOfRange(2, message)
+                        raise DsdError(DSD_ETIMEOUT, message)
+                    raise OutOfRange(DSD_ERANGE, message)
 
     # ---- operators
     def append(self, k, v, page_table, seq_lens, token_offsets=None, rotary: RotaryTable | None = None,
