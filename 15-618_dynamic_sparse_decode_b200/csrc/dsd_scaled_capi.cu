@@ -209,13 +209,15 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   const int j = ve == 1 || block_slots > largest ? 0 : block_slots <= 32 ? 1 : block_slots <= largest / 2 ? 2 : 4;
   p.team = 1;
   while (p.team < 8 && p.team * 32 * (j ? j : dsds::kAppendKeep) < block_slots) p.team *= 2;
-  // blockIdx.y: CTAs of one block of tokens, keys and values first, then queries;
-  // as many as fill the GPU eight times over when there are few blocks, and no more
-  // than four rounds (of heads) to a CTA when there are many
+  // blockIdx.y: CTAs of one block of tokens, keys and values first, then queries; as
+  // many as give every SM one when there are few blocks, else up to eight rounds (of
+  // heads) to a CTA: its first loads wait for one another (offsets, lengths, pages), so
+  // fewer and longer CTAs win (7400 tokens of int8: 45 us, with eight CTAs per SM and
+  // four rounds 52 us).
   const int teams = dsds::kAppendThreads / 32 / p.team;
   const auto parts = [&](int rounds) {
-    const int64_t want = (8ll * dev.sms + units - 1) / units;
-    return int(std::min<int64_t>(rounds, std::max<int64_t>(want, (rounds + 3) / 4)));
+    const int64_t want = (dev.sms + units - 1) / units;
+    return int(std::min<int64_t>(rounds, std::max<int64_t>(want, (rounds + 7) / 8)));
   };
   p.y_kv = parts(((j ? 1 : 2) * p.Hk + teams - 1) / teams);
   const int y_q = p.Hq ? parts((p.Hq + 4 * dsds::kAppendHeads - 1) / (4 * dsds::kAppendHeads)) : 0;
