@@ -568,6 +568,64 @@ def test_scales_of_every_size(torch, dsd):
         close(f32(lse).astype(np.float64), wl, tl)
 
 
+def test_scales_of_every_size_with_many_rows(torch, dsd):
+    """The same with 16 query rows a key head: zero scales, and values that grow and shrink by 2^12 between pages,
+    so that the reference of the weights moves from tile to tile."""
+    for fmt, dtype in (("fp8", "bf16"), ("int8", "f16")):
+        s = Setup(torch, dsd, fmt, [700, 130], 64, 2, 16, seed=17)
+        v = s.pool.scales["v"]
+        for b, n in enumerate(s.lens):
+            for i in range(-(-n // 16)):
+                v[s.table[b, i]] = np.float32(0.0 if i % 7 == 6 else 2.0 ** (12 * ((i * 5) % 3 - 1)) * 1.3)
+        s.cache.v_scales.copy_(torch.from_numpy(v))
+        q = (torch.randn(2, 32, 64, device="cuda") * 3).to(getattr(torch, TYPES[dtype]))
+        out, lse = s.cache.attend(q, s.d_table, s.d_lens, return_lse=True)
+        for b, n in enumerate(s.lens):
+            x = f32(q[b:b + 1])
+            want, wl = o.attend(s.pool, x, s.table[b], n, 0.125)
+            to, tl = tolerance(x, s.pool, s.table[b], n, 0.125, want, wl, dtype, 16)
+            got = f32(out[b:b + 1]).astype(np.float64)
+            if dtype == "f16":
+                # the largest fp16 is 65504 and half a step behind it rounds to infinity: what is
+                # beyond 65520 by more than its bound has to be infinite, what may be, may
+                assert (np.isinf(got) | (np.abs(want) - to < 65520)).all()
+                over = np.isinf(got) & (np.abs(want) + to >= 65520) & (np.sign(got) == np.sign(want))
+                got = np.where(over, want, got)
+            close(got, want, to)
+            close(f32(lse[b:b + 1]).astype(np.float64), wl, tl)
+        s.cache.v_scales.zero_()
+        out, lse2 = s.cache.attend(q, s.d_table, s.d_lens, return_lse=True)
+        assert not out.any()
+        for b in range(2):
+            x = f32(q[b:b + 1])
+            want, wl = o.attend(s.pool, x, s.table[b], s.lens[b], 0.125)
+            close(f32(lse2[b:b + 1]).astype(np.float64), wl,
+                  tolerance(x, s.pool, s.table[b], s.lens[b], 0.125, want, wl, dtype, 16)[1])
+
+
+def test_threads_with_their_own_streams(torch, dsd):
+    """Calls from several host threads at once, each on its stream, into one cache's reader."""
+    import threading
+    s = Setup(torch, dsd, "int8", [900, 300, 50], 128, 2, 16, seed=23)
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    want = s.cache.attend(q, s.d_table, s.d_lens)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                if not torch.equal(s.cache.attend(q, s.d_table, s.d_lens), want):
+                    bad.append(1)
+        st.synchronize()
+
+    ts = [threading.Thread(target=work) for _ in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+
+
 def test_bad_pages_and_lengths_are_masked(torch, dsd):
     for D, P in ((128, 16), (72, 6)):
         s = Setup(torch, dsd, "int8", [100, 60, 30], D, 2, P, seed=14)
