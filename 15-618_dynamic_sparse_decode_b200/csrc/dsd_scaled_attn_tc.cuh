@@ -40,7 +40,7 @@
 namespace dsds {
 
 constexpr int kTcThreads = 256;
-constexpr int kTokenBytes = 3072;   // shared memory for token data, see TokenRing
+constexpr int kTokenBytes = 3 * 1024;   // shared memory for token data, see TokenRing
 constexpr int kTokenStages = 8;     // tiles of token data ahead at most
 constexpr int kTcTileBytes = kTile * 128;
 
