@@ -79,10 +79,6 @@ __device__ __forceinline__ uint64_t operand16_desc(uint32_t addr) {
          (uint64_t(2) << 61);
 }
 
-__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&x)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
-}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&x)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]),

@@ -10,10 +10,10 @@
 // walked by a gang of CTAs at once, one for each key head: in a token-major pool
 // the heads' rows of a token are neighbours in memory, and CTAs that read them at
 // about the same time keep DRAM in its open pages (64 requests x 16-32k: 604 us
-// with the heads one after another along the axis, 505 us with gangs).  A CTA derives its range from the lengths on the device
-// (no host knowledge of them, so a captured graph follows them); a unit that spans
-// ranges leaves partial results, at most two per CTA, which combine_kernel joins
-// in tile order.
+// with the heads one after another along the axis, 505 us with gangs).  A CTA
+// derives its range from the lengths on the device (no host knowledge of them, so a
+// captured graph follows them); a unit that spans ranges leaves partial results, at
+// most two per CTA, which combine_kernel joins in tile order.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -193,7 +193,7 @@ __device__ __forceinline__ unsigned bad_request(const AttnParams& p, int b, cons
 }
 
 // plan_walk for one query each and at most 128 requests, by one warp: a lane has four
-// requests in registers, and one scan finds the range (3.1 -> 2 us of a launch).
+// requests in registers, and one scan finds the range.
 __device__ __forceinline__ void plan_few(const AttnParams& p, int gang, Walk* w) {
   const int lane = threadIdx.x & 31;
   const int per = (p.batch + 31) / 32, first = lane * per;
