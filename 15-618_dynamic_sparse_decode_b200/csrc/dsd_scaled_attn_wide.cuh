@@ -11,11 +11,17 @@
 // 2^-29 of the row's largest).
 //
 // A weight carries its value scale: P = 2^(s - r) vs, fp16, back in TMEM as the A
-// operand of the second product.  The row's reference r comes from its largest
-// logit and the tile's largest value scale, so that O / sum is the output as it
-// stands and a column has two constants, its scales (with the exponent of vs in the
-// logits, as in the narrow kernel, it had four: chunks 522 us, with two 489 us).  A
-// weight keeps its bits down to 2^-20 of the row's largest.
+// operand of the second product, so that O / sum is the output as it stands.  The
+// row's reference r bounds the largest weight that it SEES from above.  Where every
+// row sees a whole tile and the tile's value scales lie within 2^8 of one another,
+// the largest logit and the largest scale bound it closely enough, and a column has
+// two constants, its scales (with the exponent of vs in the logits, as in the narrow
+// kernel, it had four: chunks 522 us, with two 489 us).  Elsewhere r comes from each
+// seen token's own logit and exponent: what a row does not see must not move its
+// weights, and a token with a large scale and next to no weight must not push the
+// others out of fp16 (chunks 502 us with the first bound for every tile, 507 us so).
+// A weight keeps its bits down to 2^-11 of the row's largest and an absolute 2^-22
+// of it below.
 //
 // The reference stays while nothing has grown past it by more than 2^8, which fp16
 // weights bear, so a tile is one pass over its logits; else the eight warps vote, O
@@ -172,11 +178,17 @@ __device__ __forceinline__ void widen_row(const uint8_t* codes, uint8_t* wide, i
   }
 }
 
+// Exponent that bounds a value scale from above, in the range of token_scale().
+__device__ __forceinline__ int scale_bound(float vs) {
+  return min(max(static_cast<int>(__float_as_uint(vs) >> 23 & 255) - 126, -64), 100);
+}
+constexpr int kWideSpread = 8;   // log2 of how far a tile's value scales may lie apart under one bound
+
 // A tile's tokens as the softmax reads them, four at a time.
 struct __align__(16) Columns {   // its size too: float4 reads of the second one
-  float ks[kTile], vs[kTile];
+  float ks[kTile], vs[kTile], bound[kTile];
   uint32_t valid[4];   // a bit per token
-  uint32_t largest[4]; // value scale of each 32 tokens, as bits
+  int largest[4], least[4];   // bounding exponents of each 32 tokens' value scales
   int place, open;     // open: every row sees every token that is there
 };
 
@@ -432,14 +444,16 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       }
       const float vs = !valid ? 0.0f : nan_row ? NAN : scales.y;
       const uint32_t present = __ballot_sync(~0u, valid);
-      const uint32_t largest = __reduce_max_sync(~0u, vs < INFINITY ? __float_as_uint(vs) : 0u);
+      const int largest = __reduce_max_sync(~0u, scale_bound(vs)), least = __reduce_min_sync(~0u, scale_bound(vs));
       ok = ok && mbar_wait(&cols_empty[cb], (g >> 1 & 1) ^ 1, &stop, p.status);
       Columns& c = cols[cb];
       c.ks[t] = valid ? scales.x : 0.0f;
       c.vs[t] = vs;
+      c.bound[t] = float(scale_bound(vs));
       if (lane == 0) {
         c.valid[t >> 5] = present;
         c.largest[t >> 5] = largest;
+        c.least[t >> 5] = least;
       }
       if (t == 0) {
         c.place = tile.place;
@@ -547,19 +561,22 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         in = mbar_wait(&s_full[buf], g >> 1 & 1, &stop, p.status) && in;
         __syncwarp();
         tc_fence_after();
-        const uint4 valid = *reinterpret_cast<const uint4*>(c.valid), largest = *reinterpret_cast<const uint4*>(c.largest);
-        const bool open = c.open != 0 && (valid.x & valid.y & valid.z & valid.w) == ~0u;
-        // 2^scale_up bounds the tile's value scales from above
-        const int top_bits = static_cast<int>(max(max(largest.x, largest.y), max(largest.z, largest.w)) >> 23) - 126;
-        const float scale_up = static_cast<float>(min(max(top_bits, -64), 100));
+        const uint4 valid = *reinterpret_cast<const uint4*>(c.valid);
+        const int4 largest = *reinterpret_cast<const int4*>(c.largest), least = *reinterpret_cast<const int4*>(c.least);
+        const int up = max(max(largest.x, largest.y), max(largest.z, largest.w));
+        // every row sees all places, and 2^up bounds their value scales closely
+        const bool open = c.open != 0 && (valid.x & valid.y & valid.z & valid.w) == ~0u &&
+                          up - min(min(least.x, least.y), min(least.z, least.w)) <= kWideSpread;
         // P and O are the last tile's until its product is done
         if (i > 0) {
           in = mbar_wait(&o_full, (g - 1) & 1, &stop, p.status) && in;
           __syncwarp();
           tc_fence_after();
         }
-        // The half's weights under the reference r, into P; their sum and the largest
-        // product S ks.  Values lie two to a register pair: one instruction for both.
+        // The half's weights under the reference r, into P; their sum and what bounds the
+        // largest: of an open tile the largest product S ks, else of what the row sees the
+        // largest logit with its scale's exponent.  Values lie two to a register pair: one
+        // instruction for both.
         const auto weigh = [&](float r, float& top) {
           const uint64_t factor2 = pair(factor, factor), r2 = pair(-r, -r);
           float sum = 0.0f;
@@ -595,7 +612,9 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
                 unpair(mul2(pair(raw[2 * j], raw[2 * j + 1]), j & 1 ? k[j / 2].y : k[j / 2].x), a, b);
                 const bool see_a = (there >> (2 * j) & 1) && 2 * j <= hi && 2 * j >= lo;
                 const bool see_b = (there >> (2 * j + 1) & 1) && 2 * j + 1 <= hi && 2 * j + 1 >= lo;
-                t[j & 3] = fmaxf(t[j & 3], fmaxf(see_a ? a : -INFINITY, see_b ? b : -INFINITY));
+                const float2 bound = *reinterpret_cast<const float2*>(&c.bound[at + 2 * j]);
+                t[j & 3] = fmaxf(t[j & 3], fmaxf(see_a ? fmaf(a, factor, bound.x) : -INFINITY,
+                                                 see_b ? fmaf(b, factor, bound.y) : -INFINITY));
                 const uint64_t w = pair(see_a ? ex2(fmaf(a, factor, -r)) : 0.0f, see_b ? ex2(fmaf(b, factor, -r)) : 0.0f);
                 sums[j & 1] = add2(sums[j & 1], w);
                 // the scale of a place that the row does not see may be NaN
@@ -624,13 +643,15 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
           }
           return sum;
         };
-        // One pass on the reference of the tiles so far; where a row's largest product
+        // One pass on the reference of the tiles so far; where a row's largest weight
         // has grown past what fp16 bears (seldom after the first tile), all eight warps
         // agree on new references and make the weights again.
         float top = -INFINITY;
         float sum = weigh(m == -INFINITY ? 0.0f : m, top);
         // the reference that this tile alone would take (-inf: the row sees nothing of it)
-        const auto fresh = [&](float t) { return t == -INFINITY ? -INFINITY : t * factor + scale_up - kWideOne; };
+        const auto fresh = [&](float t) {
+          return t == -INFINITY ? -INFINITY : (open ? fmaf(t, factor, float(up)) : t) - kWideOne;
+        };
         const auto grown = [&](float f) { return f > m + kWideGrow || (m == -INFINITY && f > m); };
         if (wide_sync_or(grown(fresh(top)) || !in)) {
           ok = !wide_sync_or(!in);

@@ -1,0 +1,140 @@
+"""The scaled 8-bit paged cache at its edges (GPU): what a row does not see, or barely sees, leaves it alone.
+
+attend: with p the exact softmax over the tokens that a row SEES and v = code * vs their values,
+  |out - exact| <= half a step of the output type * |exact| + (logits + exp + piece) * sum p |v|
+                   + spot * max(p vs) * sum |code| + half of the output type's least step
+logits, exp and piece as in test_scaled_cache_gpu.py, taken over the tokens seen.  spot: a weight p vs
+is kept to an absolute step of the row's largest.  Narrow kernel, largest in [1, 2): int8 2^-20, e4m3
+2^-25.  Wide kernel: the largest is at least 2^-3 in fp16, whose least step is 2^-24: 2^-22.  Taken: 2^-19.
+"""
+import numpy as np
+import pytest
+
+import scaled_cache_oracle as o
+from test_scaled_cache_gpu import Setup, TYPES, close, f32, offsets_of, torch  # noqa: F401  (torch is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+LEAST = {"f32": 0.0, "bf16": 0.0, "f16": 2.0 ** -25}   # the values here stay above 2^-100
+SPOT = 2.0 ** -19
+
+
+def exact_and_bounds(s, b, q, n, causal=True, window=0, dtype="bf16"):
+    """q [n][H][D] of request b: exact out and lse, and the bounds above, from the tokens each row sees."""
+    pool, L, D = s.pool, s.lens[b], s.D
+    H = q.shape[1]
+    G, scale = H // pool.Hk, D ** -0.5
+    out, lse = np.zeros(q.shape), np.full((n, H), -np.inf)
+    tol_o, tol_l = np.zeros(q.shape), np.zeros((n, H))
+    t = np.arange(L)
+    page, slot = s.table[b][t // s.P].astype(np.int64), t % s.P
+    for h in range(pool.Hk):
+        code = o.decode(pool.codes["v"][page, slot, h], pool.fmt)
+        vs = pool.scales["v"][page, h, slot // pool.bt].astype(np.float64)
+        k = pool.rows("k", s.table[b], t, h)
+        for j in range(n):
+            pos = L - n + j
+            seen = (t <= pos if causal else t >= 0) & ((t > pos - window) if window else True)
+            if not seen.any():
+                continue
+            for g in range(h * G, (h + 1) * G):
+                x = q[j, g].astype(np.float64)
+                z = k[seen] @ x * scale
+                p = np.exp(z - z.max())
+                total = p.sum()
+                p /= total
+                v = code[seen] * vs[seen][:, None]
+                out[j, g], lse[j, g] = p @ v, z.max() + np.log(total)
+                zerr = 2 * (D + 8) * 2.0 ** -24 * (np.abs(k[seen]) @ np.abs(x)).max() * scale
+                tol_o[j, g] = (HALF[dtype] * np.abs(out[j, g]) + (zerr + 2.0 ** -20 + 2.0 ** -11) * (p @ np.abs(v))
+                               + SPOT * (p * vs[seen]).max() * np.abs(code[seen]).sum(0) + LEAST[dtype])
+                tol_l[j, g] = zerr + 2.0 ** -20 * max(1.0, abs(lse[j, g]))
+    return out, lse, tol_o, tol_l
+
+
+def upload(torch, s):
+    for n in "kv":
+        getattr(s.cache, n + "_scales").copy_(torch.from_numpy(s.pool.scales[n]))
+        getattr(s.cache, n + "_codes").view(torch.int8).copy_(torch.from_numpy(s.pool.codes[n].view(np.int8)))
+
+
+def queries(torch, s, H, counts, dtype):
+    gen = torch.Generator("cuda").manual_seed(7)
+    q = torch.randn(sum(counts), H, s.D, device="cuda", generator=gen).to(getattr(torch, TYPES[dtype]))
+    q[..., 0] = 8.0          # element 0 of a key moves its logits by that element, 8 / sqrt(64)
+    return q
+
+
+def attend(torch, s, H, new, dtype, check=True, causal=True, window=0):
+    counts = new or [1] * len(s.lens)
+    q = queries(torch, s, H, counts, dtype)
+    out, lse = s.cache.attend(q, s.d_table, s.d_lens, offsets_of(torch, counts) if new else None, causal=causal, window=window,
+                              return_lse=True)
+    s.cache.check()
+    at = 0
+    for b, n in enumerate(counts if check else []):
+        want, wl, to, tl = exact_and_bounds(s, b, f32(q[at:at + n]), n, causal, window, dtype)
+        got = f32(out[at:at + n]).astype(np.float64)
+        if dtype == "f16":   # behind the largest fp16 there is no value to compare
+            got = np.where(np.abs(want) < 65000, got, want)
+        close(f32(lse[at:at + n]).astype(np.float64), wl, tl)
+        close(got, want, to)
+        at += n
+    return out, lse
+
+
+KINDS = [("fp8", "bf16"), ("int8", "bf16"), ("int8", "f16"), ("fp8", "f32")]
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("H,new", [(8, [33, 17]), (2, [150, 40])])
+@pytest.mark.parametrize("power", [16, 24, 40])
+def test_scales_that_a_row_must_not_see(torch, dsd, fmt, dtype, H, new, power):
+    """Later tokens of the same prompt with larger value scales: the rows before them stay as they are, bit for bit."""
+    s = Setup(torch, dsd, fmt, [300, 140], 64, 2, 16, bt=1, seed=51, spread=0.3)
+    ordinary = attend(torch, s, H, new, dtype, check=False)
+    for b, n in enumerate(new):
+        for t in range(s.lens[b] - n // 2, s.lens[b]):   # seen by the later half of the queries only
+            s.pool.scales["v"][s.table[b, t // 16], :, t % 16] *= np.float32(2.0 ** power)
+    upload(torch, s)
+    got = attend(torch, s, H, new, dtype)
+    at = 0
+    for n in new:
+        rows = slice(at, at + n - n // 2)
+        assert torch.equal(got[0][rows], ordinary[0][rows]) and torch.equal(got[1][rows], ordinary[1][rows])
+        at += n
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("H,new", [(8, None), (32, None), (8, [33, 17]), (2, [150, 40])])
+@pytest.mark.parametrize("power,drop", [(16, 200), (24, 200), (40, 200), (24, 12), (40, 25), (-40, 0)])
+@pytest.mark.parametrize("where", ["first tile", "all over"])
+def test_scales_of_tokens_that_weigh_nothing(torch, dsd, fmt, dtype, H, new, power, drop, where):
+    """Tokens that a row sees, with a far larger (or smaller) value scale and a logit lower by `drop`."""
+    s = Setup(torch, dsd, fmt, [400, 140], 64, 2, 16, bt=1, seed=52, spread=0.3)
+    for b, n in enumerate(s.lens):
+        for t in range(3, 100 if where == "first tile" else n, 9):
+            page, slot = s.table[b, t // 16], t % 16
+            s.pool.scales["v"][page, :, slot] *= np.float32(2.0 ** power)
+            s.pool.codes["k"][page, slot, :, :] = 0
+            s.pool.codes["k"][page, slot, :, 0] = o.encode(np.float32(-o.QMAX[fmt]), fmt)
+            s.pool.scales["k"][page, :, slot] = np.float32(drop / o.QMAX[fmt])
+    upload(torch, s)
+    attend(torch, s, H, new, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("H,new", [(8, None), (32, None), (2, [150, 40])])
+def test_tokens_with_scale_zero_that_weigh_most(torch, dsd, fmt, dtype, H, new):
+    """A token whose values are all zero takes most of the weight: the others keep their bits."""
+    s = Setup(torch, dsd, fmt, [400, 140], 64, 2, 16, bt=1, seed=53, spread=0.3)
+    for b, n in enumerate(s.lens):
+        for t in range(0, n, 50):
+            page, slot = s.table[b, t // 16], t % 16
+            s.pool.scales["v"][page, :, slot] = 0
+            s.pool.codes["k"][page, slot, :, :] = 0
+            s.pool.codes["k"][page, slot, :, 0] = o.encode(np.float32(o.QMAX[fmt]), fmt)
+            s.pool.scales["k"][page, :, slot] = np.float32(25 / o.QMAX[fmt])
+    upload(torch, s)
+    attend(torch, s, H, new, dtype)
