@@ -40,9 +40,10 @@
 namespace dsds {
 
 constexpr int kTcThreads = 256;
-constexpr int kTokenBytes = 3 * 1024;   // shared memory for token data, see TokenRing
+constexpr int kTokenBytes = 2816;   // shared memory for token data, see TokenRing
 constexpr int kTokenStages = 8;     // tiles of token data ahead at most
 constexpr int kTcTileBytes = kTile * 128;
+constexpr size_t kTcStatic = 4096;  // static shared memory of a narrow CTA at most
 
 __host__ __device__ constexpr int pad16(int n) { return (n + 15) / 16 * 16; }
 __host__ __device__ constexpr int pow2_at_least(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
@@ -52,10 +53,15 @@ struct TcShape {
   static constexpr int N = pad16(R * PIECES);           // columns of S and of O
   static constexpr int kColumns = pow2_at_least(4 * N);
   static constexpr int kOperand = (R * PIECES + 7) / 8 * 1024;   // bytes of Q' (and of one P')
-  // CTAs per SM and ring stages that 512 TMEM columns and 227 KiB allow
+  // CTAs per SM, and as many ring stages as shared memory then allows: an SM has 228 KiB,
+  // of which each CTA takes 1 KiB for the system and up to kTcStatic for its own variables.
+  // The host checks on its first call that this many CTAs fit: with one, the ranges cut for
+  // two run one after the other (64 requests of 1024-4096 tokens, 64 heads over 8: 128 us,
+  // with two 96).
   static constexpr int kCtas = 2;
-  static constexpr int kStages = N <= 32 ? 3 : 2;
-  static constexpr size_t kSmem = 1024 + size_t(kStages) * 2 * kTcTileBytes + 4 * kOperand;
+  static constexpr size_t bytes(int stages) { return 1024 + size_t(stages) * 2 * kTcTileBytes + 4 * kOperand; }
+  static constexpr int kStages = bytes(3) + kTcStatic + 1024 <= 228 * 1024 / kCtas ? 3 : 2;
+  static constexpr size_t kSmem = bytes(kStages);
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {

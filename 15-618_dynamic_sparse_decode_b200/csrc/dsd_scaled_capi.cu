@@ -32,7 +32,7 @@ struct Device {
 std::mutex g_mutex;
 Device g_devices[kMaxDevices];
 
-void SetAttentionAttributes();
+void SetAttentionAttributes(int device);
 
 const Device& DeviceOf(int device) {
   if (device < 0 || device >= kMaxDevices) Fail(DSD_EINVAL, "device index out of range");
@@ -43,7 +43,7 @@ const Device& DeviceOf(int device) {
     Check(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device), "device");
     if (major != 10) Fail(DSD_EUNAVAILABLE, "no sm_100 GPU at this device index");
     Check(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device), "SM count");
-    SetAttentionAttributes();
+    SetAttentionAttributes(device);
     d.ready = true;
   }
   return d;
@@ -270,19 +270,34 @@ void WithWide(bool i8, int dtype, F&& f) {
   else f(dsds::attn_wide_kernel<false, 1>, Tag<dsds::WideShape<1>>{});
 }
 
-void SetAttentionAttributes() {
+void SetAttentionAttributes(int device) {
   SetSimple<false, 1>(); SetSimple<false, 2>(); SetSimple<false, 4>(); SetSimple<false, 8>();
   SetSimple<true, 1>(); SetSimple<true, 2>(); SetSimple<true, 4>(); SetSimple<true, 8>();
+  int reserve = 0, shared = 0, registers = 0;   // of a block; of an SM
+  Check(cudaDeviceGetAttribute(&reserve, cudaDevAttrReservedSharedMemoryPerBlock, device), "device");
+  Check(cudaDeviceGetAttribute(&shared, cudaDevAttrMaxSharedMemoryPerMultiprocessor, device), "device");
+  Check(cudaDeviceGetAttribute(&registers, cudaDevAttrMaxRegistersPerMultiprocessor, device), "device");
   for (int i8 = 0; i8 < 2; ++i8)
-    for (int fp32 = 0; fp32 < 2; ++fp32)
-    {
-      const auto set = [](auto kernel, auto tag) {
+    for (int fp32 = 0; fp32 < 2; ++fp32) {
+      // The plan cuts the work for this many CTAs per SM.  (The occupancy call answers one
+      // for every kernel that allocates tensor memory, also where two run.)
+      const auto set = [&](auto kernel, auto tag, int threads, int ctas) {
         using Shape = typename decltype(tag)::type;
         Check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape::kSmem)),
               "shared memory attribute");
+        cudaFuncAttributes fa;
+        Check(cudaFuncGetAttributes(&fa, kernel), "function attributes");
+        const size_t bytes = (fa.sharedSizeBytes + Shape::kSmem + reserve + 127) / 128 * 128;
+        if (bytes * ctas > size_t(shared) || (fa.numRegs + 7) / 8 * 8 * threads * ctas > registers)
+          Fail(DSD_EUNAVAILABLE, "an SM has no room for " + std::to_string(ctas) + " attention blocks of " +
+                                     std::to_string(bytes) + " bytes and " + std::to_string(fa.numRegs) + " registers");
       };
-      for (int R = 1; R <= kTcMaxRows; R *= 2) WithTc(i8, fp32, R, set);
-      WithWide(i8, fp32 ? DSD_TYPE_F16 : DSD_TYPE_BF16, set);
+      const auto set_narrow = [&](auto kernel, auto tag) {
+        set(kernel, tag, dsds::kTcThreads, decltype(tag)::type::kCtas);
+      };
+      const auto set_wide = [&](auto kernel, auto tag) { set(kernel, tag, dsds::kWideThreads, 1); };
+      for (int R = 1; R <= kTcMaxRows; R *= 2) WithTc(i8, fp32, R, set_narrow);
+      WithWide(i8, fp32 ? DSD_TYPE_F16 : DSD_TYPE_BF16, set_wide);
     }
 }
 

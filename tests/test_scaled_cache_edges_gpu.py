@@ -138,3 +138,13 @@ def test_tokens_with_scale_zero_that_weigh_most(torch, dsd, fmt, dtype, H, new):
             s.pool.scales["k"][page, :, slot] = np.float32(25 / o.QMAX[fmt])
     upload(torch, s)
     attend(torch, s, H, new, dtype)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 8])
+def test_every_group_of_heads_fits_an_SM_as_planned(torch, dsd, fmt, dtype, rows):
+    """The first call checks that each kernel fits on an SM as often as the work is cut for; every shape then runs, with
+    more requests than one round of CTAs holds."""
+    s = Setup(torch, dsd, fmt, [130, 700, 5, 260], 128, 3, 32, bt=8, seed=54, spread=0.3)
+    attend(torch, s, 3 * rows, None, dtype)
