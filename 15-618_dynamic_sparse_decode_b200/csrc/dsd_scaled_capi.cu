@@ -259,7 +259,17 @@ void WithTc(bool i8, bool fp32, int R, F&& f) {
   if (fp32) return WithTc<false, 6>(R, f);
   return WithTc<false, 3>(R, f);
 }
-constexpr int kTcMaxRows = 8;
+constexpr int kTcMaxRows = 8;   // query rows of a narrow unit
+
+// More query rows of a request than this, on average, go to the wide kernel (never
+// fp32, see there).  The narrow one reads the cache once for every 8 rows, the wide
+// one widens each tile once whatever the rows.  64 requests of 1024-4096 tokens, 4 key
+// heads, bf16, narrow / wide: 12 rows 88 / 115 us, 16 rows 90 / 115, 20 rows 129 / 124,
+// 24 rows 127 / 117, 28 rows 163 / 128, 48 rows 237 / 131; int8 at 16 rows 88 / 119, at
+// 24 124 / 137, at 28 153 / 137; fp16 98 / 149, 129 / 144 and 164 / 155.  Between 16 and
+// 24 the two are near one another, unless a chunk stands among single tokens: with 63
+// of those, one of 100 queries (12 rows) 174 / 243, one of 320 (24 rows) 325 / 268.
+constexpr int kNarrowMaxRows = 16;
 
 template <typename F>
 void WithWide(bool i8, int dtype, F&& f) {
@@ -402,7 +412,7 @@ AttnPlan PlanAttention(const Device& dev, const dsd_scaled_cache* c, const dsd_s
   // query rows of a request: exact for one query each, the average otherwise
   const int64_t queries = a->q_offsets ? (int64_t(a->total_queries) + a->batch - 1) / a->batch : 1;
   const int64_t rows = queries * group;
-  pl.wide = pl.tc && !fp32 && rows > kTcMaxRows;
+  pl.wide = pl.tc && !fp32 && rows > kNarrowMaxRows;
   if (pl.wide) pl.R = dsds::kWideRows;
   while (pl.R < kTcMaxRows && pl.R < rows) pl.R *= 2;
   int per_sm = pl.wide ? 1 : 8;

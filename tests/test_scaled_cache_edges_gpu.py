@@ -148,3 +148,28 @@ def test_every_group_of_heads_fits_an_SM_as_planned(torch, dsd, fmt, dtype, rows
     more requests than one round of CTAs holds."""
     s = Setup(torch, dsd, fmt, [130, 700, 5, 260], 128, 3, 32, bt=8, seed=54, spread=0.3)
     attend(torch, s, 3 * rows, None, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("H,new", [(18, None), (24, None), (32, None), (34, None), (36, None), (50, None), (8, [4, 4]), (8, [4, 5]),
+                                   (8, [1, 7]), (8, [1, 30])])
+def test_rows_on_both_sides_of_the_kernels_limit(torch, dsd, fmt, dtype, H, new):
+    """9 query rows a key head and more: several narrow units, or one wide one; pages of different scales."""
+    s = Setup(torch, dsd, fmt, [400, 140], 64, 2, 16, bt=4, seed=55, spread=1.0)
+    attend(torch, s, H, new, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("power,drop", [(16, 200), (24, 12), (40, 25), (-40, 0)])
+def test_scales_of_tokens_that_weigh_nothing_for_large_groups(torch, dsd, fmt, dtype, power, drop):
+    """One query each, 32 heads a key head."""
+    s = Setup(torch, dsd, fmt, [400, 140], 64, 2, 16, bt=1, seed=56, spread=0.3)
+    for b, n in enumerate(s.lens):
+        for t in range(3, n, 9):
+            page, slot = s.table[b, t // 16], t % 16
+            s.pool.scales["v"][page, :, slot] *= np.float32(2.0 ** power)
+            s.pool.codes["k"][page, slot, :, :] = 0
+            s.pool.codes["k"][page, slot, :, 0] = o.encode(np.float32(-o.QMAX[fmt]), fmt)
+            s.pool.scales["k"][page, :, slot] = np.float32(drop / o.QMAX[fmt])
+    upload(torch, s)
+    attend(torch, s, 64, None, dtype)
