@@ -86,7 +86,7 @@ __device__ __forceinline__ void load_vec(const T* p, float* x) {
     __align__(16) T raw[VE];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
-      reinterpret_cast<uint4*>(raw)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(p)[i];
 #pragma unroll
     for (int i = 0; i < VE; ++i) x[i] = to_float(raw[i]);
   }
@@ -109,12 +109,12 @@ __device__ __forceinline__ void load_table(const float* p, float* x) {
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const float4 y = __ldg(reinterpret_cast<const float4*>(p) + i);
+      const float4 y = reinterpret_cast<const float4*>(p)[i];
       x[4 * i] = y.x; x[4 * i + 1] = y.y; x[4 * i + 2] = y.z; x[4 * i + 3] = y.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __ldg(p + i);
+    for (int i = 0; i < N; ++i) x[i] = p[i];
   }
 }
 template <bool I8, int VE>
@@ -182,9 +182,9 @@ struct RawSlot {
       constexpr int kVecs = VE * sizeof(T) / 16;
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
-        reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row + s.e0) + i);
+        reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(row + s.e0)[i];
         reinterpret_cast<uint4*>(v)[kVecs + i] =
-            s.two ? __ldg(reinterpret_cast<const uint4*>(row + s.e1) + i) : make_uint4(0, 0, 0, 0);
+            s.two ? reinterpret_cast<const uint4*>(row + s.e1)[i] : make_uint4(0, 0, 0, 0);
       }
     }
   }

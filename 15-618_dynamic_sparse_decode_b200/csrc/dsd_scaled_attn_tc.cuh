@@ -410,12 +410,12 @@ __device__ __forceinline__ void walk_tokens(const AttnParams& p, Walk w, int hea
 __device__ __forceinline__ uint4 load_four(const uint8_t* at, int elem, bool aligned) {
   uint4 y{0, 0, 0, 0};
   if (elem == 4) {
-    if (aligned) return __ldg(reinterpret_cast<const uint4*>(at));
+    if (aligned) return *reinterpret_cast<const uint4*>(at);
     const uint32_t* p = reinterpret_cast<const uint32_t*>(at);
     return {p[0], p[1], p[2], p[3]};
   }
   if (aligned) {
-    const uint2 z = __ldg(reinterpret_cast<const uint2*>(at));
+    const uint2 z = *reinterpret_cast<const uint2*>(at);
     y.x = z.x;
     y.y = z.y;
   } else {

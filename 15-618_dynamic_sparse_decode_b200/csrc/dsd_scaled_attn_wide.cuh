@@ -508,7 +508,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
         if (q_aligned) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (8 * i < n) raw[i] = __ldg(reinterpret_cast<const uint4*>(q) + i);
+            if (8 * i < n) raw[i] = reinterpret_cast<const uint4*>(q)[i];
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)

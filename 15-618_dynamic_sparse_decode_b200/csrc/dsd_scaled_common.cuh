@@ -50,7 +50,9 @@ __device__ __forceinline__ int operator/(int n, const Divisor& v) {
 __device__ __forceinline__ int operator%(int n, const Divisor& v) { return n - n / v * v.d; }
 
 // Every kernel here is launched before its predecessor in the stream has ended: it
-// touches memory after pdl_wait(), which waits for that end.  pdl_trigger() lets the
+// touches memory after pdl_wait(), which waits for that end.  What the predecessor may
+// have written is read with ordinary loads: the read-only path (ld.global.nc) wants
+// memory that stays as it is for the kernel's whole life.  pdl_trigger() lets the
 // successor's blocks be placed once all blocks of this grid have started.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

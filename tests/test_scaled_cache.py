@@ -147,3 +147,15 @@ def test_struct_sizes_match_the_header(tmp_path):
     assert [binding._APPEND_ARGS.size, binding._ATTENTION_ARGS.size] == got[1:3]
     assert got[3:] == [dsd.ScaledCacheDesc.v_stride.offset, dsd.ScaledAppendArgs.status.offset,
                        dsd.ScaledAttentionArgs.status.offset]
+
+
+def test_kernels_that_start_early_use_no_read_only_loads():
+    """They are placed before their predecessor ends: what it writes must not be read through the read-only path."""
+    import glob
+    import os
+    from conftest import PKG_NAME, ROOT
+    files = glob.glob(os.path.join(ROOT, PKG_NAME, "csrc", "dsd_scaled_*"))
+    assert len(files) > 4
+    for f in files:
+        code = "\n".join(line.split("//")[0] for line in open(f))
+        assert "__ldg" not in code and "ld.global.nc" not in code, f
