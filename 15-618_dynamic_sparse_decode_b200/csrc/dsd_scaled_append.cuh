@@ -247,6 +247,10 @@ __device__ __noinline__ void requantise(const AppendParams& p, uint8_t* codes, l
   }
 }
 
+// 1 / scale.  A block of scale 0 has finite values below 2^-100 only, which 2^-126 rounds
+// to 0 as 0 would, but infinities stay infinite and saturate.
+__device__ __forceinline__ float inverse_of(float scale) { return scale > 0.0f ? 1.0f / scale : 1.17549435e-38f; }
+
 // Largest magnitude, NaN aside; may be infinite.
 template <int VE>
 __device__ __forceinline__ float largest(const float (&x)[2 * VE], float m) {
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(kAppendThreads, J ? 2 : 3) append_kernel(const
       const auto finish = [&](bool is_v, float m, float old) {
         const float fresh = m < 7.888609052210118e-31f ? 0.0f : m * (1.0f / kQmax);   // 2^-100
         const float scale = held ? fmaxf(old, fresh) : fresh;
-        const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+        const float inv = inverse_of(scale);
         const long long* st = is_v ? p.vst : p.kst;
         uint8_t* codes = (is_v ? p.v : p.k) + page * st[0] + first * st[1] + head * st[2];
         if (held && scale > old) requantise<I8, VE>(p, codes, st[1], held, rank, width, old * inv);
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kAppendThreads, J ? 2 : 3) append_kernel(const
       constexpr float kQmax = I8 ? 127.0f : 448.0f;
       const float fresh = m < 7.888609052210118e-31f ? 0.0f : m * (1.0f / kQmax);   // 2^-100
       const float scale = held ? fmaxf(old, fresh) : fresh;
-      const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+      const float inv = inverse_of(scale);
       const long long* st = is_v ? p.vst : p.kst;
       uint8_t* codes = (is_v ? p.v : p.k) + page * st[0] + first * st[1] + head * st[2];
       if (held && scale > old) requantise<I8, VE>(p, codes, st[1], held, rank, width, old * inv);

@@ -173,3 +173,46 @@ def test_scales_of_tokens_that_weigh_nothing_for_large_groups(torch, dsd, fmt, d
             s.pool.scales["k"][page, :, slot] = np.float32(drop / o.QMAX[fmt])
     upload(torch, s)
     attend(torch, s, 64, None, dtype)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("D,bt,dtype", [(64, 16, "bf16"), (256, 128, "f16"), (72, 4, "f32"), (128, 16, "f32")])
+def test_append_infinities_into_blocks_of_zeros(torch, dsd, fmt, D, bt, dtype):
+    """Infinities saturate in a block without any finite value above 2^-100 too, and read as 0 there; NaN stays NaN
+    (e4m3) or 0 (int8).  When the block's scale grows they become 0."""
+    s = Setup(torch, dsd, fmt, [bt + 1, 1], D, 2, bt, seed=57)
+    n = [bt - 1, 1]
+    k, v = (torch.zeros(bt, 2, D, device="cuda", dtype=getattr(torch, TYPES[dtype])) for _ in range(2))
+    inf, top = float("inf"), 126 if fmt == "fp8" else 127
+    k[0, 0, 3], k[0, 1, 4], k[1, 0, 5] = inf, -inf, float("nan")
+    v[bt - 1] = inf                       # the one token of the other request: nothing finite
+    v[bt - 1, 1, ::2] = -inf
+    if dtype != "f16":
+        k[2, 0, 1] = -1e-35               # below 2^-100
+    lens = torch.tensor(n, dtype=torch.int32, device="cuda")
+    s.cache.append(k, v, s.d_table, lens, offsets_of(torch, n))
+    minus = 128 + 126 if fmt == "fp8" else 256 - 127
+    codes = {x: getattr(s.cache, x + "_codes").view(torch.int8).cpu().numpy().view(np.uint8) for x in "kv"}
+    scales = {x: getattr(s.cache, x + "_scales").cpu().numpy() for x in "kv"}
+    a, b = s.table[0, 0], s.table[1, 0]
+    want = np.zeros((bt - 1, 2, D), np.uint8)
+    want[0, 0, 3], want[0, 1, 4] = top, minus
+    if fmt == "fp8":
+        want[1, 0, 5] = 127
+        if dtype != "f16":
+            want[2, 0, 1] = 128           # -0
+    assert np.array_equal(codes["k"][a, :bt - 1], want) and not scales["k"][a].any()
+    want = np.full((2, D), top, np.uint8)
+    want[1, ::2] = minus
+    assert np.array_equal(codes["v"][b, 0], want) and not scales["v"][b].any()
+    # one token more, of ordinary size: the older codes are rounded to its scale
+    one = torch.ones(1, 2, D, device="cuda", dtype=k.dtype)
+    s.cache.append(one, one, s.d_table[:1], lens[:1] + 1)
+    got = s.cache.k_codes.view(torch.int8).cpu().numpy().view(np.uint8)[a]
+    assert (got[bt - 1] == top).all() and (got[:bt - 1][want_nan_free(fmt, got[:bt - 1])] & 127 == 0).all()
+    assert np.array_equal(s.cache.k_scales.cpu().numpy()[a], np.full((2, 1), np.float32(1 / o.QMAX[fmt]), np.float32))
+    s.cache.check()
+
+
+def want_nan_free(fmt, codes):
+    return codes & 127 != 127 if fmt == "fp8" else np.ones(codes.shape, bool)
