@@ -279,28 +279,34 @@ __global__ void __launch_bounds__(kAppendThreads, J ? 2 : 3) append_kernel(const
   const int u = blockIdx.x;
   pdl_wait();
   pdl_trigger();
-  int b = u, row0 = u, n = 1, i = 0;
+  int b = u, row0 = u, end = u + 1;
   if (p.off) {
+    // a request whose offsets descend has no unit: the last block, mostly an idle one, looks
+    if (p.status && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {
+      bool bad = false;
+      for (int at = threadIdx.x; at < p.batch; at += kAppendThreads) bad = bad || p.off[at + 1] < p.off[at];
+      if (bad) atomicOr(p.status, DSD_SCALED_BAD_LENGTH);
+    }
     // the last request whose first unit is not behind u
     int lo = 0, hi = p.batch;
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
-      const bool past = at >= hi || p.off[at] / p.bt + 2 * at > u;
+      const bool past = at >= hi || p.off[at] / p.bt > u - 2 * at;
       lo += step * __popc(__ballot_sync(~0u, !past));
       hi = min(hi, lo + step);
     }
     b = lo;
     row0 = p.off[b];
-    n = p.off[b + 1] - row0;
-    i = u - (row0 / p.bt + 2 * b);
+    end = p.off[b + 1];
   }
-  if (n <= 0) return;
-  const int len = p.lens[b], start = len - n;
+  if (end <= row0) return;
+  const int len = p.lens[b];
   const bool lead = threadIdx.x == 0 && blockIdx.y == 0;
-  if (start < 0 || row0 < 0 || row0 > p.total - n) {
+  if (row0 < 0 || end > p.total || len < end - row0) {
     if (lead && p.status) atomicOr(p.status, DSD_SCALED_BAD_LENGTH);
     return;
   }
+  const int start = len - (end - row0), i = p.off ? u - 2 * b - row0 / p.bt : 0;
   const long long blk = 1ll * (start / p.bt) + i;
   const long long from = max(static_cast<long long>(start), blk * p.bt);
   const long long to = min(static_cast<long long>(len), (blk + 1) * p.bt);

@@ -385,11 +385,15 @@ typedef struct dsd_scaled_cache {
  * 2^-100; whatever the scale array held is ignored).  A block that holds older
  * tokens keeps its scale unless the new tokens need a larger one; then the older
  * codes are rounded again to the larger scale.  code = round-to-nearest-even(
- * value * (1/scale)), saturating; infinities saturate, NaN is stored as NaN
+ * value * (1/scale)), saturating; infinities saturate (a block whose scale is 0
+ * reads them as 0), NaN is stored as NaN
  * (e4m3) or 0 (int8).
  *
  * A token whose page, position or length is bad is left out (its status bit is
- * set) and nothing outside the arrays is touched.  Two requests that append into
+ * set) and nothing outside the arrays is touched.  Offsets that descend set
+ * DSD_SCALED_BAD_LENGTH; which tokens of such a call are stored is unspecified.
+ * The query row of a token with a bad position, of a request with a bad length and
+ * behind the last request keeps what q_out held.  Two requests that append into
  * the same block in one call race: their codes and its scale are unspecified. */
 typedef struct dsd_scaled_append_args {
   int32_t dtype;                 /* DSD_TYPE_* of k, v, q, q_out */

@@ -216,3 +216,29 @@ def test_append_infinities_into_blocks_of_zeros(torch, dsd, fmt, D, bt, dtype):
 
 def want_nan_free(fmt, codes):
     return codes & 127 != 127 if fmt == "fp8" else np.ones(codes.shape, bool)
+
+
+@pytest.mark.parametrize("lens,offsets,good", [
+    ([20, 20, 20], [0, 20, 15, 35], None),                  # the middle request's offsets descend
+    ([20, 20, 20], [0, 20, 20, 10], [0]),                   # the last one's
+    ([20, -2 ** 31, 20], [0, 20, 40, 60], [0, 2]),          # no length at all
+    ([20, -1, 20], [0, 20, 40, 60], [0, 2]),
+    ([20, 19, 20], [0, 20, 40, 60], [0, 2]),                # fewer tokens than new ones
+    ([20, 20, 20], [0, 20, 40, 2 ** 31 - 1], [0, 1]),       # rows behind the arrays
+    ([20, 20, 20], [-2 ** 31, 20, 40, 60], [1, 2]),
+])
+@pytest.mark.parametrize("bt", [1, 16])
+def test_append_reports_lengths_and_offsets_that_fit_nothing(torch, dsd, lens, offsets, good, bt):
+    """The request is left out and its status bit set; the others are stored (where no later offset descends)."""
+    s = Setup(torch, dsd, "int8", [20, 20, 20], 64, 2, 16, bt=bt, seed=58)
+    k, v = (torch.randn(60, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    s.cache.append(k, v, s.d_table, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                   torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+    for b in good or []:
+        for name, x in (("k", k), ("v", v)):
+            s.pool.append(name, f32(x[offsets[b]:offsets[b + 1]]), s.table[b], 20)
+    if good:
+        s.same(torch)
+    with pytest.raises(dsd.OutOfRange, match="seq_lens or offsets"):
+        s.cache.check()
+    s.cache.check()
