@@ -148,6 +148,7 @@ SIGNATURES = [
     ("dsd_scaled_attention_workspace", ctypes.c_int, [ctypes.c_int, _VP, _VP,
                                                       ctypes.POINTER(ctypes.c_int64)]),
     ("dsd_scaled_attention", ctypes.c_int, [ctypes.c_int, _VP, _VP, _VP]),
+    ("dsd_scaled_take_status", ctypes.c_int, [ctypes.c_int, _VP, _VP, _VP]),
 ]
 
 _lib = None

@@ -544,6 +544,19 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   Launch(dsds::combine_kernel, dim3(unsigned(p.ncta), unsigned(std::min(p.R, 32))), p.D <= 128 ? 128 : 256, 0, s, p);
 }
 
+__global__ void take_status_kernel(int* status, int* bits) {
+  dsds::pdl_wait();
+  *bits = atomicExch(status, 0);
+}
+
+void TakeStatus(int device, int32_t* status, int32_t* bits, cudaStream_t s) {
+  if (!status || !bits || !Aligned(status, 4) || !Aligned(bits, 4))
+    Fail(DSD_EINVAL, "status and bits must be 4-byte aligned device words");
+  DeviceGuard guard(device);
+  DeviceOf(device);
+  Launch(take_status_kernel, dim3(1), 1, 0, s, status, bits);
+}
+
 }  // namespace
 
 extern "C" {
@@ -568,6 +581,10 @@ int dsd_scaled_attention_workspace(int device, const dsd_scaled_cache* cache,
 int dsd_scaled_attention(int device, const dsd_scaled_cache* cache, const dsd_scaled_attention_args* args,
                          void* stream) {
   return Guard([&]() { Attention(device, cache, args, static_cast<cudaStream_t>(stream)); });
+}
+
+int dsd_scaled_take_status(int device, int32_t* status, int32_t* bits, void* stream) {
+  return Guard([&]() { TakeStatus(device, status, bits, static_cast<cudaStream_t>(stream)); });
 }
 
 }  // extern "C"

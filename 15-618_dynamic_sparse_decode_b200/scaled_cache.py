@@ -30,7 +30,8 @@ _APPEND_ARGS = struct.Struct("@4i2P4q3Pq3P4i2P4q2P")
 _ATTENTION_ARGS = struct.Struct("@4i3P4q3PqPifiiPqP")
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the current stream's handle, without a Stream object
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_BAD = ((8, "a device-side wait exceeded its budget"),
+_TIMEOUT = 8
+_BAD = ((_TIMEOUT, "a device-side wait exceeded its budget"),
         (1, "a page id is outside the pool or a page is beyond the page-table row"),
         (2, "a position is outside the rotation table"),
         (4, "seq_lens or offsets that fit no token"))
@@ -166,15 +167,20 @@ class ScaledKVCache:
         return table.data_ptr(), table.stride(0) if batch > 1 else table.shape[1]
 
     def check(self) -> None:
-        """Waits for the device and raises if a call since the last check met bad device data."""
-        bits = int(self.status.item())
+        """Waits for the device, all its streams, and raises if a call since the last check met bad device data.
+
+        The message names all that was met.  What a call that is launched meanwhile meets
+        is raised here or by the next check.
+        """
+        torch.cuda.synchronize(self.device)
+        taken = self.status.new_empty(1)
+        _check(self.lib.dsd_scaled_take_status(self._index, self._status_at, taken.data_ptr(), _raw_stream(self._index)))
+        bits = int(taken.item())
         if bits:
-            self.status.zero_()
-            for bit, message in _BAD:
-                if bits & bit:
-                    if bit == 8:
-                        raise DsdError(DSD_ETIMEOUT, message)
-                    raise OutOfRange(DSD_ERANGE, message)
+            message = "; ".join(text for bit, text in _BAD if bits & bit)
+            if bits & _TIMEOUT:
+                raise DsdError(DSD_ETIMEOUT, message)
+            raise OutOfRange(DSD_ERANGE, message)
 
     # ---- operators
     def append(self, k, v, page_table, seq_lens, token_offsets=None, rotary: RotaryTable | None = None,

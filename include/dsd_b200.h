@@ -476,6 +476,11 @@ int dsd_scaled_attention_workspace(int device, const dsd_scaled_cache* cache,
 int dsd_scaled_attention(int device, const dsd_scaled_cache* cache,
                          const dsd_scaled_attention_args* args, void* stream);
 
+/* Moves the bits of a device status word to the device word `bits` and clears them, in
+ * one atomic step: a bit that a call on another stream sets meanwhile is in `bits` or
+ * stays in `status`. */
+int dsd_scaled_take_status(int device, int32_t* status, int32_t* bits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -159,3 +159,8 @@ def test_kernels_that_start_early_use_no_read_only_loads():
     for f in files:
         code = "\n".join(line.split("//")[0] for line in open(f))
         assert "__ldg" not in code and "ld.global.nc" not in code, f
+
+
+def test_refuses_status_words():
+    for status, bits in ((None, 4096), (4096, None), (4098, 4096), (4096, 4097)):
+        assert refused("dsd_scaled_take_status", status, bits, None)

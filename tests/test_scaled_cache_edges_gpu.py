@@ -242,3 +242,30 @@ def test_append_reports_lengths_and_offsets_that_fit_nothing(torch, dsd, lens, o
     with pytest.raises(dsd.OutOfRange, match="seq_lens or offsets"):
         s.cache.check()
     s.cache.check()
+
+
+def test_check_waits_for_every_stream_and_names_all_it_met(torch, dsd):
+    """Bits set by a call that still waits on another stream, several at once, each reported once."""
+    s = Setup(torch, dsd, "fp8", [20, 20], 64, 2, 16, seed=59)
+    k, v = (torch.randn(2, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    rot = dsd.RotaryTable.from_base(10, 64)
+    table = s.d_table.clone()
+    table[0, 1] = -1
+    s.cache.append(k, v, s.d_table, s.d_lens)
+    s.cache.attend(q, s.d_table, s.d_lens)
+    s.cache.check()
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(200_000_000)                           # a tenth of a second
+        s.cache.append(k, v, table, s.d_lens, rotary=rot)        # place 19 of a table with 10; no such page
+    with pytest.raises(dsd.OutOfRange, match="(?s)page.*rotation"):
+        s.cache.check()
+    s.cache.check()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(200_000_000)
+        s.cache.attend(q, table, s.d_lens)
+    with pytest.raises(dsd.OutOfRange, match="page"):
+        s.cache.check()
+    s.cache.check()
