@@ -72,6 +72,12 @@ void CheckCachePointers(const dsd_scaled_cache* c) {
   if (!Aligned(c->k_scales, 4) || !Aligned(c->v_scales, 4)) Fail(DSD_EINVAL, "scales must be 4-byte aligned");
 }
 
+// int32 arrays on the device; null where the call has none
+template <typename... T>
+void CheckInts(const T*... p) {
+  if (!(Aligned(p, 4) && ...)) Fail(DSD_EINVAL, "int32 device arrays must be 4-byte aligned");
+}
+
 void CheckType(int dtype) {
   if (dtype != DSD_TYPE_F32 && dtype != DSD_TYPE_BF16 && dtype != DSD_TYPE_F16)
     Fail(DSD_EINVAL, "dtype must be DSD_TYPE_F32, DSD_TYPE_BF16 or DSD_TYPE_F16");
@@ -136,6 +142,7 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   if (!a->k || !a->v || !a->seq_lens || (!a->page_table && a->max_pages_per_request > 0))
     Fail(DSD_EINVAL, "null device array");
   if (a->num_q_heads && (!a->q || !a->q_out)) Fail(DSD_EINVAL, "num_q_heads > 0 needs q and q_out");
+  CheckInts(a->token_offsets, a->seq_lens, a->page_table, a->positions, a->token_counts, a->status);
   const int eb = ElemBytes(a->dtype);
   const void* rows[] = {a->k, a->v, a->num_q_heads ? a->q : a->k, a->num_q_heads ? a->q_out : a->k};
   const int64_t* strides[] = {a->k_stride, a->v_stride, a->num_q_heads ? a->q_stride : a->k_stride,
@@ -456,6 +463,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
   CheckCachePointers(c);
   if (!a->q || !a->out || !a->lens || (!a->page_table && a->max_pages_per_request > 0))
     Fail(DSD_EINVAL, "null device array");
+  CheckInts(a->q_offsets, a->lens, a->page_table, a->page_counts, a->status);
   const int eb = ElemBytes(a->dtype);
   if (!Aligned(a->q, eb) || !Aligned(a->out, eb) || !Aligned(a->lse, 4))
     Fail(DSD_EINVAL, "q, out and lse must be aligned to their type");

@@ -164,3 +164,17 @@ def test_kernels_that_start_early_use_no_read_only_loads():
 def test_refuses_status_words():
     for status, bits in ((None, 4096), (4096, None), (4098, 4096), (4096, 4097)):
         assert refused("dsd_scaled_take_status", status, bits, None)
+
+
+@pytest.mark.parametrize("field", ["token_offsets", "seq_lens", "page_table", "positions", "token_counts", "status"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_refuses_misaligned_ints_of_an_append(field, off):
+    assert refused("dsd_scaled_append", ctypes.byref(cache()), ctypes.byref(append_args(**{field: 4096 + off})), None)
+
+
+@pytest.mark.parametrize("field", ["q_offsets", "lens", "page_table", "page_counts", "status"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_refuses_misaligned_ints_of_an_attention(field, off):
+    args = attention_args(causal=0, **{field: 4096 + off})
+    args.workspace, args.workspace_bytes = 4096, 2 ** 40
+    assert refused("dsd_scaled_attention", ctypes.byref(cache()), ctypes.byref(args), None)
