@@ -6,8 +6,10 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include "dsd_b200.h"
 #include "dsd_internal.h"
@@ -76,6 +78,16 @@ void CheckCachePointers(const dsd_scaled_cache* c) {
 template <typename... T>
 void CheckInts(const T*... p) {
   if (!(Aligned(p, 4) && ...)) Fail(DSD_EINVAL, "int32 device arrays must be 4-byte aligned");
+}
+
+// Rows of head_dim elements that a call writes: where two of them certainly share
+// memory (a stride below a row's length, or two dimensions of one stride), the blocks
+// that write them would race.
+void CheckWritten(int head_dim, std::initializer_list<std::pair<int64_t, int64_t>> dims, const char* what) {
+  for (auto a = dims.begin(); a != dims.end(); ++a)
+    for (auto b = dims.begin(); b != dims.end(); ++b)
+      if (a->first > 1 && (a->second < head_dim || (a != b && b->first > 1 && a->second == b->second)))
+        Fail(DSD_EINVAL, std::string("the rows of ") + what + " overlap");
 }
 
 void CheckType(int dtype) {
@@ -151,6 +163,10 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
     if (!Aligned(rows[i], eb)) Fail(DSD_EINVAL, "k, v, q and q_out must be aligned to their type");
     if (strides[i][0] < 0 || strides[i][1] < 0) Fail(DSD_EINVAL, "row strides must not be negative");
   }
+  for (const int64_t* st : {c->k_stride, c->v_stride})
+    CheckWritten(c->head_dim, {{c->num_pages, st[0]}, {c->page_size, st[1]}, {c->num_kv_heads, st[2]}}, "the cache");
+  if (a->num_q_heads)
+    CheckWritten(c->head_dim, {{a->total_tokens, a->q_out_stride[0]}, {a->num_q_heads, a->q_out_stride[1]}}, "q_out");
 
   // 8-element accesses where every row starts on their boundary, else single
   // elements (measured on unaligned rows only: no other path takes those)
@@ -469,6 +485,7 @@ void Attention(int device, const dsd_scaled_cache* c, const dsd_scaled_attention
     Fail(DSD_EINVAL, "q, out and lse must be aligned to their type");
   for (int i = 0; i < 2; ++i)
     if (a->q_stride[i] < 0 || a->out_stride[i] < 0) Fail(DSD_EINVAL, "row strides must not be negative");
+  CheckWritten(c->head_dim, {{a->total_queries, a->out_stride[0]}, {a->num_q_heads, a->out_stride[1]}}, "out");
   DeviceGuard guard(device);
   const Device& dev = DeviceOf(device);
   const AttnPlan pl = PlanAttention(dev, c, a);

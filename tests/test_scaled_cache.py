@@ -178,3 +178,32 @@ def test_refuses_misaligned_ints_of_an_attention(field, off):
     args = attention_args(causal=0, **{field: 4096 + off})
     args.workspace, args.workspace_bytes = 4096, 2 ** 40
     assert refused("dsd_scaled_attention", ctypes.byref(cache()), ctypes.byref(args), None)
+
+
+def strides(*n):
+    return (ctypes.c_int64 * len(n))(*n)
+
+
+def test_refuses_rows_that_overlap():
+    """Rows that a call writes must not share memory; rows that it reads may."""
+    lib = dsd.load_library()
+    for st in (strides(0, 64), strides(256, 0), strides(63, 256), strides(256, 8), strides(64, 64)):
+        args = append_args(num_q_heads=4, q=4096, q_out=4096, q_stride=strides(0, 0), q_out_stride=st)
+        assert refused("dsd_scaled_append", ctypes.byref(cache()), ctypes.byref(args), None)
+        assert b"q_out overlap" in lib.dsd_last_error()
+        args = attention_args(q_stride=strides(0, 0), out_stride=st, workspace=4096, workspace_bytes=2 ** 40)
+        assert refused("dsd_scaled_attention", ctypes.byref(cache()), ctypes.byref(args), None)
+        assert b"out overlap" in lib.dsd_last_error()
+    for name in ("k_stride", "v_stride"):
+        for st in (strides(32, 128, 64), strides(2048, 64, 64), strides(2048, 128, 1)):
+            assert refused("dsd_scaled_append", ctypes.byref(cache(**{name: st})), ctypes.byref(append_args()), None)
+            assert b"the cache overlap" in lib.dsd_last_error()
+
+
+def test_dimensions_of_one_may_have_any_stride():
+    lib = dsd.load_library()
+    args = append_args(batch=1, total_tokens=1, num_q_heads=1, q=4096, q_out=4096, q_out_stride=strides(0, 0))
+    one = cache(num_pages=1, page_size=1, block_tokens=1, num_kv_heads=1, k_stride=strides(1, 1, 1))
+    # the arrays are made up: no device has this index, so the call ends behind its checks
+    assert lib.dsd_scaled_append(99, ctypes.byref(one), ctypes.byref(args), None) not in (dsd.DSD_OK, dsd.DSD_EINVAL)
+    assert b"overlap" not in lib.dsd_last_error()
