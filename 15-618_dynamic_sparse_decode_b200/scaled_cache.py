@@ -28,6 +28,7 @@ _CODES = {v: k for k, v in _FORMATS.items()}
 # dsd_scaled_append_args and dsd_scaled_attention_args: one pack costs a tenth of setting the fields
 _APPEND_ARGS = struct.Struct("@4i2P4q3Pq3P4i2P4q2P")
 _ATTENTION_ARGS = struct.Struct("@4i3P4q3PqPifiiPqP")
+_UNFIT = (struct.error, OverflowError)   # pack: a number of another kind, or beyond its field
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the current stream's handle, without a Stream object
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TIMEOUT = 8
@@ -129,6 +130,8 @@ class ScaledKVCache:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = pages, page_size, heads, dim
         self.block_tokens = page_size // blocks
+        if dim % 8 or not 8 <= dim <= 256 or page_size > 4096 or self.block_tokens > 256 or heads > 128:
+            _invalid("head_dim must be a multiple of 8 in [8, 256]; page_size at most 4096, block_tokens 256, num_kv_heads 128")
         self.kv_format = _FORMATS[k_codes.dtype]
         strides = lambda c: [max(1, s) for s in c.stride()[:3]]  # noqa: E731  (a dimension of one may have any)
         self._desc = ScaledCacheDesc(self.kv_format, pages, page_size, heads, dim, self.block_tokens,
@@ -195,13 +198,13 @@ class ScaledKVCache:
         token's place in its request).  ``q_out`` may be ``q``.  ``token_counts`` ``[num_pages]``
         receives the tokens that the touched pages hold (what :meth:`attend_pages` reads).
         """
-        batch = seq_lens.shape[0]
-        tokens, heads, dim = k.shape[0], self.num_kv_heads, self.head_dim
-        kp = self._rows("k", k, None, (tokens, heads, dim))
+        lens = self._ints("seq_lens", seq_lens)
+        batch, heads, dim = seq_lens.shape[0], self.num_kv_heads, self.head_dim
+        kp = self._rows("k", k, None, (*k.shape[:1], heads, dim))
+        tokens = k.shape[0]
         vp = self._rows("v", v, k.dtype, (tokens, heads, dim))
         table, stride = self._table(page_table, batch)
         offsets = None if token_offsets is None else self._ints("token_offsets", token_offsets, batch + 1)
-        lens = self._ints("seq_lens", seq_lens)
         cos = sin = None
         places = turned = pairs = 0
         if rotary is not None:
@@ -228,23 +231,25 @@ class ScaledKVCache:
             _invalid("q_out needs q")
         counts = None if token_counts is None else self._ints("token_counts", token_counts, self.num_pages)
         k_stride, v_stride = k.stride(), v.stride()
-        args = _APPEND_ARGS.pack(
-            _TYPES[k.dtype], batch, tokens, page_table.shape[1], kp or 0, vp or 0, k_stride[0], k_stride[1], v_stride[0],
-            v_stride[1], offsets or 0, lens or 0, table or 0, stride, cos or 0, sin or 0, at or 0, places, turned, pairs,
-            q_heads, qp or 0, op or 0, q_stride[0], q_stride[1], out_stride[0], out_stride[1], counts or 0, self._status_at)
+        try:
+            args = _APPEND_ARGS.pack(
+                _TYPES[k.dtype], batch, tokens, page_table.shape[1], kp or 0, vp or 0, k_stride[0], k_stride[1], v_stride[0],
+                v_stride[1], offsets or 0, lens or 0, table or 0, stride, cos or 0, sin or 0, at or 0, places, turned, pairs,
+                q_heads, qp or 0, op or 0, q_stride[0], q_stride[1], out_stride[0], out_stride[1], counts or 0, self._status_at)
+        except _UNFIT as e:
+            _invalid(f"a size does not fit: {e}")
         _check(self.lib.dsd_scaled_append(self._index, self._desc_at, args, _raw_stream(self._index)))
         return q_out
 
     def _attend(self, q, table, lens, q_offsets, counts, scale, causal, window, out, return_lse):
-        batch = lens.shape[0]
-        rows, heads = q.shape[0], q.shape[1]
+        lens_at = self._ints("lens", lens)
         qp = self._rows("q", q)
+        batch, rows, heads = lens.shape[0], q.shape[0], q.shape[1]
         if out is None:
             out = torch.empty_like(q)
             op = out.data_ptr()
         else:
             op = self._rows("out", out, q.dtype, q.shape)
-        lens_at = self._ints("lens", lens)
         table_at, stride = self._table(table, batch)
         offsets = None if q_offsets is None else self._ints("q_offsets", q_offsets, batch + 1)
         held = None if counts is None else self._ints("page_counts", counts, self.num_pages)
@@ -258,10 +263,13 @@ class ScaledKVCache:
         # a new block each call: torch orders its reuse by stream, and a captured graph keeps its own
         work = self.status.new_empty((need + 3) // 4)
         q_stride, out_stride = q.stride(), out.stride()
-        args = _ATTENTION_ARGS.pack(
-            _TYPES[q.dtype], batch, rows, heads, qp or 0, op or 0, lse.data_ptr() if return_lse else 0, q_stride[0], q_stride[1],
-            out_stride[0], out_stride[1], offsets or 0, lens_at or 0, table_at or 0, stride, held or 0, table.shape[1], scale,
-            causal, min(window, 0x7fffffff), work.data_ptr() or 0, need, self._status_at)
+        try:
+            args = _ATTENTION_ARGS.pack(
+                _TYPES[q.dtype], batch, rows, heads, qp or 0, op or 0, lse.data_ptr() if return_lse else 0, q_stride[0],
+                q_stride[1], out_stride[0], out_stride[1], offsets or 0, lens_at or 0, table_at or 0, stride, held or 0,
+                table.shape[1], scale, causal, min(window, 0x7fffffff), work.data_ptr() or 0, need, self._status_at)
+        except _UNFIT as e:
+            _invalid(f"scale, window or a size does not fit: {e}")
         _check(self.lib.dsd_scaled_attention(self._index, self._desc_at, args, _raw_stream(self._index)))
         return (out, lse) if return_lse else out
 

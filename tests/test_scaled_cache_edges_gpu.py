@@ -269,3 +269,33 @@ def test_check_waits_for_every_stream_and_names_all_it_met(torch, dsd):
     with pytest.raises(dsd.OutOfRange, match="page"):
         s.cache.check()
     s.cache.check()
+
+
+def test_refusals_of_shapes_and_numbers(torch, dsd):
+    """What cannot be an argument is refused as one, not by an error of the binding's inside."""
+    s = Setup(torch, dsd, "fp8", [20, 20], 64, 2, 16, seed=60)
+    c = s.cache
+    k = torch.randn(2, 2, 64, device="cuda").half()
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    one = torch.tensor(1, dtype=torch.int32, device="cuda")
+    codes, scales = torch.zeros(2, 16, 2, 12, dtype=torch.int8, device="cuda"), torch.ones(2, 2, 1, device="cuda")
+    for call in (
+            lambda: c.attend(q, s.d_table, s.d_lens, scale=1e300),
+            lambda: c.attend(q, s.d_table, s.d_lens, window=2.0),
+            lambda: c.attend(q, s.d_table, s.d_lens, window=-2 ** 40),
+            lambda: c.attend(q, s.d_table, one),
+            lambda: c.attend(one, s.d_table, s.d_lens),
+            lambda: c.attend(q, one, s.d_lens),
+            lambda: c.attend(q, s.d_table, s.d_lens, out=torch.empty_like(q)[:, :1].expand(2, 4, 64)),
+            lambda: c.append(k, k, s.d_table, one),
+            lambda: c.append(one, k, s.d_table, s.d_lens),
+            lambda: c.append(k, k, s.d_table, s.d_lens, q=one),
+            lambda: c.append(k, k, s.d_table, s.d_lens, q=q, q_out=q[:1].expand(2, 4, 64)),
+            lambda: dsd.ScaledKVCache(1, 512, 2, 64),
+            lambda: dsd.ScaledKVCache(1, 8192, 2, 64, block_tokens=16),
+            lambda: dsd.ScaledKVCache(1, 16, 129, 64),
+            lambda: dsd.ScaledKVCache.from_tensors(codes, codes, scales, scales),
+    ):
+        with pytest.raises(dsd.InvalidArgument):
+            call()
+    c.check()
