@@ -46,11 +46,13 @@ def build_library(force: bool = False, verbose: bool = False, out: str = LIB,
     if verbose:
         flags.insert(0, "-Xptxas=-v")
     objects, jobs = [], []
-    os.makedirs(os.path.join(PKG, "build"), exist_ok=True)
+    # objects of another library or with other defines lie beside it: never linked into this one
+    at = os.path.join(PKG, "build") if out == LIB and not defines else os.path.abspath(out) + ".build"
+    os.makedirs(at, exist_ok=True)
     for src in SOURCES:
         deps = [os.path.join(CSRC, src), os.path.join(INCLUDE, "dsd_b200.h")]
         deps += [os.path.join(CSRC, h) for h in HEADERS if ONLY.get(h, src) == src]
-        obj = os.path.join(PKG, "build", os.path.basename(out) + "." + src + ".o")
+        obj = os.path.join(at, os.path.basename(out) + "." + src + ".o")
         objects.append(obj)
         if force or defines or not _newer(obj, deps):
             cmd = [NVCC, *flags, "-c", "-o", obj, os.path.join(CSRC, src)]
