@@ -59,9 +59,8 @@ def build_library(force: bool = False, verbose: bool = False, out: str = LIB,
             if verbose:
                 print(" ".join(cmd))
             jobs.append((cmd, subprocess.Popen(cmd)))
-    for cmd, job in jobs:
-        if job.wait():
-            raise subprocess.CalledProcessError(job.returncode, cmd)
+    for failed in [(job.returncode, cmd) for cmd, job in jobs if job.wait()]:   # all have ended by then
+        raise subprocess.CalledProcessError(*failed)
     if jobs or not _newer(out, objects):
         subprocess.run([NVCC, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", out, *objects], check=True)
     return out

@@ -19,6 +19,8 @@ while [ $# -gt 0 ]; do
   esac
   shift
 done
+[ -n "$FAIL" ] && case "$src" in *"$FAIL"*) exit 3;; esac
+[ -n "$FAIL" ] && sleep 0.5
 if [ -n "$compile" ]; then echo "$(basename $src)$d" > "$out"; else cat $inputs > "$out"; fi
 """
 
@@ -50,3 +52,12 @@ def test_objects_with_defines_stay_out_of_other_libraries(build, tmp_path):
     # experiments under the library's own name are not taken for it afterwards
     build.build_library(out=build.LIB, defines=("X=3",))
     assert "-D" not in open(build.build_library(out=build.LIB, force=True)).read()
+
+
+def test_a_build_that_fails_ends_its_other_compilers_first(build, monkeypatch):
+    import subprocess
+    monkeypatch.setenv("FAIL", build.SOURCES[0])
+    with pytest.raises(subprocess.CalledProcessError):
+        build.build_library(out=build.LIB)
+    objects = os.path.join(build.PKG, "build", os.path.basename(build.LIB) + "." + build.SOURCES[1] + ".o")
+    assert os.path.exists(objects) and not os.path.exists(build.LIB)
