@@ -299,3 +299,21 @@ def test_refusals_of_shapes_and_numbers(torch, dsd):
         with pytest.raises(dsd.InvalidArgument):
             call()
     c.check()
+
+
+@pytest.mark.parametrize("fmt,dtype", [("fp8", "bf16"), ("int8", "bf16"), ("fp8", "f32"), ("int8", "f32")])
+@pytest.mark.parametrize("D,H,new", [(64, 2, None), (64, 8, None), (64, 64, None), (64, 2, [150, 40]), (72, 8, [9, 20])])
+@pytest.mark.parametrize("kind", ["least", "both ends", "largest late"])
+def test_value_scales_at_the_ends_of_their_range(torch, dsd, fmt, dtype, D, H, new, kind):
+    """Scales of 0 and from 2^-64 to 2^36 keep outputs and the softmax sum, alone and together."""
+    s = Setup(torch, dsd, fmt, [400, 140], D, 2, 16, bt=1, seed=61, spread=0.3)
+    v = s.pool.scales["v"]
+    v[:] = np.float32(2.0 ** -64)
+    if kind == "both ends":
+        v[::2, :, 1::5], v[1::2, :, 2::5], v[:, :, 3::7] = np.float32(2.0 ** 36), 1, 0
+    elif kind == "largest late":
+        for b, n in enumerate(s.lens):
+            t = n - 45 if new else n - 1
+            v[s.table[b, t // 16], :, t % 16] = np.float32(2.0 ** 36)
+    upload(torch, s)
+    attend(torch, s, H, new, dtype)
