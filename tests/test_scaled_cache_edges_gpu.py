@@ -317,3 +317,30 @@ def test_value_scales_at_the_ends_of_their_range(torch, dsd, fmt, dtype, D, H, n
             v[s.table[b, t // 16], :, t % 16] = np.float32(2.0 ** 36)
     upload(torch, s)
     attend(torch, s, H, new, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("fp8", "bf16"), ("int8", "f16")])
+@pytest.mark.parametrize("D", [16, 32, 48, 112])
+@pytest.mark.parametrize("P,bt", [(8, 2), (24, 3), (264, 33)])
+def test_many_rows_at_other_head_dims_and_pages(torch, dsd, fmt, dtype, D, P, bt):
+    s = Setup(torch, dsd, fmt, [310, 77], D, 2, P, bt=bt, seed=62, spread=0.5)
+    attend(torch, s, 4, [70, 40], dtype, window=120)
+
+
+@pytest.mark.parametrize("D,P", [(128, 16), (72, 6)])
+def test_a_page_listed_twice_counts_twice(torch, dsd, D, P):
+    s = Setup(torch, dsd, "fp8", [3 * P], D, 2, P, seed=63)
+    a, b = int(s.table[0, 0]), int(s.table[0, 1])
+    counts = np.full(s.pool.pages, P, np.int32)
+    q = torch.randn(1, 4, D, device="cuda").bfloat16()
+
+    def pages(ids):
+        return s.cache.attend_pages(q, torch.tensor([ids], dtype=torch.int32, device="cuda"),
+                                    torch.tensor([len(ids)], dtype=torch.int32, device="cuda"), torch.from_numpy(counts).cuda(),
+                                    return_lse=True)
+
+    out, lse = pages([a, b, a])
+    want, wl = o.attend_pages(s.pool, f32(q), [a, b, a], counts, D ** -0.5)
+    assert np.abs(f32(out) - want).max() <= 2.0 ** -8 * np.abs(want).max() + 2.0 ** -9 * np.abs(want).max()
+    assert np.abs(f32(lse) - wl).max() <= 2.0 ** -16 * np.maximum(1, np.abs(wl)).max()
+    s.cache.check()
