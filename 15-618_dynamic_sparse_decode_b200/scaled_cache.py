@@ -200,8 +200,8 @@ class ScaledKVCache:
         """
         lens = self._ints("seq_lens", seq_lens)
         batch, heads, dim = seq_lens.shape[0], self.num_kv_heads, self.head_dim
-        kp = self._rows("k", k, None, (*k.shape[:1], heads, dim))
-        tokens = k.shape[0]
+        tokens = k.shape[0] if k.dim() else 0
+        kp = self._rows("k", k, None, (tokens, heads, dim))
         vp = self._rows("v", v, k.dtype, (tokens, heads, dim))
         table, stride = self._table(page_table, batch)
         offsets = None if token_offsets is None else self._ints("token_offsets", token_offsets, batch + 1)
