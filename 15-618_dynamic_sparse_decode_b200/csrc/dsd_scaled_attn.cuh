@@ -7,6 +7,10 @@
 // token for the dot products (its 8-bit key row against the R query rows in
 // shared memory) and one or two output elements for the weighted sum (value codes
 // of a token are adjacent across the threads).
+//
+// Bound: byte loads, one dependent key row a thread.  64 requests of 1024-4096 tokens,
+// 32 heads over 8: 2.7 ms at head_dim 256 (floor 102 us), 2.05 ms with pages of one
+// token (floor 57 us); the tensor-core kernels do that batch in 79 us at head_dim 128.
 #pragma once
 
 #include "dsd_scaled_common.cuh"

@@ -17,11 +17,11 @@
 // with 8 query rows per key head, S and O have 24 of their up to 256 columns.
 //
 // Bound: HBM.  64 requests of 16-32k tokens, 32 heads over 8, token-major pages of
-// 32: 0.505 ms, 6.4 TB/s (0.98 of the measured copy rate; head-major 6.58 TB/s);
-// about 20 us of every call are its start, the tail of its ranges and the join, so
-// smaller calls reach less.  Two CTAs per SM with three stages each; three CTAs with
-// two stages measured the same for 1 or 2 rows and a fifth slower for 4 (80
-// registers).
+// 32: 0.50-0.52 ms, 6.2-6.4 TB/s (0.94-0.98 of the measured copy rate).  Some 20 us of
+// a call are its plan (2.5), a CTA's first tile (4-5), the spread of the ranges' ends
+// (5-11) and the join (4-9), so smaller calls reach less.  Two CTAs per SM with three
+// stages each, two stages for 8 rows of four pieces or more; three CTAs with two stages
+// measured the same for 1 or 2 rows and a fifth slower for 4 (80 registers).
 //
 // Roles: warps 0-3 softmax (thread = token for S^T, = element d for O^T), warp 4
 // TMA, warp 5 MMA issue, warp 6 token data (page, scales, masks of a tile), warp 7

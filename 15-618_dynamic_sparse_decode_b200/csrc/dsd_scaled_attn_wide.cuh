@@ -31,7 +31,7 @@
 // quarter each came out at 766 us.
 //
 // Bound: the softmax warps' latency (the tensor cores are 20% busy, ex2 21%); three
-// requests of 300-700 queries over 5000-9000 tokens, 32 heads over 8: 0.49 ms, 484
+// requests of 300-700 queries over 5000-9000 tokens, 32 heads over 8: 0.50-0.51 ms, 467
 // TFLOP/s of the 1679 a bf16 product reaches.
 //
 // Roles: warps 0-7 softmax, 8-11 widen the codes, 12 TMA, 13 MMA issue, 14 token

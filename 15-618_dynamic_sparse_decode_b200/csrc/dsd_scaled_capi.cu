@@ -168,8 +168,9 @@ void Append(int device, const dsd_scaled_cache* c, const dsd_scaled_append_args*
   if (a->num_q_heads)
     CheckWritten(c->head_dim, {{a->total_tokens, a->q_out_stride[0]}, {a->num_q_heads, a->q_out_stride[1]}}, "q_out");
 
-  // 8-element accesses where every row starts on their boundary, else single
-  // elements (measured on unaligned rows only: no other path takes those)
+  // 8-element accesses where every row, and each half of its rotated part, starts on
+  // their boundary, else single elements (7400 tokens of bf16, 32 + 2 x 8 heads of 96:
+  // rotary_dim 32 23 us, rotary_dim 24 96 us)
   const int rd = a->cos ? a->rotary_dim : 0;
   bool wide = rd % 16 == 0;
   for (int i = 0; i < 4; ++i)

@@ -195,7 +195,8 @@ class ScaledKVCache:
         ``token_offsets[b] : token_offsets[b + 1]`` (None: one token for each request).
         ``seq_lens`` counts each request's tokens with the new ones; ``page_table`` ``[batch,
         pages]`` lists its pages.  ``rotary`` turns keys and queries by ``positions`` (None: the
-        token's place in its request).  ``q_out`` may be ``q``.  ``token_counts`` ``[num_pages]``
+        token's place in its request).  ``q_out`` may be ``q``; the rows of tokens that are left out (a
+        bad position or length, behind the last request) keep what it held, and mean nothing in a fresh one.  ``token_counts`` ``[num_pages]``
         receives the tokens that the touched pages hold (what :meth:`attend_pages` reads).
         """
         lens = self._ints("seq_lens", seq_lens)
@@ -291,7 +292,8 @@ class ScaledKVCache:
         ``q`` ``[queries, num_q_heads, head_dim]``: request b's are rows ``q_offsets[b] :
         q_offsets[b + 1]`` (None: one query for each request), its last tokens.  ``scale`` defaults
         to ``head_dim ** -0.5``.  ``window`` > 0 lets a query see that many tokens, itself
-        included.  A query that sees nothing gets zeros and -inf.  Returns ``out`` or
+        included.  A query that sees nothing gets zeros and -inf; rows behind the last request's stay as
+        they are in ``out`` and mean nothing in a fresh one.  Returns ``out`` or
         ``(out, lse)``, lse float32 ``[queries, num_q_heads]``.
         """
         return self._attend(q, page_table, seq_lens, q_offsets, None, scale, causal, window, out, return_lse)

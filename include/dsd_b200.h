@@ -348,7 +348,9 @@ int dsd_decode_batch_noalloc(int device, const dsd_model_config* config, int cap
  * p*stride[0] + t*stride[1] + h*stride[2] + d of k_codes / v_codes; strides are
  * positive, so pages may hold token-major or head-major rows and K and V may be
  * interleaved.  Scales are [num_pages][num_kv_heads][page_size / block_tokens],
- * finite and >= 0. */
+ * finite and >= 0.  The attention takes value scales of 0 and from 2^-64 to 2^36, any of
+ * them in one row: a smaller one counts as 2^-64 with few bits left or none, and larger
+ * ones may push tokens with small scales out of the softmax sum. */
 typedef struct dsd_scaled_cache {
   int32_t kv_format;      /* DSD_KV_FP8_SCALED or DSD_KV_I8_SCALED */
   int32_t num_pages;
@@ -385,9 +387,8 @@ typedef struct dsd_scaled_cache {
  * 2^-100; whatever the scale array held is ignored).  A block that holds older
  * tokens keeps its scale unless the new tokens need a larger one; then the older
  * codes are rounded again to the larger scale.  code = round-to-nearest-even(
- * value * (1/scale)), saturating; infinities saturate (a block whose scale is 0
- * reads them as 0), NaN is stored as NaN
- * (e4m3) or 0 (int8).
+ * value * (1/scale)), saturating; infinities saturate (a block whose scale is 0 reads
+ * them as 0), NaN is stored as NaN (e4m3) or 0 (int8).
  *
  * A token whose page, position or length is bad is left out (its status bit is
  * set) and nothing outside the arrays is touched.  Offsets that descend set
@@ -427,7 +428,12 @@ typedef struct dsd_scaled_append_args {
 int dsd_scaled_append(int device, const dsd_scaled_cache* cache,
                       const dsd_scaled_append_args* args, void* stream);
 
-/* dsd_scaled_attention: softmax(scale * q.k) v over the cache in fp32.
+/* dsd_scaled_attention: softmax(scale * q.k) v over the cache.  Logits, the softmax and
+ * its sums are fp32.  Operands of the tensor cores have fewer bits: of a 16-bit query
+ * row, elements near its largest keep all, smaller ones an absolute 2^-20 of that; a
+ * weight times its value scale keeps 11 bits for 16-bit rows (two such pieces for fp16
+ * rows beyond 16 query rows per key head) and an absolute 2^-19 of the row's largest
+ * below; fp32 rows keep 22 bits and more.
  *
  * Request b's queries are rows q_offsets[b] .. q_offsets[b+1] of q / out / lse
  * (q_offsets NULL: one query per request, row b).  Two ways to name its tokens:
@@ -437,7 +443,8 @@ int dsd_scaled_append(int device, const dsd_scaled_cache* cache,
  *    of those (without `causal`: tokens from lens[b] - n + j - window + 1 on).
  *  page_counts != NULL: lens[b] is the number of pages its row lists, in any
  *    order (the pages a selection picked), and a listed page p holds
- *    min(page_counts[p], page_size) tokens; causal and window must be 0.
+ *    min(page_counts[p], page_size) tokens; causal and window must be 0.  A page that
+ *    is listed twice counts twice.
  * A query that sees no token gets zeros and lse = -inf.  Rows behind the last
  * request's are left as they were.  A listed page outside [0, num_pages) counts
  * as masked and sets the status bit.
