@@ -186,7 +186,7 @@ constexpr int kWideSpread = 8;   // log2 of how far a tile's value scales may li
 
 // A tile's tokens as the softmax reads them, four at a time.
 struct __align__(16) Columns {   // its size too: float4 reads of the second one
-  float ks[kTile], vs[kTile], bound[kTile];
+  float ks[kTile], vs[kTile], bound[kTile];   // bound: scale_bound(vs), with one piece
   uint32_t valid[4];   // a bit per token
   int largest[4], least[4];   // bounding exponents of each 32 tokens' value scales
   int place, open;     // open: every row sees every token that is there
@@ -449,7 +449,7 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
       Columns& c = cols[cb];
       c.ks[t] = valid ? scales.x : 0.0f;
       c.vs[t] = vs;
-      c.bound[t] = float(scale_bound(vs));
+      if constexpr (PP == 1) c.bound[t] = static_cast<float>(scale_bound(vs));
       if (lane == 0) {
         c.valid[t >> 5] = present;
         c.largest[t >> 5] = largest;
@@ -612,7 +612,14 @@ attn_wide_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ C
                 unpair(mul2(pair(raw[2 * j], raw[2 * j + 1]), j & 1 ? k[j / 2].y : k[j / 2].x), a, b);
                 const bool see_a = (there >> (2 * j) & 1) && 2 * j <= hi && 2 * j >= lo;
                 const bool see_b = (there >> (2 * j + 1) & 1) && 2 * j + 1 <= hi && 2 * j + 1 >= lo;
-                const float2 bound = *reinterpret_cast<const float2*>(&c.bound[at + 2 * j]);
+                // from shared memory chunks take 507 us, made here 517; with two pieces 576 and 562
+                float2 bound;
+                if constexpr (PP == 1) {
+                  bound = *reinterpret_cast<const float2*>(&c.bound[at + 2 * j]);
+                } else {
+                  unpair(j & 1 ? v[j / 2].y : v[j / 2].x, bound.x, bound.y);
+                  bound = make_float2(static_cast<float>(scale_bound(bound.x)), static_cast<float>(scale_bound(bound.y)));
+                }
                 t[j & 3] = fmaxf(t[j & 3], fmaxf(see_a ? fmaf(a, factor, bound.x) : -INFINITY,
                                                  see_b ? fmaf(b, factor, bound.y) : -INFINITY));
                 const uint64_t w = pair(see_a ? ex2(fmaf(a, factor, -r)) : 0.0f, see_b ? ex2(fmaf(b, factor, -r)) : 0.0f);

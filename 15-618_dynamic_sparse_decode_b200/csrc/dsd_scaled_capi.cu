@@ -290,7 +290,7 @@ constexpr int kTcMaxRows = 8;   // query rows of a narrow unit
 // one widens each tile once whatever the rows.  64 requests of 1024-4096 tokens, 4 key
 // heads, bf16, narrow / wide: 12 rows 88 / 115 us, 16 rows 90 / 115, 20 rows 129 / 124,
 // 24 rows 127 / 117, 28 rows 163 / 128, 48 rows 237 / 131; int8 at 16 rows 88 / 119, at
-// 24 124 / 137, at 28 153 / 137; fp16 98 / 149, 129 / 144 and 164 / 155.  Between 16 and
+// 24 124 / 137, at 28 153 / 137; fp16 98 / 146, 130 / 141 and 167 / 151.  Between 16 and
 // 24 the two are near one another, unless a chunk stands among single tokens: with 63
 // of those, one of 100 queries (12 rows) 174 / 243, one of 320 (24 rows) 325 / 268.
 constexpr int kNarrowMaxRows = 16;
