@@ -350,7 +350,9 @@ int dsd_decode_batch_noalloc(int device, const dsd_model_config* config, int cap
  * interleaved.  Scales are [num_pages][num_kv_heads][page_size / block_tokens],
  * finite and >= 0.  The attention takes value scales of 0 and from 2^-64 to 2^36, any of
  * them in one row: a smaller one counts as 2^-64 with few bits left or none, and larger
- * ones may push tokens with small scales out of the softmax sum. */
+ * ones may push tokens with small scales out of the softmax sum.  A scale of 0 counts
+ * as 2^-64 too where weights are rounded: beside such a token, outputs below 2^-80 may
+ * come out as 0. */
 typedef struct dsd_scaled_cache {
   int32_t kv_format;      /* DSD_KV_FP8_SCALED or DSD_KV_I8_SCALED */
   int32_t num_pages;
